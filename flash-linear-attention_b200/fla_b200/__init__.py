@@ -15,9 +15,9 @@ __version__ = "0.1.0"
 
 
 def install_as_fla_ops():
-    """Alias `fla.ops.{gla,simple_gla,retention,delta_rule,gated_delta_rule}` to this package."""
+    """Alias `fla.ops.{gla,simple_gla,retention,delta_rule,gated_delta_rule,hgrn}` to this package."""
     from . import ops
-    from .ops import delta_rule, gated_delta_rule, gla, retention, simple_gla
+    from .ops import delta_rule, gated_delta_rule, gla, hgrn, retention, simple_gla
     root = sys.modules.get("fla")
     if root is None:
         root = types.ModuleType("fla")
@@ -26,7 +26,7 @@ def install_as_fla_ops():
     sys.modules["fla.ops"] = ops
     root.ops = ops
     for name, mod in (("gla", gla), ("simple_gla", simple_gla), ("retention", retention),
-                      ("delta_rule", delta_rule), ("gated_delta_rule", gated_delta_rule)):
+                      ("delta_rule", delta_rule), ("gated_delta_rule", gated_delta_rule), ("hgrn", hgrn)):
         sys.modules[f"fla.ops.{name}"] = mod
 
 

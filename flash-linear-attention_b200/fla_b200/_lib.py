@@ -7,6 +7,7 @@ without the built library raises immediately with the build command.
 
 import ctypes
 import os
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -108,6 +109,13 @@ def load() -> ctypes.CDLL:
     lib.flab_gdn_gate_fwd.argtypes = [ap, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.flab_gdn_gate_bwd.restype = ci
     lib.flab_gdn_gate_bwd.argtypes = [ap, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    sz = ctypes.c_size_t
+    lib.flab_hgrn_workspace.restype = sz
+    lib.flab_hgrn_workspace.argtypes = [ci, ll, ci]
+    lib.flab_hgrn_fwd.restype = ci
+    lib.flab_hgrn_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ll, ci, ci, ci, vp, sz, vp]
+    lib.flab_hgrn_bwd.restype = ci
+    lib.flab_hgrn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ll, ci, ci, ci, vp, sz, vp]
     lib.flab_state_chain.restype = ci
     lib.flab_state_chain.argtypes = [vp, vp, ll, vp, vp, vp, ci, ci, ci, ci, ci, ci, vp]
     _lib = lib
@@ -162,6 +170,21 @@ def call(entry: str, ref: torch.Tensor, **kw):
         rc = getattr(lib, entry)(ctypes.byref(a), ctypes.c_void_p(stream))
     if rc != 0:
         raise RuntimeError(f"{entry} failed ({rc}): {lib.flab_last_error().decode()}")
+    global LAUNCHES
+    LAUNCHES += 1
+    if CHECK_EVERY_CALL:
+        check_device_waits(entry)
+
+
+def device_of(t: torch.Tensor):
+    """Context in which `t`'s device is the current one; nothing to enter where it already is."""
+    return nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+
+def finish(entry: str, rc: int) -> None:
+    """What follows every call of an entry point with plain arguments: the error of a refused one, the count of a good one."""
+    if rc != 0:
+        raise RuntimeError(f"{entry} failed ({rc}): {load().flab_last_error().decode()}")
     global LAUNCHES
     LAUNCHES += 1
     if CHECK_EVERY_CALL:

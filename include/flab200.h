@@ -256,6 +256,21 @@ int flab_recurrent_delta_fwd(const flab_args *a, void *stream);
  * v, beta, h0, d_o, dht; writes dq, dk, dv (fp32), dbeta (fp32), dh0. */
 int flab_recurrent_delta_bwd(const flab_args *a, void *stream);
 
+/* ---- element-wise gated linear recurrence ------------------------------------------------------
+ * Replaces chunk_hgrn / fused_recurrent_hgrn (fla/ops/hgrn/chunk.py, fused_recurrent.py), forward and backward:
+ *   h_t = e^{g_t} h_{t-1} + x_t, o_t = h_t;   c_t = e^{g_t} (do_t + c_{t+1}), dx_t = do_t + c_{t+1}, dg_t = c_t h_{t-1}.
+ * x, g, o, d_o, dx, dg: [B, T, D] contiguous of element type dtype. h0 (h before a sequence) and dht (gradient of its last h)
+ * fp32 [N, D] or NULL (zeros); ht (its last h) and dh0 (c at its first token) fp32 [N, D] or NULL (not wanted).
+ * cu_seqlens NULL: N = B sequences of T tokens. Otherwise B = 1 and cu_seqlens holds the N + 1 cumulative lengths on the device
+ * (int32, or int64 with cu_is_int64); empty sequences pass h0 to ht (dht to dh0), and rows of no sequence get zeros.
+ * Scratch: ws, 16-byte aligned, of flab_hgrn_workspace(B, T, D) bytes (0: ws may be NULL); its contents need no preparation.
+ * Blocks wait for earlier blocks of the same launch, with a bound: flab_tc_check() reports a wait that ran out. */
+size_t flab_hgrn_workspace(int B, long long T, int D);
+int flab_hgrn_fwd(const void *x, const void *g, const float *h0, void *o, float *ht, const void *cu_seqlens, int cu_is_int64, int B, long long T,
+                  int D, int N, int dtype, void *ws, size_t ws_bytes, void *stream);
+int flab_hgrn_bwd(const void *g, const void *o, const float *h0, const void *d_o, const float *dht, void *dx, void *dg, float *dh0,
+                  const void *cu_seqlens, int cu_is_int64, int B, long long T, int D, int N, int dtype, void *ws, size_t ws_bytes, void *stream);
+
 /* ---- whole-forward entry points --------------------------------------------------------------
  * Replaces chunk_gated_delta_rule_fwd (fla/ops/gated_delta_rule/chunk.py:20-73): the four stages
  * (gate cumsum, WY factors, state scan, output) enqueued by one call. Reads q, k, v, g (the RAW fp32
