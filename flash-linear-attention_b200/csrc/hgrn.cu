@@ -42,10 +42,9 @@ struct HgrnParams {
   int B, D, N;
   int nT, nCG;       // tiles along time, channel groups
   long long T;
-  int *flags;        // [tiles] 1: the tile's map is there; null with one tile along time
   int *ticket;
-  float2 *maps;      // [tiles][C] (P, Q)
-  unsigned long long *ends;  // [groups][C] end value and mark
+  unsigned long long *maps;  // [tiles][C] words; null with one tile along time
+  unsigned long long *ends;  // [groups][C] words
 };
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
@@ -77,46 +76,36 @@ __device__ __forceinline__ bool is_cut(float P) { return __float_as_uint(P) == 0
 // y = P c + Q.  A zero start stays out of the product, so that a P that overflowed (gates above 0) makes no NaN of it.
 __device__ __forceinline__ float through(float P, float Q, float c) { return c == 0.f || is_cut(P) ? Q : fmaf(P, c, Q); }
 
-__device__ __forceinline__ int load_acquire(const int *a) {
-  int v;
-  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(a) : "memory");
-  return v;
+// What tiles tell each other goes in words of 64 bits that hold a value and the mark that it is there, stored and loaded
+// relaxed: whoever sees the mark has the value.  (A flag behind a fence was measured at 4000 cycles a tile under load.)  The
+// words are cleared before the launch.
+__device__ __forceinline__ unsigned long long end_word(float v) { return (1ull << 32) | __float_as_uint(v); }
+__device__ __forceinline__ float end_of(unsigned long long w) { return __uint_as_float((unsigned)w); }
+// A map: P's bits plus one are never 0 (the one pattern that would be, a NaN, is not what arithmetic makes of a NaN).
+__device__ __forceinline__ unsigned long long map_word(float P, float Q) {
+  return ((unsigned long long)(__float_as_uint(P) + 1u) << 32) | __float_as_uint(Q);
 }
-__device__ __forceinline__ void store_release(int *a, int v) {
-  asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(a), "r"(v) : "memory");
+__device__ __forceinline__ float2 map_of(unsigned long long w) { return make_float2(__uint_as_float((unsigned)(w >> 32) - 1u), __uint_as_float((unsigned)w)); }
+__device__ __forceinline__ void put(unsigned long long *a, unsigned long long w) {
+  asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(a), "l"(w) : "memory");
 }
-// Bounded wait for a tile's flag: about a second; once any wait has run out, no further one waits.
-__device__ __forceinline__ int wait_flag(const int *a) {
-  int v = load_acquire(a);
-  if (v) return v;
+__device__ __forceinline__ unsigned long long look(const unsigned long long *a) {
+  unsigned long long w;
+  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(a) : "memory");
+  return w;
+}
+// Bounded wait for a word's mark, about a second; once any wait has run out, no further one waits.
+__device__ __forceinline__ unsigned long long await(const unsigned long long *a, unsigned long long w) {
+  if (w >> 32) return w;
   const long long t0 = clock64();
   for (int spins = 1;; ++spins) {
-    v = load_acquire(a);
-    if (v) return v;
+    w = look(a);
+    if (w >> 32) return w;
     if ((spins & 255) == 0 && (clock64() - t0 > (1ll << 31) || *reinterpret_cast<volatile int *>(&tu_tc_error))) {
       tu_tc_error = 700;
-      return 0;
+      return map_word(0.f, 0.f);
     }
   }
-}
-
-// A group's end value and the mark that it is there, in one word of 64 bits: whoever sees the mark has the value.
-__device__ __forceinline__ void put_end(unsigned long long *a, float v) {
-  const unsigned long long word = (1ull << 32) | __float_as_uint(v);
-  asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(a), "l"(word) : "memory");
-}
-__device__ __forceinline__ float wait_end(const unsigned long long *a) {
-  unsigned long long v;
-  const long long t0 = clock64();
-  for (int spins = 1;; ++spins) {
-    asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(a) : "memory");
-    if (v >> 32) break;
-    if ((spins & 255) == 0 && (clock64() - t0 > (1ll << 31) || *reinterpret_cast<volatile int *>(&tu_tc_error))) {
-      tu_tc_error = 701;
-      break;
-    }
-  }
-  return __uint_as_float((unsigned)v);
 }
 
 template <typename T, int V, int W, int R, bool BWD, bool VAR>
@@ -129,7 +118,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
   __shared__ int sTile;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int tile = blockIdx.x;
-  if (p.flags) {
+  if (p.maps) {
     if (threadIdx.x == 0) sTile = atomicAdd(p.ticket, 1);
     __syncthreads();
     tile = sTile;
@@ -206,25 +195,21 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
   float c[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) c[j] = !VAR && step < G && edge && on ? edge[(size_t)b * p.D + ch + j] : 0.f;
-  if (p.flags) {
+  if (p.maps) {
     const int group = step / G, first = group * G, before = step - first;
     const bool leader = before == G - 1 && step + 1 < p.nT;  // hands the group's end on
     if (w == 0 && !leader) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float2 m = joined(j);
-        p.maps[((size_t)step * chains + chain) * C + lane * V + j] = m;
+        put(p.maps + ((size_t)step * chains + chain) * C + lane * V + j, map_word(m.x, m.y));
       }
-      __threadfence();
-      __syncwarp();
-      if (lane == 0) store_release(p.flags + (size_t)step * chains + chain, 1);
     }
     if (w < before) {  // W >= G - 1: a warp fetches one earlier tile's map
-      const size_t at = (size_t)(first + w) * chains + chain;
-      wait_flag(p.flags + at);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float2 m = __ldcg(p.maps + at * C + lane * V + j);
+        const unsigned long long *a = p.maps + ((size_t)(first + w) * chains + chain) * C + lane * V + j;
+        const float2 m = map_of(await(a, look(a)));
         lP[w][lane * V + j] = m.x;
         lQ[w][lane * V + j] = m.y;
       }
@@ -235,7 +220,10 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
     __syncthreads();
     if (group > 0) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) c[j] = wait_end(p.ends + ((size_t)(group - 1) * chains + chain) * C + lane * V + j);
+      for (int j = 0; j < V; ++j) {
+        const unsigned long long *a = p.ends + ((size_t)(group - 1) * chains + chain) * C + lane * V + j;
+        c[j] = end_of(await(a, look(a)));
+      }
     }
 #pragma unroll
     for (int i = 0; i < G - 1; ++i)
@@ -246,7 +234,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
     if (leader && w == 0) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        put_end(p.ends + ((size_t)group * chains + chain) * C + lane * V + j, through(own[j].x, own[j].y, c[j]));
+        put(p.ends + ((size_t)group * chains + chain) * C + lane * V + j, end_word(through(own[j].x, own[j].y, c[j])));
     }
   }
 #pragma unroll
@@ -311,6 +299,346 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
   }
 }
 
+// ---- the streaming form: one persistent block an SM, tiles by TMA ----------------------------------------------------
+// The same maps and order of sums, as a pipeline over S stages of shared memory whose warps meet only at mbarriers:
+//   load warp    takes a ticket and fetches the tile (rows and channels outside the tensor arrive as zeros: the identity map)
+//   map warps    compose the tile's rows, R to a warp, and wait for nothing outside the block
+//   chain warps  publish the tile's map, fetch what came before it and leave the start value of every R rows
+//   row warps    run the recurrence from there, outputs in place of inputs
+//   store warp   sends the tile off and hands the stage back
+// A tile's start value costs two or three trips to L2; the map warps being stages ahead of the row warps hides them, and keeps
+// several groups of a long chain in flight.  Gates are evaluated twice (map, rows): two more instructions an element, against
+// 64 registers a thread that would have to live through the wait.
+template <typename T> __device__ __forceinline__ float2 unpack2(const T *s) {
+  const Pack<T, 2> v = *reinterpret_cast<const Pack<T, 2> *>(s);
+  return make_float2(Num<T>::f(v.v[0]), Num<T>::f(v.v[1]));
+}
+template <typename T> __device__ __forceinline__ void pack2(T *s, float a, float b) {
+  Pack<T, 2> v;
+  v.v[0] = Num<T>::t(a), v.v[1] = Num<T>::t(b);
+  *reinterpret_cast<Pack<T, 2> *>(s) = v;
+}
+// e^g as 2^(g log2 e): the product's rounding moves the result by |g| 2^-24 of itself, less than the exponential's own error
+// wherever the gate is near 1 and errors live long.
+__device__ __forceinline__ float gate(float g) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(g * 1.4426950408889634f));
+  return y;
+}
+
+template <typename T, int R, int S, bool BWD> struct Stream {
+  static constexpr int V = 2, C = 32 * V, W = 8, L = W * R;
+  static constexpr int TILE = L * C, TENSORS = BWD ? 3 : 2;
+  // Chain warps, on tiles in turn.  Their number divides S, so that one warp sees every phase of a stage's barriers: a wait for
+  // a phase's parity says nothing to one that has not seen the phase before it.
+  static constexpr int CHAINS = S % 4 == 0 ? 4 : 3;
+  static_assert(S % CHAINS == 0, "a stage belongs to one chain warp");
+  static constexpr int THREADS = 32 * (2 * W + CHAINS + 2);
+  struct Stage {
+    T buf[TENSORS][TILE];   // x (do), g, o of a token earlier
+    float2 P[W][32], Q[W][32];  // the warps' maps; the start values take the place of P
+    int code[L];
+  };
+  struct Shared {
+    Stage st[S];
+    int tile[S], edges[S];
+    uint64_t full[S], mapped[S], ready[S], done[S], empty[S];
+  };
+};
+
+template <typename T, int R, int S, bool BWD, bool VAR>
+__global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
+    hgrn_stream_kernel(const HgrnParams p, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mg,
+                       const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap my, const __grid_constant__ CUtensorMap mz) {
+  typedef Stream<T, R, S, BWD> Z;
+  constexpr int W = Z::W, L = Z::L, C = Z::C;
+  constexpr int AHEAD = BWD ? ROW_END : ROW_START;  // the edge that a scan meets first
+  extern __shared__ __align__(128) char raw[];
+  typename Z::Shared &sh = *reinterpret_cast<typename Z::Shared *>(raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chains = p.B * p.nCG;
+  const long long tiles = (long long)chains * p.nT;
+  const float *const edge = BWD ? p.dht : p.h0;  // values in front of the sequences, in scan order
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      tc::mbar_init(&sh.full[s], 1);
+      tc::mbar_init(&sh.mapped[s], W);
+      tc::mbar_init(&sh.ready[s], 1);
+      tc::mbar_init(&sh.done[s], W);
+      tc::mbar_init(&sh.empty[s], 1);
+    }
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  struct Place {
+    int step, chain, b, cg, t0;
+  };
+  auto place = [&](int tile) {
+    Place z;
+    z.step = tile / chains;
+    z.chain = tile - z.step * chains;
+    z.b = z.chain / p.nCG;
+    z.cg = z.chain - z.b * p.nCG;
+    z.t0 = (BWD ? p.nT - 1 - z.step : z.step) * L;
+    return z;
+  };
+  // position r of warp w's rows is this row of the tile
+  auto row = [&](int w, int r) -> int { return BWD ? L - 1 - (w * R + r) : w * R + r; };
+
+  if (warp < W) {  // ---- map warps
+    const int w = warp;
+    for (int it = 0;; ++it) {
+      const int s = it % S;
+      if (!tc::mbar_wait(&sh.full[s], (it / S) & 1)) {
+        tu_tc_error = 702;
+        break;
+      }
+      const int tile = sh.tile[s];
+      if (tile < 0) break;
+      typename Z::Stage &st = sh.st[s];
+      const T *const xs = st.buf[0] + lane * 2, *const gs = st.buf[1] + lane * 2;
+      float2 P = make_float2(1.f, 1.f), Q = make_float2(0.f, 0.f);
+      auto take = [&](float2 g, float2 x) {
+        const float2 a = make_float2(gate(g.x), gate(g.y));
+        Q.x = BWD ? a.x * (Q.x + x.x) : fmaf(a.x, Q.x, x.x);
+        Q.y = BWD ? a.y * (Q.y + x.y) : fmaf(a.y, Q.y, x.y);
+        P.x *= a.x, P.y *= a.y;
+      };
+      if (!VAR || !sh.edges[s]) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) take(unpack2(gs + row(w, r) * C), unpack2(xs + row(w, r) * C));
+      } else {
+        const int ch = place(tile).cg * C + lane * 2;
+#pragma unroll 4
+        for (int r = 0; r < R; ++r) {
+          const int code = st.code[row(w, r)];
+          const bool out = code & ROW_OUT;
+          if (code & (ROW_OUT | AHEAD)) {
+            P = make_float2(CUT, CUT);
+            Q = out || !edge || ch >= p.D ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2 *>(edge + (size_t)(code >> ROW_SHIFT) * p.D + ch);
+          }
+          if (!out) take(unpack2(gs + row(w, r) * C), unpack2(xs + row(w, r) * C));
+        }
+      }
+      st.P[w][lane] = P;
+      st.Q[w][lane] = Q;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.mapped[s]);
+    }
+  } else if (warp < 2 * W) {  // ---- row warps
+    const int w = warp - W;
+    for (int it = 0;; ++it) {
+      const int s = it % S;
+      if (!tc::mbar_wait(&sh.full[s], (it / S) & 1)) {
+        tu_tc_error = 703;
+        break;
+      }
+      const int tile = sh.tile[s];
+      if (tile < 0) break;
+      if (!tc::mbar_wait(&sh.ready[s], (it / S) & 1)) {
+        tu_tc_error = 704;
+        break;
+      }
+      typename Z::Stage &st = sh.st[s];
+      const Place z = place(tile);
+      const int ch = z.cg * C + lane * 2;
+      const bool on = ch < p.D;
+      T *const xs = st.buf[0] + lane * 2, *const gs = st.buf[1] + lane * 2;
+      const T *const os = st.buf[BWD ? 2 : 0] + lane * 2;
+      float2 c = st.P[w][lane];
+      auto take = [&](int at, float2 g, float2 x, float2 h) {
+        const float2 a = make_float2(gate(g.x), gate(g.y));
+        if (!BWD) {
+          c.x = fmaf(a.x, c.x, x.x), c.y = fmaf(a.y, c.y, x.y);
+          pack2(xs + at, c.x, c.y);
+        } else {
+          const float2 d = make_float2(x.x + c.x, x.y + c.y);
+          c.x = a.x * d.x, c.y = a.y * d.y;
+          pack2(xs + at, d.x, d.y);
+          pack2(gs + at, c.x * h.x, c.y * h.y);
+        }
+      };
+      const float2 none = make_float2(0.f, 0.f);
+      if (!VAR || !sh.edges[s]) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int at = row(w, r) * C;
+          float2 h = BWD ? unpack2(os + at) : none;
+          // the first token's h_{t-1} (the load of it fell in front of the tensor and arrived as 0)
+          if (BWD && !VAR && r == R - 1 && w == W - 1 && z.t0 == 0 && p.h0 && on) h = *reinterpret_cast<const float2 *>(p.h0 + (size_t)z.b * p.D + ch);
+          take(at, unpack2(gs + at), unpack2(xs + at), h);
+        }
+      } else {
+#pragma unroll 2
+        for (int r = 0; r < R; ++r) {
+          const int at = row(w, r) * C, code = st.code[row(w, r)];
+          const size_t of = (size_t)(code >> ROW_SHIFT) * p.D + ch;
+          if (code & ROW_OUT) {
+            c = none;
+            pack2(xs + at, 0.f, 0.f);
+            if (BWD) pack2(gs + at, 0.f, 0.f);
+            continue;
+          }
+          if (code & AHEAD) c = edge && on ? *reinterpret_cast<const float2 *>(edge + of) : none;
+          float2 h = BWD ? unpack2(os + at) : none;
+          if (BWD && (code & ROW_START)) h = p.h0 && on ? *reinterpret_cast<const float2 *>(p.h0 + of) : none;
+          take(at, unpack2(gs + at), unpack2(xs + at), h);
+          if ((code & (BWD ? ROW_START : ROW_END)) && p.ht && on) *reinterpret_cast<float2 *>(p.ht + of) = c;
+        }
+      }
+      // rows past T are the identity, so the last warp's last value is the sequence's
+      if (!VAR && z.step == p.nT - 1 && w == W - 1 && p.ht && on) *reinterpret_cast<float2 *>(p.ht + (size_t)z.b * p.D + ch) = c;
+      if (VAR && p.ht && z.step == 0 && on) {  // empty sequences hand their edge value through
+        for (int n = w; n < p.N; n += W)
+          if (cu_at(p, n) >= cu_at(p, n + 1))
+            *reinterpret_cast<float2 *>(p.ht + (size_t)n * p.D + ch) = edge ? *reinterpret_cast<const float2 *>(edge + (size_t)n * p.D + ch) : none;
+      }
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.done[s]);
+    }
+  } else if (warp < 2 * W + Z::CHAINS) {  // ---- chain warps
+    for (int it = warp - 2 * W;; it += Z::CHAINS) {
+      const int s = it % S;
+      if (!tc::mbar_wait(&sh.full[s], (it / S) & 1)) {
+        tu_tc_error = 705;
+        break;
+      }
+      const int tile = sh.tile[s];
+      if (tile < 0) break;
+      if (!tc::mbar_wait(&sh.mapped[s], (it / S) & 1)) {
+        tu_tc_error = 706;
+        break;
+      }
+      typename Z::Stage &st = sh.st[s];
+      const Place z = place(tile);
+      const int ch = z.cg * C + lane * 2;
+      float2 jP = make_float2(1.f, 1.f), jQ = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float2 P = st.P[i][lane], Q = st.Q[i][lane];
+        jQ.x = through(P.x, Q.x, jQ.x), jQ.y = through(P.y, Q.y, jQ.y);
+        jP.x = is_cut(P.x) ? CUT : jP.x * P.x, jP.y = is_cut(P.y) ? CUT : jP.y * P.y;
+      }
+      const int group = z.step / G, first = group * G, before = z.step - first;
+      const bool leader = before == G - 1 && z.step + 1 < p.nT;  // hands the group's end on
+      auto words = [&](unsigned long long *base, int step) { return base + ((size_t)step * chains + z.chain) * C + lane * 2; };
+      if (before < G - 1) {
+        put(words(p.maps, z.step), map_word(jP.x, jQ.x));
+        put(words(p.maps, z.step) + 1, map_word(jP.y, jQ.y));
+      }
+      // everything that comes before is asked for at once
+      unsigned long long m[G - 1][2], e[2];
+#pragma unroll
+      for (int i = 0; i < G - 1; ++i)
+        if (i < before) m[i][0] = look(words(p.maps, first + i)), m[i][1] = look(words(p.maps, first + i) + 1);
+      float2 c = make_float2(0.f, 0.f);
+      if (group > 0) e[0] = look(words(p.ends, group - 1)), e[1] = look(words(p.ends, group - 1) + 1);
+      else if (!VAR && edge && ch < p.D) c = *reinterpret_cast<const float2 *>(edge + (size_t)z.b * p.D + ch);
+#pragma unroll
+      for (int i = 0; i < G - 1; ++i)
+        if (i < before) m[i][0] = await(words(p.maps, first + i), m[i][0]), m[i][1] = await(words(p.maps, first + i) + 1, m[i][1]);
+      if (group > 0) {
+        c.x = end_of(await(words(p.ends, group - 1), e[0]));
+        c.y = end_of(await(words(p.ends, group - 1) + 1, e[1]));
+      }
+#pragma unroll
+      for (int i = 0; i < G - 1; ++i)
+        if (i < before) {
+          const float2 mx = map_of(m[i][0]), my = map_of(m[i][1]);
+          c.x = through(mx.x, mx.y, c.x), c.y = through(my.x, my.y, c.y);
+        }
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float2 P = st.P[i][lane], Q = st.Q[i][lane];
+        st.P[i][lane] = c;
+        c.x = through(P.x, Q.x, c.x), c.y = through(P.y, Q.y, c.y);
+      }
+      if (leader) {
+        put(words(p.ends, group), end_word(c.x));
+        put(words(p.ends, group) + 1, end_word(c.y));
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.ready[s]);
+    }
+  } else if (warp == 2 * W + Z::CHAINS) {  // ---- load warp
+    for (int it = 0;; ++it) {
+      const int s = it % S;
+      int tile = 0;
+      if (lane == 0) tile = atomicAdd(p.ticket, 1);  // its way to L2 falls into the wait for the stage
+      if (it >= S && !tc::mbar_wait(&sh.empty[s], (it / S - 1) & 1)) {
+        tu_tc_error = 707;
+        break;
+      }
+      __syncwarp();
+      tile = __shfl_sync(0xffffffffu, tile, 0);
+      const bool more = tile < tiles;
+      if (more) {
+        const Place z = place(tile);
+        typename Z::Stage &st = sh.st[s];
+        if (lane == 0) {
+          tc::tma_load_3d(st.buf[1], &mg, &sh.full[s], z.cg * C, z.t0, z.b);
+          tc::tma_load_3d(st.buf[0], &mx, &sh.full[s], z.cg * C, z.t0, z.b);
+          if (BWD) tc::tma_load_3d(st.buf[Z::TENSORS - 1], &mo, &sh.full[s], z.cg * C, z.t0 - 1, z.b);
+        }
+        if (VAR) {
+          bool any = false;
+          for (int r = lane; r < L; r += 32) {
+            const int code = z.t0 + r < p.T ? row_code(p, z.t0 + r) : ROW_OUT;
+            st.code[r] = code;
+            any = any || (code & (ROW_START | ROW_END | ROW_OUT));
+          }
+          any = __any_sync(0xffffffffu, any);
+          if (lane == 0) sh.edges[s] = any;
+        }
+      }
+      __syncwarp();
+      // the end is told once for every chain warp's turn: each of the next CHAINS stages says so
+      if (lane == 0) {
+        sh.tile[s] = more ? tile : -1;
+        if (more) tc::mbar_expect_tx(&sh.full[s], Z::TENSORS * Z::TILE * sizeof(T));
+        else tc::mbar_arrive(&sh.full[s]);
+      }
+      if (!more) {
+        for (int next = it + 1; next < it + Z::CHAINS; ++next) {
+          const int n = next % S;
+          if (next >= S && !tc::mbar_wait(&sh.empty[n], (next / S - 1) & 1)) {
+            tu_tc_error = 708;
+            break;
+          }
+          if (lane == 0) {
+            sh.tile[n] = -1;
+            tc::mbar_arrive(&sh.full[n]);
+          }
+        }
+        break;
+      }
+    }
+  } else if (lane == 0) {  // ---- store warp
+    for (int it = 0;; ++it) {
+      const int s = it % S;
+      if (!tc::mbar_wait(&sh.full[s], (it / S) & 1)) {
+        tu_tc_error = 709;
+        break;
+      }
+      const int tile = sh.tile[s];
+      if (tile < 0) break;
+      if (!tc::mbar_wait(&sh.done[s], (it / S) & 1)) {
+        tu_tc_error = 710;
+        break;
+      }
+      const Place z = place(tile);
+      tc::tma_store_3d(&my, sh.st[s].buf[0], z.cg * C, z.t0, z.b);
+      if (BWD) tc::tma_store_3d(&mz, sh.st[s].buf[1], z.cg * C, z.t0, z.b);
+      tc::tma_store_commit();
+      tc::tma_store_wait_read();
+      tc::mbar_arrive(&sh.empty[s]);
+    }
+    tc::tma_store_wait_all();
+  }
+  __syncthreads();
+}
+
 template <typename T> struct HgrnTile {
   static constexpr int W = 8, R = 16, L = W * R;
 };
@@ -318,7 +646,7 @@ template <typename T> struct HgrnTile {
 struct HgrnPlan {
   int V, C, nT, nCG;
   long long tiles;
-  size_t flag_bytes, end_bytes, map_bytes;  // the first two are cleared before a launch
+  size_t bytes, end_bytes, map_bytes;  // the ticket (256 bytes), the ends, the maps
 };
 
 HgrnPlan hgrn_plan(int B, long long T, int D, int V, int L) {
@@ -327,38 +655,82 @@ HgrnPlan hgrn_plan(int B, long long T, int D, int V, int L) {
   q.nT = (int)((T + L - 1) / L);
   q.nCG = (D + q.C - 1) / q.C;
   q.tiles = (long long)q.nT * B * q.nCG;
-  q.flag_bytes = ((size_t)(q.tiles + 1) * 4 + 255) / 256 * 256;
   q.map_bytes = (size_t)q.tiles * q.C * 8;
   q.end_bytes = (size_t)(q.nT / G) * B * q.nCG * q.C * 8;
+  q.bytes = 256 + q.end_bytes + q.map_bytes;
   return q;
 }
 
+// Hands the workspace out and clears it.
+int hgrn_scratch(HgrnParams &p, const HgrnPlan &q, void *ws, size_t ws_bytes, cudaStream_t st) {
+  FLAB_REQUIRE(ws && ws_bytes >= q.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0, FLAB_E_BADARG,
+               "hgrn needs a 16-byte aligned workspace of flab_hgrn_workspace() bytes");
+  char *w = reinterpret_cast<char *>(ws);
+  p.ticket = reinterpret_cast<int *>(w);
+  p.ends = reinterpret_cast<unsigned long long *>(w + 256);
+  p.maps = reinterpret_cast<unsigned long long *>(w + 256 + q.end_bytes);
+  FLAB_REQUIRE(cudaMemsetAsync(w, 0, q.bytes, st) == cudaSuccess, FLAB_E_LAUNCH, "hgrn: clearing the workspace failed");
+  return FLAB_OK;
+}
+
 template <typename T, bool BWD, bool VAR, int V> int launch_hgrn(HgrnParams p, void *ws, size_t ws_bytes, cudaStream_t st) {
-  typedef HgrnTile<T> G;
-  const HgrnPlan q = hgrn_plan(p.B, p.T, p.D, V, G::L);
+  typedef HgrnTile<T> Z;
+  const HgrnPlan q = hgrn_plan(p.B, p.T, p.D, V, Z::L);
   p.nT = q.nT, p.nCG = q.nCG;
-  FLAB_REQUIRE(q.tiles < (1ll << 31) && p.T < (1ll << 36) && p.D <= (1 << 23) && p.N < (1 << 28), FLAB_E_UNSUPPORTED,
-               "hgrn: T = %lld, D = %d, N = %d are beyond what the kernel indexes", p.T, p.D, p.N);
   if (q.nT > 1) {
-    FLAB_REQUIRE(ws && ws_bytes >= q.flag_bytes + q.map_bytes + q.end_bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0, FLAB_E_BADARG,
-                 "hgrn needs a 16-byte aligned workspace of flab_hgrn_workspace() bytes");
-    char *w = reinterpret_cast<char *>(ws);
-    p.ticket = reinterpret_cast<int *>(w);
-    p.flags = p.ticket + 1;
-    p.ends = reinterpret_cast<unsigned long long *>(w + q.flag_bytes);
-    p.maps = reinterpret_cast<float2 *>(w + q.flag_bytes + q.end_bytes);
-    FLAB_REQUIRE(cudaMemsetAsync(w, 0, q.flag_bytes + q.end_bytes, st) == cudaSuccess, FLAB_E_LAUNCH, "hgrn: clearing the workspace failed");
+    const int rc = hgrn_scratch(p, q, ws, ws_bytes, st);
+    if (rc) return rc;
   }
-  hgrn_tile_kernel<T, V, G::W, G::R, BWD, VAR><<<(unsigned)q.tiles, G::W * 32, 0, st>>>(p);
+  hgrn_tile_kernel<T, V, Z::W, Z::R, BWD, VAR><<<(unsigned)q.tiles, Z::W * 32, 0, st>>>(p);
+  return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+}
+
+template <typename T, bool BWD> struct StreamOf {  // 32 KB (48 KB) of inputs a stage, as many stages as an SM holds
+  static constexpr int R = sizeof(T) == 2 ? 16 : 8, S = BWD ? 4 : 6;
+};
+
+template <typename T, bool BWD, bool VAR> int launch_stream(HgrnParams p, void *ws, size_t ws_bytes, cudaStream_t st) {
+  constexpr int R = StreamOf<T, BWD>::R, S = StreamOf<T, BWD>::S;
+  typedef Stream<T, R, S, BWD> Z;
+  const HgrnPlan q = hgrn_plan(p.B, p.T, p.D, Z::V, Z::L);
+  p.nT = q.nT, p.nCG = q.nCG;
+  int rc = hgrn_scratch(p, q, ws, ws_bytes, st);
+  if (rc) return rc;
+  const CUtensorMapDataType type = sizeof(T) == 4                ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : Num<T>::id == FLAB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t dims[3] = {(uint64_t)p.D, (uint64_t)p.T, (uint64_t)p.B};
+  const uint64_t strides[2] = {(uint64_t)p.D * sizeof(T), (uint64_t)p.T * p.D * sizeof(T)};
+  const uint32_t box[3] = {Z::C, Z::L, 1};
+  CUtensorMap m[5];
+  const void *base[5] = {p.x, p.g, BWD ? p.o_in : p.x, p.o, BWD ? p.dg : p.o};
+  for (int i = 0; i < 5; ++i)
+    if ((rc = make_tensor_map(&m[i], base[i], type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE))) return rc;
+  auto kernel = hgrn_stream_kernel<T, R, S, BWD, VAR>;
+  const int bytes = (int)sizeof(typename Z::Shared);
+  FLAB_REQUIRE(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess, FLAB_E_LAUNCH,
+               "hgrn: %d bytes of shared memory were refused", bytes);
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const long long grid = q.tiles < sms ? q.tiles : sms;
+  kernel<<<(unsigned)grid, Z::THREADS, bytes, st>>>(p, m[0], m[1], m[2], m[3], m[4]);
   return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
 }
 
 template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws, size_t ws_bytes, cudaStream_t st) {
-  constexpr int V = 2;
-  bool vec = p.D % V == 0;
-  for (const void *q : {p.x, p.g, p.o_in, (const void *)p.o, (const void *)p.dg}) vec = vec && reinterpret_cast<uintptr_t>(q) % (V * sizeof(T)) == 0;
-  if (p.cu) return vec ? launch_hgrn<T, BWD, true, V>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, true, 1>(p, ws, ws_bytes, st);
-  return vec ? launch_hgrn<T, BWD, false, V>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, false, 1>(p, ws, ws_bytes, st);
+  FLAB_REQUIRE(p.T < (1ll << 30) && p.D <= (1 << 23) && p.N < (1 << 28) && (p.T + 63) / 64 * p.B * ((p.D + 31) / 32) < (1ll << 31), FLAB_E_UNSUPPORTED,
+               "hgrn: B = %d, T = %lld, D = %d, N = %d are beyond what the kernels index", p.B, p.T, p.D, p.N);
+  bool pair = p.D % 2 == 0, tma = p.D * sizeof(T) % 16 == 0;
+  for (const void *q : {p.x, p.g, p.o_in, (const void *)p.o, (const void *)p.dg}) {
+    pair = pair && reinterpret_cast<uintptr_t>(q) % (2 * sizeof(T)) == 0;
+    tma = tma && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+  }
+  for (const float *q : {p.h0, p.dht, (const float *)p.ht}) tma = tma && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  if (tma && p.T > HgrnTile<T>::L)
+    return p.cu ? launch_stream<T, BWD, true>(p, ws, ws_bytes, st) : launch_stream<T, BWD, false>(p, ws, ws_bytes, st);
+  if (p.cu) return pair ? launch_hgrn<T, BWD, true, 2>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, true, 1>(p, ws, ws_bytes, st);
+  return pair ? launch_hgrn<T, BWD, false, 2>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, false, 1>(p, ws, ws_bytes, st);
 }
 
 template <bool BWD> int run_hgrn(HgrnParams &p, int dtype, void *ws, size_t ws_bytes, cudaStream_t st) {
@@ -381,11 +753,12 @@ size_t flab_hgrn_workspace(int B, long long T, int D) {
   using namespace flab;
   if (B <= 0 || T <= 0 || D <= 0) return 0;
   size_t most = 0;  // of the layouts that a call of this size may take
-  for (int V : {1, 2}) {
-    const HgrnPlan q = hgrn_plan(B, T, D, V, HgrnTile<float>::L);
-    const size_t n = q.nT > 1 ? q.flag_bytes + q.map_bytes + q.end_bytes : 0;
-    most = n > most ? n : most;
-  }
+  for (int V : {1, 2})
+    for (int L : {64, HgrnTile<float>::L}) {
+      const HgrnPlan q = hgrn_plan(B, T, D, V, L);
+      const size_t n = T > HgrnTile<float>::L ? q.bytes : 0;
+      most = n > most ? n : most;
+    }
   return most;
 }
 

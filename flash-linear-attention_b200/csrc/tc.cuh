@@ -91,6 +91,11 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void 
                "r"(c1)
                : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(c0),
+               "r"(c1), "r"(c2)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, const void *src, int c0, int c1, int c2, int c3) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(smem_u32(src)),
                "r"(c0), "r"(c1), "r"(c2), "r"(c3)
@@ -265,6 +270,8 @@ int make_token_map(CUtensorMap *map, const void *base, const flab_args *a, int D
 int make_state_map(CUtensorMap *map, const void *base, const flab_args *a, int box_rows);
 
 // host: tensor-map construction without linking libcuda (entry point fetched from the runtime)
+int make_tensor_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                    const uint32_t *box, CUtensorMapSwizzle swizzle);
 int make_tensor_map_bf16(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
                          const uint32_t *box, int elem_fp16);
 

@@ -21,10 +21,9 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// rank <= 4; dims[0] is the contiguous extent; strides_bytes[i] is the stride of dims[i+1].
-// 128-byte swizzle, zero fill outside the tensor.
-int make_tensor_map_bf16(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
-                         const uint32_t *box, int elem_fp16) {
+// rank <= 4; dims[0] is the contiguous extent; strides_bytes[i] is the stride of dims[i+1].  Zero fill outside the tensor.
+int make_tensor_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                    const uint32_t *box, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_fn();
   // A driver-API call needs a current context; a thread that has only used the runtime lazily (an
   // autograd worker thread, say) may not have bound the primary context yet.  cudaSetDevice binds it
@@ -45,14 +44,19 @@ int make_tensor_map_bf16(CUtensorMap *map, const void *base, int rank, const uin
     es[i] = 1;
     if (i + 1 < rank) gstr[i] = strides_bytes[i];
   }
-  CUresult r = fn(map, elem_fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
-                  const_cast<void *>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void *>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   FLAB_REQUIRE(r == CUDA_SUCCESS, FLAB_E_BADARG, "cuTensorMapEncodeTiled failed with code %d (base %p must be 16-byte aligned, strides multiples of 16)",
                (int)r, base);
   return 0;
 }
 
+// the same for bf16 / fp16 operands with the 128-byte swizzle
+int make_tensor_map_bf16(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                         const uint32_t *box, int elem_fp16) {
+  return make_tensor_map(map, base, elem_fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, dims, strides_bytes, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 int make_token_map(CUtensorMap *map, const void *base, const flab_args *a, int D) {
   const uint64_t e = 2;

@@ -81,7 +81,8 @@ def check(x, g, do, h0, dht, lengths, dtype, shape, offsets, fn=chunk_hgrn, fina
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("B,T,D,state", [(1, 1, 1, True), (2, 1, 64, True), (3, 2, 33, False), (1, 7, 2, True), (2, 127, 66, True), (1, 128, 64, False),
-                                         (2, 129, 31, True), (1, 700, 130, True), (1, 1500, 8, False), (5, 260, 96, True), (2, 9, 24, True)])
+                                         (2, 129, 31, True), (1, 700, 130, True), (1, 1500, 8, False), (5, 260, 96, True), (2, 9, 24, True),
+                                         (2, 1300, 72, True), (3, 1024, 136, False), (1, 129, 8, True)])
 def test_fixed_length(B, T, D, state, dtype):
     x, g, do, h0, dht = inputs(B * T, D, B, dtype, B * T + D, state)
     check(x, g, do, h0, dht, [T] * B, dtype, (B, T, D), None)
@@ -93,7 +94,9 @@ def test_fixed_length(B, T, D, state, dtype):
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 @pytest.mark.parametrize("lengths,behind,D,state", [([1], 0, 64, True), ([5, 1, 130], 0, 34, True), ([0, 3, 0, 0, 300, 1, 0], 0, 70, True),
                                                     ([128, 128, 256], 0, 64, False), ([1] * 150, 0, 65, True), ([600, 90], 17, 32, True),
-                                                    ([0, 0], 5, 32, True), ([127, 1, 129], 140, 64, False)])
+                                                    ([0, 0], 5, 32, True), ([127, 1, 129], 140, 64, False),
+                                                    ([1] * 300, 0, 64, True), ([0, 3, 0, 0, 300, 1, 0], 0, 72, True),
+                                                    ([700, 513, 1, 0, 900], 0, 136, True), ([0, 1100], 1200, 8, True)])
 def test_packed(lengths, behind, D, state, index, dtype):
     """Sequences of no and of one token, edges on and next to a tile's edge, rows behind the last sequence (zeros)."""
     N, rows = len(lengths), sum(lengths) + behind
