@@ -47,7 +47,7 @@ struct HgrnParams {
   unsigned long long *ends;  // [groups][C] words
 };
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
+template <typename T, int V> struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
   T v[V];
 };
 
@@ -73,6 +73,27 @@ __device__ __forceinline__ int row_code(const HgrnParams &p, long long t) {
 // infinity.  Gates are exponentials, so no other factor has a sign; one that underflowed to +0 still hands a NaN on.
 #define CUT (-0.f)
 __device__ __forceinline__ bool is_cut(float P) { return __float_as_uint(P) == 0x80000000u; }
+// e^g as 2^(g log2 e): the product's rounding moves the result by |g| 2^-24 of itself, less than the exponential's own error
+// wherever the gate is near 1 and errors live long.
+__device__ __forceinline__ float gate(float g) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(g * 1.4426950408889634f));
+  return y;
+}
+
+// The number of cumulative lengths that are <= t, by a warp together.
+__device__ __forceinline__ int warp_count(const HgrnParams &p, long long t, int lane) {
+  int lo = 0, hi = p.N + 1;
+  while (lo < hi) {
+    const int by = (hi - lo + 31) / 32, at = lo + lane * by;
+    const int below = __popc(__ballot_sync(0xffffffffu, at < hi && cu_at(p, at) <= t));
+    if (below == 0) break;
+    hi = min(hi, lo + below * by);
+    lo += (below - 1) * by + 1;
+  }
+  return lo;
+}
+
 // y = P c + Q.  A zero start stays out of the product, so that a P that overflowed (gates above 0) makes no NaN of it.
 __device__ __forceinline__ float through(float P, float Q, float c) { return c == 0.f || is_cut(P) ? Q : fmaf(P, c, Q); }
 
@@ -170,7 +191,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      a[r][j] = live ? expf(Num<T>::f(gv[r].v[j])) : 1.f;
+      a[r][j] = live ? gate(Num<T>::f(gv[r].v[j])) : 1.f;
       const float in = live ? Num<T>::f(xv[r].v[j]) : 0.f;
       Q[j] = BWD ? a[r][j] * (Q[j] + in) : fmaf(a[r][j], Q[j], in);
       P[j] *= a[r][j];
@@ -318,21 +339,12 @@ template <typename T> __device__ __forceinline__ void pack2(T *s, float a, float
   v.v[0] = Num<T>::t(a), v.v[1] = Num<T>::t(b);
   *reinterpret_cast<Pack<T, 2> *>(s) = v;
 }
-// e^g as 2^(g log2 e): the product's rounding moves the result by |g| 2^-24 of itself, less than the exponential's own error
-// wherever the gate is near 1 and errors live long.
-__device__ __forceinline__ float gate(float g) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(g * 1.4426950408889634f));
-  return y;
-}
-
 template <typename T, int R, int S, bool BWD> struct Stream {
   static constexpr int V = 2, C = 32 * V, W = 8, L = W * R;
   static constexpr int TILE = L * C, TENSORS = BWD ? 3 : 2;
-  // Chain warps, on tiles in turn.  Their number divides S, so that one warp sees every phase of a stage's barriers: a wait for
-  // a phase's parity says nothing to one that has not seen the phase before it.
-  static constexpr int CHAINS = S % 4 == 0 ? 4 : 3;
-  static_assert(S % CHAINS == 0, "a stage belongs to one chain warp");
+  // One chain warp a stage: each sees every phase of its stage's barriers (a wait for a phase's parity says nothing to one that
+  // has not seen the phase before it), and the waits of all stages overlap.
+  static constexpr int CHAINS = S;
   static constexpr int THREADS = 32 * (2 * W + CHAINS + 2);
   struct Stage {
     T buf[TENSORS][TILE];   // x (do), g, o of a token earlier
@@ -341,7 +353,9 @@ template <typename T, int R, int S, bool BWD> struct Stream {
   };
   struct Shared {
     Stage st[S];
-    int tile[S], edges[S];
+    struct Place {
+      int step, chain, b, cg, t0, edges;  // step: position along the scan, -1 behind the last tile; edges: codes are set
+    } at[S];
     uint64_t full[S], mapped[S], ready[S], done[S], empty[S];
   };
 };
@@ -370,18 +384,6 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
     tc::fence_barrier_init();
   }
   __syncthreads();
-  struct Place {
-    int step, chain, b, cg, t0;
-  };
-  auto place = [&](int tile) {
-    Place z;
-    z.step = tile / chains;
-    z.chain = tile - z.step * chains;
-    z.b = z.chain / p.nCG;
-    z.cg = z.chain - z.b * p.nCG;
-    z.t0 = (BWD ? p.nT - 1 - z.step : z.step) * L;
-    return z;
-  };
   // position r of warp w's rows is this row of the tile
   auto row = [&](int w, int r) -> int { return BWD ? L - 1 - (w * R + r) : w * R + r; };
 
@@ -393,8 +395,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         tu_tc_error = 702;
         break;
       }
-      const int tile = sh.tile[s];
-      if (tile < 0) break;
+      if (sh.at[s].step < 0) break;
       typename Z::Stage &st = sh.st[s];
       const T *const xs = st.buf[0] + lane * 2, *const gs = st.buf[1] + lane * 2;
       float2 P = make_float2(1.f, 1.f), Q = make_float2(0.f, 0.f);
@@ -404,11 +405,11 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         Q.y = BWD ? a.y * (Q.y + x.y) : fmaf(a.y, Q.y, x.y);
         P.x *= a.x, P.y *= a.y;
       };
-      if (!VAR || !sh.edges[s]) {
+      if (!VAR || !sh.at[s].edges) {
 #pragma unroll
         for (int r = 0; r < R; ++r) take(unpack2(gs + row(w, r) * C), unpack2(xs + row(w, r) * C));
       } else {
-        const int ch = place(tile).cg * C + lane * 2;
+        const int ch = sh.at[s].cg * C + lane * 2;
 #pragma unroll 4
         for (int r = 0; r < R; ++r) {
           const int code = st.code[row(w, r)];
@@ -433,14 +434,13 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         tu_tc_error = 703;
         break;
       }
-      const int tile = sh.tile[s];
-      if (tile < 0) break;
+      if (sh.at[s].step < 0) break;
       if (!tc::mbar_wait(&sh.ready[s], (it / S) & 1)) {
         tu_tc_error = 704;
         break;
       }
       typename Z::Stage &st = sh.st[s];
-      const Place z = place(tile);
+      const typename Z::Shared::Place z = sh.at[s];
       const int ch = z.cg * C + lane * 2;
       const bool on = ch < p.D;
       T *const xs = st.buf[0] + lane * 2, *const gs = st.buf[1] + lane * 2;
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         }
       };
       const float2 none = make_float2(0.f, 0.f);
-      if (!VAR || !sh.edges[s]) {
+      if (!VAR || !sh.at[s].edges) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const int at = row(w, r) * C;
@@ -504,14 +504,13 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         tu_tc_error = 705;
         break;
       }
-      const int tile = sh.tile[s];
-      if (tile < 0) break;
+      if (sh.at[s].step < 0) break;
       if (!tc::mbar_wait(&sh.mapped[s], (it / S) & 1)) {
         tu_tc_error = 706;
         break;
       }
       typename Z::Stage &st = sh.st[s];
-      const Place z = place(tile);
+      const typename Z::Shared::Place z = sh.at[s];
       const int ch = z.cg * C + lane * 2;
       float2 jP = make_float2(1.f, 1.f), jQ = make_float2(0.f, 0.f);
 #pragma unroll
@@ -573,32 +572,35 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       __syncwarp();
       tile = __shfl_sync(0xffffffffu, tile, 0);
       const bool more = tile < tiles;
+      typename Z::Shared::Place z;
+      z.step = -1;
       if (more) {
-        const Place z = place(tile);
         typename Z::Stage &st = sh.st[s];
+        z.step = tile / chains;
+        z.chain = tile - z.step * chains;
+        z.b = z.chain / p.nCG;
+        z.cg = z.chain - z.b * p.nCG;
+        z.t0 = (BWD ? p.nT - 1 - z.step : z.step) * L;
+        z.edges = 0;
         if (lane == 0) {
           tc::tma_load_3d(st.buf[1], &mg, &sh.full[s], z.cg * C, z.t0, z.b);
           tc::tma_load_3d(st.buf[0], &mx, &sh.full[s], z.cg * C, z.t0, z.b);
           if (BWD) tc::tma_load_3d(st.buf[Z::TENSORS - 1], &mo, &sh.full[s], z.cg * C, z.t0 - 1, z.b);
         }
-        if (VAR) {
-          bool any = false;
-          for (int r = lane; r < L; r += 32) {
-            const int code = z.t0 + r < p.T ? row_code(p, z.t0 + r) : ROW_OUT;
-            st.code[r] = code;
-            any = any || (code & (ROW_START | ROW_END | ROW_OUT));
-          }
-          any = __any_sync(0xffffffffu, any);
-          if (lane == 0) sh.edges[s] = any;
+        if (VAR) {  // most tiles lie inside one sequence
+          const int n = warp_count(p, z.t0, lane) - 1;
+          z.edges = n < 0 || n >= p.N || cu_at(p, n) == z.t0 || cu_at(p, n + 1) <= z.t0 + L;
+          if (z.edges)
+            for (int r = lane; r < L; r += 32) st.code[r] = z.t0 + r < p.T ? row_code(p, z.t0 + r) : ROW_OUT;
         }
       }
       __syncwarp();
-      // the end is told once for every chain warp's turn: each of the next CHAINS stages says so
       if (lane == 0) {
-        sh.tile[s] = more ? tile : -1;
+        sh.at[s] = z;
         if (more) tc::mbar_expect_tx(&sh.full[s], Z::TENSORS * Z::TILE * sizeof(T));
         else tc::mbar_arrive(&sh.full[s]);
       }
+      // every chain warp is told of the end in its own next stage
       if (!more) {
         for (int next = it + 1; next < it + Z::CHAINS; ++next) {
           const int n = next % S;
@@ -607,7 +609,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
             break;
           }
           if (lane == 0) {
-            sh.tile[n] = -1;
+            sh.at[n].step = -1;
             tc::mbar_arrive(&sh.full[n]);
           }
         }
@@ -621,13 +623,12 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         tu_tc_error = 709;
         break;
       }
-      const int tile = sh.tile[s];
-      if (tile < 0) break;
+      if (sh.at[s].step < 0) break;
       if (!tc::mbar_wait(&sh.done[s], (it / S) & 1)) {
         tu_tc_error = 710;
         break;
       }
-      const Place z = place(tile);
+      const typename Z::Shared::Place z = sh.at[s];
       tc::tma_store_3d(&my, sh.st[s].buf[0], z.cg * C, z.t0, z.b);
       if (BWD) tc::tma_store_3d(&mz, sh.st[s].buf[1], z.cg * C, z.t0, z.b);
       tc::tma_store_commit();
@@ -637,6 +638,48 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
     tc::tma_store_wait_all();
   }
   __syncthreads();
+}
+
+// ---- a few tokens a sequence (decode) ---------------------------------------------------------------------------------
+// A thread walks the tokens of 16 bytes of channels; nothing is shared.
+template <typename T, int V, bool BWD> __global__ void __launch_bounds__(256) hgrn_step_kernel(const HgrnParams p) {
+  const int per = p.D / V;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)p.B * per) return;
+  const int b = (int)(i / per), ch = (int)(i - (long long)b * per) * V;
+  const float *const edge = BWD ? p.dht : p.h0;
+  typedef Pack<T, V> PV;
+  typedef Pack<float, V> PF;
+  PF c, h;
+#pragma unroll
+  for (int j = 0; j < V; ++j) c.v[j] = h.v[j] = 0.f;
+  const size_t state = (size_t)b * p.D + ch;
+  if (edge) c = *reinterpret_cast<const PF *>(edge + state);
+  if (BWD && p.h0) h = *reinterpret_cast<const PF *>(p.h0 + state);
+  for (int k = 0; k < (int)p.T; ++k) {
+    const int t = BWD ? (int)p.T - 1 - k : k;
+    const size_t at = ((size_t)b * p.T + t) * p.D + ch;
+    const PV g = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.g) + at);
+    const PV x = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.x) + at);
+    PV y, z, o;
+    if (BWD && t > 0) o = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.o_in) + at - p.D);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float a = gate(Num<T>::f(g.v[j]));
+      if (!BWD) {
+        c.v[j] = fmaf(a, c.v[j], Num<T>::f(x.v[j]));
+        y.v[j] = Num<T>::t(c.v[j]);
+      } else {
+        const float d = Num<T>::f(x.v[j]) + c.v[j];
+        c.v[j] = a * d;
+        y.v[j] = Num<T>::t(d);
+        z.v[j] = Num<T>::t(c.v[j] * (t > 0 ? Num<T>::f(o.v[j]) : h.v[j]));
+      }
+    }
+    *reinterpret_cast<PV *>(reinterpret_cast<T *>(p.o) + at) = y;
+    if (BWD) *reinterpret_cast<PV *>(reinterpret_cast<T *>(p.dg) + at) = z;
+  }
+  if (p.ht) *reinterpret_cast<PF *>(p.ht + state) = c;
 }
 
 template <typename T> struct HgrnTile {
@@ -718,6 +761,15 @@ template <typename T, bool BWD, bool VAR> int launch_stream(HgrnParams p, void *
   return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
 }
 
+// Sequences of up to this many tokens are walked by one thread a channel group: shorter than that, a tile is mostly empty rows.
+constexpr int STEPS = 8;
+
+template <typename T, bool BWD, int V> int launch_step(const HgrnParams &p, cudaStream_t st) {
+  const long long n = (long long)p.B * (p.D / V);
+  hgrn_step_kernel<T, V, BWD><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
+  return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+}
+
 template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws, size_t ws_bytes, cudaStream_t st) {
   FLAB_REQUIRE(p.T < (1ll << 30) && p.D <= (1 << 23) && p.N < (1 << 28) && (p.T + 63) / 64 * p.B * ((p.D + 31) / 32) < (1ll << 31), FLAB_E_UNSUPPORTED,
                "hgrn: B = %d, T = %lld, D = %d, N = %d are beyond what the kernels index", p.B, p.T, p.D, p.N);
@@ -727,6 +779,11 @@ template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws,
     tma = tma && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   }
   for (const float *q : {p.h0, p.dht, (const float *)p.ht}) tma = tma && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  if (!p.cu && p.T <= STEPS) {
+    bool wide = tma && p.D % (16 / sizeof(T)) == 0;
+    for (const float *q : {p.h0, p.dht, (const float *)p.ht}) wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    return wide ? launch_step<T, BWD, 16 / sizeof(T)>(p, st) : launch_step<T, BWD, 1>(p, st);
+  }
   if (tma && p.T > HgrnTile<T>::L)
     return p.cu ? launch_stream<T, BWD, true>(p, ws, ws_bytes, st) : launch_stream<T, BWD, false>(p, ws, ws_bytes, st);
   if (p.cu) return pair ? launch_hgrn<T, BWD, true, 2>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, true, 1>(p, ws, ws_bytes, st);
