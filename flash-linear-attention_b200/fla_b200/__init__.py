@@ -31,7 +31,7 @@ def install_as_fla_ops():
 
 
 def install_as_fla_modules():
-    """Alias `fla.modules.l2norm` and `fla.modules.fused_norm_gate` to this package's CUDA implementation."""
+    """Alias `fla.modules.{l2norm,fused_norm_gate,convolution,layernorm}` to this package's CUDA implementation."""
     from . import modules
     from .modules import l2norm
     root = sys.modules.get("fla")
@@ -45,5 +45,7 @@ def install_as_fla_modules():
     sys.modules["fla.modules.fused_norm_gate"] = fused_norm_gate
     from .modules import convolution
     sys.modules["fla.modules.convolution"] = convolution
+    from .modules import layernorm
+    sys.modules["fla.modules.layernorm"] = layernorm
     root.modules = modules
 

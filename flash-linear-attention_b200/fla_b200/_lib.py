@@ -109,6 +109,12 @@ def load() -> ctypes.CDLL:
     lib.flab_gdn_gate_fwd.argtypes = [ap, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.flab_gdn_gate_bwd.restype = ci
     lib.flab_gdn_gate_bwd.argtypes = [ap, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.flab_rms_norm_fwd.restype = ci
+    lib.flab_rms_norm_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, ll, ci, ci, ci, ci, ci, ci, cf, vp]
+    lib.flab_rms_norm_partials.restype = ci
+    lib.flab_rms_norm_partials.argtypes = [ll, ci, ci]
+    lib.flab_rms_norm_bwd.restype = ci
+    lib.flab_rms_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ll, ci, ci, ci, ci, vp]
     sz = ctypes.c_size_t
     lib.flab_hgrn_workspace.restype = sz
     lib.flab_hgrn_workspace.argtypes = [ci, ll, ci]

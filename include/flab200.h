@@ -126,6 +126,23 @@ int flab_rms_norm_swish_gate_fwd(const void *x, const void *gate, const float *w
 int flab_rms_norm_swish_gate_bwd(const void *x, const void *gate, const float *weight, const void *dy, const float *rstd, void *dx, void *dgate,
                                  float *dw_partial, long long rows, int n, int dtype, void *stream);
 
+/* ---- RMS norm with the residual's addition, 16 / 32-bit or e4m3 output (the step that opens a block) ----
+ * Replaces rms_norm of fla/modules/layernorm.py (weight, no bias) and adds an 8-bit output:
+ *   s = round(x + residual) in sum_dtype;  y = s rstd weight,  rstd = 1 / sqrt(mean_n s^2 + eps)
+ *   FLAB_NORM_E4M3: y holds e4m3 bytes q = round(y / scale) instead, scale [rows] fp32 = max_n |y| / 448 (0 for a row of zeros)
+ *   FLAB_NORM_NONE (with FLAB_NORM_E4M3): no norm, the rows of x are quantised as they are
+ * x, y: [rows, n] contiguous of type dtype; residual (or NULL) of type dtype or fp32; sum (or NULL: not wanted) of type sum_dtype =
+ * dtype or fp32 (fp32 where the residual is); weight [n] of type weight_dtype or NULL (ones); rstd [rows] fp32 or NULL.
+ * Backward: ds = rstd (weight dy - xhat mean_n(xhat weight dy)) + dsum (or NULL), written as dx (dtype) and / or dresidual (sum_dtype),
+ * each may be NULL; dweight [n] of type weight_dtype or NULL, summed in a fixed order over dw_partial, fp32
+ * [flab_rms_norm_partials(rows, n, dtype), n]. rows == 0 gives zeros in dweight. */
+enum { FLAB_NORM_E4M3 = 1, FLAB_NORM_NONE = 2 };
+int flab_rms_norm_fwd(const void *x, const void *residual, const void *weight, void *y, void *sum, float *rstd, float *scale, long long rows, int n,
+                      int dtype, int residual_dtype, int sum_dtype, int weight_dtype, int flags, float eps, void *stream);
+int flab_rms_norm_partials(long long rows, int n, int dtype);
+int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const void *weight, const float *rstd, void *dx, void *dresidual, void *dweight,
+                      float *dw_partial, long long rows, int n, int dtype, int sum_dtype, int weight_dtype, void *stream);
+
 /* ---- causal depthwise short convolution (q, k, v of the reference's layers pass through it first) ----
  * Replaces the convolution of ShortConvolution.forward / .step (fla/modules/convolution.py:142-216):
  *   y[b,t,d] = act(bias[d] + sum_{w<W} weight[d,w] x[b, t-(W-1)+w, d]),  x = 0 before the sequence, act = SiLU or none.
