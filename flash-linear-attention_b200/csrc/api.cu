@@ -1,4 +1,5 @@
 // Error reporting and version entry points of the C ABI.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -13,6 +14,18 @@ void set_error(const char *fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
   va_end(ap);
+}
+
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
 }
 
 int check_launch(const char *what) {

@@ -459,6 +459,8 @@ __device__ __forceinline__ float warp_sum(float x) {
 // host side
 // ------------------------------------------------------------------------------------------------
 void set_error(const char *fmt, ...);
+// multiprocessors of the current device (looked up once a device)
+int sm_count();
 int check_launch(const char *what);
 
 #define FLAB_REQUIRE(cond, code, ...) \

@@ -751,11 +751,8 @@ template <typename T, bool BWD, bool VAR> int launch_stream(HgrnParams p, void *
     if ((rc = make_tensor_map(&m[i], base[i], type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE))) return rc;
   auto kernel = hgrn_stream_kernel<T, R, S, BWD, VAR>;
   const int bytes = (int)sizeof(typename Z::Shared);
-  FLAB_REQUIRE(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess, FLAB_E_LAUNCH,
-               "hgrn: %d bytes of shared memory were refused", bytes);
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if ((rc = set_smem(kernel, bytes))) return rc;
+  const int sms = sm_count();
   const long long grid = q.tiles < sms ? q.tiles : sms;
   kernel<<<(unsigned)grid, Z::THREADS, bytes, st>>>(p, m[0], m[1], m[2], m[3], m[4]);
   return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");

@@ -13,6 +13,7 @@
 #include <cuda_fp8.h>
 
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -90,10 +91,13 @@ template <int V> __device__ __forceinline__ void store_e4m3(void *base, size_t a
   *reinterpret_cast<Vec<unsigned char, V> *>(reinterpret_cast<unsigned char *>(base) + at) = q;
 }
 
-// T: x and y;  S: the stored sum;  V elements a vector, NV vectors a thread (0: read again);  QUANT: e4m3 output;  NORM: without
-// it the rows are quantised as they are
-template <typename T, typename S, int V, int NV, bool QUANT, bool NORM>
+// T: x and y;  S: the stored sum;  RES: residual, 0 none, 1 of type T, 2 fp32;  V elements a vector, NV vectors a thread (0: read
+// again);  QUANT: e4m3 output;  NORM: without it the rows are quantised as they are.
+// All of a row's loads are issued before its first store: with loads and stores of one loop in turn a row was eight trips to
+// memory one after the other (2.9 TB/s at 32768 x 2048 bf16).
+template <typename T, typename S, int RES, int V, int NV, bool QUANT, bool NORM>
 __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const NormParams p) {
+  typedef typename std::conditional<RES == 2, float, T>::type R;
   __shared__ float slots[2][32];
   const int li = threadIdx.x % p.tpr;
   const long long row = (long long)blockIdx.x * (blockDim.x / p.tpr) + threadIdx.x / p.tpr;
@@ -101,34 +105,53 @@ __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const Nor
   const size_t base = (size_t)row * p.n;
   constexpr int KEEP = NV ? NV : 1;
   const int loops = NV ? NV : (p.n + V * p.tpr - 1) / (V * p.tpr);
-  float f[KEEP][V];
-
-  auto fetch = [&](int c, float (&v)[V], bool first) {  // the stored sum of a vector
-    load_f<T, V>(p.x, base + c, v);
-    if (p.res) {
-      float r[V];
-      if (p.res_fp32) load_f<float, V>(p.res, base + c, r);
-      else load_f<T, V>(p.res, base + c, r);
+  Vec<S, V> s[KEEP];
+  auto at = [&](int k) { return (k * p.tpr + li) * V; };
+  auto add = [&](const Vec<T, V> &x, const Vec<R, V> &r) {  // the stored sum
+    Vec<S, V> v;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] += r[j];
-    }
-    if (p.sum && first) store_f<S, V>(p.sum, base + c, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = rnd<S>(v[j]);
+    for (int j = 0; j < V; ++j) v.v[j] = Num<S>::t(RES ? Num<T>::f(x.v[j]) + Num<R>::f(r.v[j]) : Num<T>::f(x.v[j]));
+    return v;
   };
+  auto fetch = [&](int c) {
+    Vec<T, V> x = *reinterpret_cast<const Vec<T, V> *>(reinterpret_cast<const T *>(p.x) + base + c);
+    Vec<R, V> r;
+    if (RES) r = *reinterpret_cast<const Vec<R, V> *>(reinterpret_cast<const R *>(p.res) + base + c);
+    return add(x, r);
+  };
+  auto keep_sum = [&](int c, const Vec<S, V> &v) { *reinterpret_cast<Vec<S, V> *>(reinterpret_cast<S *>(p.sum) + base + c) = v; };
 
   float ss = 0.f;
-  if (on && (NORM || NV)) {
+  if (NV) {
+    Vec<T, V> x[KEEP];
+    Vec<R, V> r[KEEP];
 #pragma unroll
-    for (int k = 0; k < (NV ? NV : loops); ++k) {
-      const int c = (k * p.tpr + li) * V;
-      float(&v)[V] = f[NV ? k : 0];
-      if (c < p.n) {
-        fetch(c, v, true);
-#pragma unroll
-        for (int j = 0; j < V; ++j) ss = fmaf(v[j], v[j], ss);
+    for (int k = 0; k < KEEP; ++k)
+      if (on && at(k) < p.n) {
+        x[k] = *reinterpret_cast<const Vec<T, V> *>(reinterpret_cast<const T *>(p.x) + base + at(k));
+        if (RES) r[k] = *reinterpret_cast<const Vec<R, V> *>(reinterpret_cast<const R *>(p.res) + base + at(k));
       }
-    }
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+      if (on && at(k) < p.n) {
+        s[k] = add(x[k], r[k]);
+        if (p.sum) keep_sum(at(k), s[k]);
+        if (NORM) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float f = Num<S>::f(s[k].v[j]);
+            ss = fmaf(f, f, ss);
+          }
+        }
+      }
+  } else if (on && NORM) {
+    for (int k = 0; k < loops; ++k)
+      if (at(k) < p.n) {
+        const Vec<S, V> v = fetch(at(k));
+        if (p.sum) keep_sum(at(k), v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) ss = fmaf(Num<S>::f(v.v[j]), Num<S>::f(v.v[j]), ss);
+      }
   }
   float rstd = 1.f;
   if (NORM) {
@@ -136,49 +159,37 @@ __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const Nor
     rstd = 1.f / sqrtf(ss / p.n + p.eps);
     if (on && li == 0 && p.rstd) p.rstd[row] = rstd;
   }
+  auto result = [&](int k, float (&y)[V]) {
+    const Vec<S, V> v = NV ? s[NV ? k : 0] : fetch(at(k));
+    float w[V];
+    load_w<V>(p.w, p.w_type, at(k), w);
+#pragma unroll
+    for (int j = 0; j < V; ++j) y[j] = Num<S>::f(v.v[j]) * rstd * w[j];
+  };
   float inv = 0.f;
   if (QUANT) {
     float top = 0.f;
-    if (on) {
 #pragma unroll
-      for (int k = 0; k < (NV ? NV : loops); ++k) {
-        const int c = (k * p.tpr + li) * V;
-        float(&v)[V] = f[NV ? k : 0];
-        if (c < p.n) {
-          if (!NV) fetch(c, v, !NORM);
-          float w[V];
-          load_w<V>(p.w, p.w_type, c, w);
+    for (int k = 0; k < (NV ? NV : loops); ++k)
+      if (on && at(k) < p.n) {
+        float y[V];
+        result(k, y);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float y = v[j] * rstd * w[j];
-            if (NV) v[j] = y;
-            top = join<true>(top, fabsf(y));
-          }
-        }
+        for (int j = 0; j < V; ++j) top = join<true>(top, fabsf(y[j]));
       }
-    }
     top = row_reduce<true>(top, p.tpr, slots[1]);
     // a row of zeros has scale 0 and zeros; a scale below what has a reciprocal is held there
     inv = top > 0.f ? fminf(E4M3_MAX / top, 3.4e38f) : top;
     if (on && li == 0) p.scale[row] = top / E4M3_MAX;
   }
-  if (!on) return;
 #pragma unroll
-  for (int k = 0; k < (NV ? NV : loops); ++k) {
-    const int c = (k * p.tpr + li) * V;
-    float(&v)[V] = f[NV ? k : 0];
-    if (c < p.n) {
-      if (!NV) fetch(c, v, false);
-      if (!(QUANT && NV)) {
-        float w[V];
-        load_w<V>(p.w, p.w_type, c, w);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = v[j] * rstd * w[j];
-      }
-      if constexpr (QUANT) store_e4m3<V>(p.y, base + c, v, inv);
-      else store_f<T, V>(p.y, base + c, v);
+  for (int k = 0; k < (NV ? NV : loops); ++k)
+    if (on && at(k) < p.n) {
+      float y[V];
+      result(k, y);
+      if constexpr (QUANT) store_e4m3<V>(p.y, base + at(k), y, inv);
+      else store_f<T, V>(p.y, base + at(k), y);
     }
-  }
 }
 
 struct NormBwdParams {
@@ -191,7 +202,7 @@ struct NormBwdParams {
 };
 
 // one partial row of dw a block; the block's groups of TPR threads take rows in turn
-template <typename T, typename S, int V, int NV> __global__ void __launch_bounds__(NV ? 256 : 1024) rms_norm_bwd_kernel(const NormBwdParams p) {
+template <typename T, typename S, int V, int NV> __global__ void __launch_bounds__(NV ? 256 : 1024, NV ? 2 : 1) rms_norm_bwd_kernel(const NormBwdParams p) {
   extern __shared__ float sdw[];  // [groups][n]
   __shared__ float slots[2][32];
   const int li = threadIdx.x % p.tpr, group = threadIdx.x / p.tpr, groups = blockDim.x / p.tpr;
@@ -209,55 +220,51 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
     const bool on = row < p.rows;
     const size_t base = (size_t)row * p.n;
     const float rstd = on ? p.rstd[row] : 0.f;
-    float xh[KEEP][V], wd[KEEP][V], dot = 0.f;
-    Vec<S, V> keep[KEEP];  // ds_out, asked for with the rest
-    if (on) {
+    Vec<S, V> s[KEEP], ds[KEEP];
+    Vec<T, V> dy[KEEP];
+    float dot = 0.f;
+    auto at = [&](int k) { return (k * p.tpr + li) * V; };
+    auto fetch = [&](int i, int c) {
+      s[i] = *reinterpret_cast<const Vec<S, V> *>(reinterpret_cast<const S *>(p.s) + base + c);
+      dy[i] = *reinterpret_cast<const Vec<T, V> *>(reinterpret_cast<const T *>(p.dy) + base + c);
+      if (p.ds) ds[i] = *reinterpret_cast<const Vec<S, V> *>(reinterpret_cast<const S *>(p.ds) + base + c);
+    };
+    if (NV) {  // all of a row's loads first
 #pragma unroll
-      for (int k = 0; k < (NV ? NV : loops); ++k) {
-        const int c = (k * p.tpr + li) * V, i = NV ? k : 0;
-        if (c < p.n) {
-          float w[V], s[V], dy[V];
-          load_f<S, V>(p.s, base + c, s);
-          load_f<T, V>(p.dy, base + c, dy);
-          if (NV && p.ds) keep[i] = *reinterpret_cast<const Vec<S, V> *>(reinterpret_cast<const S *>(p.ds) + base + c);
-          load_w<V>(p.w, p.w_type, c, w);
+      for (int k = 0; k < KEEP; ++k)
+        if (on && at(k) < p.n) fetch(k, at(k));
+    }
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            xh[i][j] = s[j] * rstd;
-            wd[i][j] = w[j] * dy[j];
-            dot = fmaf(xh[i][j], wd[i][j], dot);
-            if (NV) acc[i][j] = fmaf(dy[j], xh[i][j], acc[i][j]);
-            else if (p.part) sdw[c + j] = fmaf(dy[j], xh[i][j], sdw[c + j]);
-          }
+    for (int k = 0; k < (NV ? NV : loops); ++k)
+      if (on && at(k) < p.n) {
+        const int c = at(k), i = NV ? k : 0;
+        if (!NV) fetch(0, c);
+        float w[V];
+        load_w<V>(p.w, p.w_type, c, w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = Num<S>::f(s[i].v[j]) * rstd, d = Num<T>::f(dy[i].v[j]);
+          dot = fmaf(xh, w[j] * d, dot);
+          if (NV) acc[i][j] = fmaf(d, xh, acc[i][j]);
+          else if (p.part) sdw[c + j] = fmaf(d, xh, sdw[c + j]);
         }
       }
-    }
     dot = row_reduce<false>(dot, p.tpr, slots[par]) / p.n;
-    if (on) {
 #pragma unroll
-      for (int k = 0; k < (NV ? NV : loops); ++k) {
-        const int c = (k * p.tpr + li) * V, i = NV ? k : 0;
-        if (c < p.n) {
-          if (!NV) {
-            float w[V], s[V], dy[V];
-            load_f<S, V>(p.s, base + c, s);
-            load_f<T, V>(p.dy, base + c, dy);
-            load_w<V>(p.w, p.w_type, c, w);
-            if (p.ds) keep[i] = *reinterpret_cast<const Vec<S, V> *>(reinterpret_cast<const S *>(p.ds) + base + c);
+    for (int k = 0; k < (NV ? NV : loops); ++k)
+      if (on && at(k) < p.n) {
+        const int c = at(k), i = NV ? k : 0;
+        if (!NV) fetch(0, c);
+        float w[V], d[V];
+        load_w<V>(p.w, p.w_type, c, w);
 #pragma unroll
-            for (int j = 0; j < V; ++j) xh[i][j] = s[j] * rstd, wd[i][j] = w[j] * dy[j];
-          }
-          float d[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            d[j] = (wd[i][j] - xh[i][j] * dot) * rstd;
-            if (p.ds) d[j] += Num<S>::f(keep[i].v[j]);
-          }
-          if (p.dx) store_f<T, V>(p.dx, base + c, d);
-          if (p.dr) store_f<S, V>(p.dr, base + c, d);
+        for (int j = 0; j < V; ++j) {
+          d[j] = (w[j] * Num<T>::f(dy[i].v[j]) - Num<S>::f(s[i].v[j]) * rstd * dot) * rstd;
+          if (p.ds) d[j] += Num<S>::f(ds[i].v[j]);
         }
+        if (p.dx) store_f<T, V>(p.dx, base + c, d);
+        if (p.dr) store_f<S, V>(p.dr, base + c, d);
       }
-    }
   }
   if (!p.part) return;
   if (NV) {
@@ -293,13 +300,6 @@ template <typename T> __global__ void __launch_bounds__(256) partial_sum_kernel(
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 // Threads a row and vectors a thread for `groups` vectors a row: the fewest threads that hold the row in `most` vectors each, then
 // more of them while the rows alone do not fill the card (512 threads an SM).
 void norm_split(long long rows, long long groups, int most, int &tpr, int &nv) {
@@ -318,21 +318,21 @@ bool aligned16(std::initializer_list<const void *> ptrs) {
   return true;
 }
 
-template <typename T, typename S, bool QUANT, bool NORM> int launch_norm_fwd(NormParams p, cudaStream_t st) {
+template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_norm_fwd(NormParams p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum});
-  int nv;
-  norm_split(p.rows, vec ? p.n / V : p.n, 8, p.tpr, nv);
+  int nv = 0;
+  if (p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum})) norm_split(p.rows, p.n / V, 8, p.tpr, nv);
+  const bool vec = nv > 0;
+  if (!vec) norm_split(p.rows, p.n, 8, p.tpr, nv);
   const int block = p.tpr < 128 ? 128 : p.tpr;
   const unsigned grid = (unsigned)((p.rows + block / p.tpr - 1) / (block / p.tpr));
-#define FLAB_NORM(VV, NN) rms_norm_fwd_kernel<T, S, VV, NN, QUANT, NORM><<<grid, block, 0, st>>>(p)
+#define FLAB_NORM(VV, NN) rms_norm_fwd_kernel<T, S, RES, VV, NN, QUANT, NORM><<<grid, block, 0, st>>>(p)
   if (vec) {
     switch (nv) {
       case 1: FLAB_NORM(V, 1); break;
       case 2: FLAB_NORM(V, 2); break;
       case 4: FLAB_NORM(V, 4); break;
-      case 8: FLAB_NORM(V, 8); break;
-      default: FLAB_NORM(V, 0); break;
+      default: FLAB_NORM(V, 8); break;
     }
   } else if (nv) {
     FLAB_NORM(1, 8);
@@ -343,13 +343,18 @@ template <typename T, typename S, bool QUANT, bool NORM> int launch_norm_fwd(Nor
   return check_launch("rms_norm_fwd");
 }
 
-template <typename T, bool QUANT, bool NORM> int norm_fwd_sum(const NormParams &p, bool wide, cudaStream_t st) {
-  return wide ? launch_norm_fwd<T, float, QUANT, NORM>(p, st) : launch_norm_fwd<T, T, QUANT, NORM>(p, st);
+template <typename T, bool QUANT> int norm_fwd_sum(const NormParams &p, bool wide, cudaStream_t st) {
+  if (!wide) return p.res ? launch_norm_fwd<T, T, 1, QUANT, true>(p, st) : launch_norm_fwd<T, T, 0, QUANT, true>(p, st);
+  if (!p.res) return launch_norm_fwd<T, float, 0, QUANT, true>(p, st);
+  if constexpr (sizeof(T) == 2) {
+    if (p.res_fp32) return launch_norm_fwd<T, float, 2, QUANT, true>(p, st);
+  }
+  return launch_norm_fwd<T, float, 1, QUANT, true>(p, st);
 }
 
 template <typename T> int norm_fwd_typed(const NormParams &p, bool wide, bool quant, bool norm, cudaStream_t st) {
-  if (!norm) return launch_norm_fwd<T, T, true, false>(p, st);
-  return quant ? norm_fwd_sum<T, true, true>(p, wide, st) : norm_fwd_sum<T, false, true>(p, wide, st);
+  if (!norm) return launch_norm_fwd<T, T, 0, true, false>(p, st);
+  return quant ? norm_fwd_sum<T, true>(p, wide, st) : norm_fwd_sum<T, false>(p, wide, st);
 }
 
 // the shape of a backward launch: everything that its number of partial rows depends on
@@ -361,10 +366,16 @@ NormBwdPlan norm_bwd_plan(long long rows, int n, int esize, bool vec) {
   NormBwdPlan q;
   const int V = 16 / esize;
   q.vec = vec && n % V == 0;
-  norm_split(rows, q.vec ? n / V : n, q.vec ? 4 : 16, q.tpr, q.nv);
-  if (q.tpr > 256) q.tpr = 1024, q.nv = 0;
+  if (q.vec) {
+    norm_split(rows, n / V, 4, q.tpr, q.nv);
+    q.vec = q.nv > 0 && q.tpr <= 256;
+  }
+  if (!q.vec) {
+    norm_split(rows, n, 16, q.tpr, q.nv);
+    if (q.tpr > 256) q.tpr = 1024, q.nv = 0;
+  }
   q.block = q.nv ? 256 : 1024;
-  const long long want = (rows + q.block / q.tpr - 1) / (q.block / q.tpr), cap = (long long)sm_count() * (q.nv ? 3 : 1);
+  const long long want = (rows + q.block / q.tpr - 1) / (q.block / q.tpr), cap = (long long)sm_count() * (q.nv ? 2 : 1);
   q.grid = (int)(want < 1 ? 1 : want < cap ? want : cap);
   return q;
 }
@@ -379,17 +390,15 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
 #define FLAB_NORM(VV, NN)                                                                                                                   \
   do {                                                                                                                                      \
     auto kernel = rms_norm_bwd_kernel<T, S, VV, NN>;                                                                                        \
-    if (bytes > 48 * 1024)                                                                                                                  \
-      FLAB_REQUIRE(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess, FLAB_E_LAUNCH,     \
-                   "rms_norm_bwd: %zu bytes of shared memory were refused", bytes);                                                         \
+    const int rc = set_smem(kernel, bytes);                                                                                                 \
+    if (rc) return rc;                                                                                                                      \
     kernel<<<q.grid, q.block, bytes, st>>>(p);                                                                                              \
   } while (0)
   if (q.vec) {
     switch (q.nv) {
       case 1: FLAB_NORM(V, 1); break;
       case 2: FLAB_NORM(V, 2); break;
-      case 4: FLAB_NORM(V, 4); break;
-      default: FLAB_NORM(V, 0); break;
+      default: FLAB_NORM(V, 4); break;
     }
   } else if (q.nv == 16) {
     FLAB_NORM(1, 16);

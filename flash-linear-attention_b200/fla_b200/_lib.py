@@ -187,6 +187,11 @@ def device_of(t: torch.Tensor):
     return nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream of `t`'s device as the C ABI takes it (torch.cuda.current_stream makes an object of it, 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def finish(entry: str, rc: int) -> None:
     """What follows every call of an entry point with plain arguments: the error of a refused one, the count of a good one."""
     if rc != 0:

@@ -20,7 +20,13 @@ def _p(t):
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
+    if x.dim() == 2:
+        return x.contiguous()
     return x.reshape(math.prod(x.shape[:-1]), x.shape[-1]).contiguous()
+
+
+def _like(t: torch.Tensor, shape) -> torch.Tensor:
+    return t if t.shape == shape else t.reshape(shape)
 
 
 def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=True):
@@ -37,7 +43,7 @@ def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=T
             rc = lib.flab_rms_norm_fwd(x2.data_ptr(), _p(r2), _p(w), y.data_ptr(), _p(total), _p(rstd), _p(scale), rows, n, _DTYPES[x2.dtype],
                                        _DTYPES[x2.dtype if r2 is None else r2.dtype], _DTYPES[sum_dtype],
                                        _DTYPES[torch.float32 if w is None else w.dtype], NORM_E4M3 * quant + NORM_NONE * (not norm), eps,
-                                       torch.cuda.current_stream(dev).cuda_stream)
+                                       _lib.stream_of(x2))
         _lib.finish("flab_rms_norm_fwd", rc)
     return y, scale, total, rstd
 
@@ -55,8 +61,8 @@ class RMSNormFunction(torch.autograd.Function):
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         ctx.r_dtype = None if residual is None else residual.dtype
         ctx.set_materialize_grads(False)
-        y = y.reshape(x.shape)
-        return (y, total.reshape(x.shape)) if prenorm else y
+        y = _like(y, x.shape)
+        return (y, _like(total, x.shape)) if prenorm else y
 
     @staticmethod
     @once_differentiable
@@ -79,12 +85,12 @@ class RMSNormFunction(torch.autograd.Function):
             with _lib.device_of(total):
                 rc = lib.flab_rms_norm_bwd(total.data_ptr(), dy.data_ptr(), _p(dsum), _p(w), rstd.data_ptr(), _p(dx), _p(dr), _p(dw), _p(part),
                                            rows, n, _DTYPES[ctx.x_dtype], _DTYPES[total.dtype],
-                                           _DTYPES[torch.float32 if w is None else w.dtype], torch.cuda.current_stream(dev).cuda_stream)
+                                           _DTYPES[torch.float32 if w is None else w.dtype], _lib.stream_of(total))
             _lib.finish("flab_rms_norm_bwd", rc)
         elif dw is not None:
             dw.zero_()
-        dx = None if dx is None else dx.reshape(ctx.x_shape)
-        dr = dr.reshape(ctx.x_shape) if wide else dx
+        dx = None if dx is None else _like(dx, ctx.x_shape)
+        dr = _like(dr, ctx.x_shape) if wide else dx
         return dx if need_x else None, dw, dr if need_r else None, None, None, None
 
 
@@ -127,8 +133,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[tor
         return (out, x) if prenorm and same else out
     y, _, total, _ = _forward(_rows(x), None if weight is None else weight.contiguous(), None if residual is None else _rows(residual), float(eps),
                               sum_dtype, prenorm and not same, False)
-    y = y.reshape(x.shape)
-    return (y, x if same else total.reshape(x.shape)) if prenorm else y
+    y = _like(y, x.shape)
+    return (y, x if same else _like(total, x.shape)) if prenorm else y
 
 
 def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -143,8 +149,8 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Op
     same = residual is None and sum_dtype == x.dtype
     q, scale, total, _ = _forward(_rows(x), None if weight is None else weight.contiguous(), None if residual is None else _rows(residual), float(eps),
                                   sum_dtype, prenorm and not same, False, quant=True)
-    q, scale = q.reshape(x.shape), scale.reshape(x.shape[:-1])
-    return (q, scale, x if same else total.reshape(x.shape)) if prenorm else (q, scale)
+    q, scale = _like(q, x.shape), _like(scale, x.shape[:-1])
+    return (q, scale, x if same else _like(total, x.shape)) if prenorm else (q, scale)
 
 
 def quantize_rows(x: torch.Tensor):
@@ -154,7 +160,7 @@ def quantize_rows(x: torch.Tensor):
     if _differentiable(x):
         raise NotImplementedError("quantize_rows has no backward: call it under torch.no_grad()")
     q, scale, _, _ = _forward(_rows(x), None, None, 0.0, x.dtype, False, False, quant=True, norm=False)
-    return q.reshape(x.shape), scale.reshape(x.shape[:-1])
+    return _like(q, x.shape), _like(scale, x.shape[:-1])
 
 
 class RMSNorm(nn.Module):

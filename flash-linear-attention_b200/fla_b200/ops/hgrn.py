@@ -23,7 +23,7 @@ def _launch(entry, ref, *args):
     ws_bytes = lib.flab_hgrn_workspace(B, T, D)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ref.device) if ws_bytes else None
     with _lib.device_of(ref):
-        rc = getattr(lib, entry)(*args, _p(ws), ws_bytes, torch.cuda.current_stream(ref.device).cuda_stream)
+        rc = getattr(lib, entry)(*args, _p(ws), ws_bytes, _lib.stream_of(ref))
     _lib.finish(entry, rc)
 
 
