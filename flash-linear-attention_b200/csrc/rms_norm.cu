@@ -15,7 +15,9 @@
 #include <initializer_list>
 #include <type_traits>
 
-#include "common.cuh"
+#include "tc.cuh"
+
+FLAB_TC_DEFINE_ERROR_WORD(rms_norm_error)
 
 namespace flab {
 namespace {
@@ -61,20 +63,36 @@ template <int V> __device__ __forceinline__ void load_w(const void *w, int type,
   }
 }
 
-// sum (or maximum, where a NaN wins) over the TPR threads of a row; `slot` is a row of shared memory per warp of the block
-template <bool MAX> __device__ __forceinline__ float join(float a, float b) { return MAX ? (b > a || b != b ? b : a) : a + b; }
-template <bool MAX> __device__ __forceinline__ float row_reduce(float v, int tpr, float *slot) {
+// Sum over the TPR threads of a row, or the largest |y|: magnitudes go as their bits, whose order is theirs and puts a NaN on top.
+// `slot` is a row of shared memory for this reduction, one value a warp of the block; sync() is the barrier of the row's threads.
+// Every thread adds the warps' values in the same order.
+__device__ __forceinline__ unsigned magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+template <typename Sync> __device__ __forceinline__ float row_sum(float v, int tpr, float *slot, Sync sync) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = join<MAX>(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (tpr > 32) {
-    const int warp = threadIdx.x >> 5, first = threadIdx.x / tpr * (tpr >> 5);
-    if ((threadIdx.x & 31) == 0) slot[warp] = v;
-    __syncthreads();
-    v = slot[first];
-    for (int i = 1; i < tpr >> 5; ++i) v = join<MAX>(v, slot[first + i]);
+    const int nw = tpr >> 5, first = threadIdx.x / tpr * nw, lane = threadIdx.x & 31;
+    if (lane == 0) slot[threadIdx.x >> 5] = v;
+    sync();
+    v = lane < nw ? slot[first + lane] : 0.f;
+    for (int o = nw >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v = __shfl_sync(0xffffffffu, v, 0);
   }
   return v;
 }
+template <typename Sync> __device__ __forceinline__ float row_top(unsigned v, int tpr, float *slot, Sync sync) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (tpr > 32) {
+    const int nw = tpr >> 5, first = threadIdx.x / tpr * nw, lane = threadIdx.x & 31;
+    if (lane == 0) slot[threadIdx.x >> 5] = __uint_as_float(v);
+    sync();
+    v = __reduce_max_sync(0xffffffffu, lane < nw ? __float_as_uint(slot[first + lane]) : 0u);
+  }
+  return __uint_as_float(v);
+}
+struct BlockSync {
+  __device__ __forceinline__ void operator()() const { __syncthreads(); }
+};
 
 // V e4m3 bytes, values beyond the type's range held at its largest (a NaN stays one)
 template <int V> __device__ __forceinline__ void store_e4m3(void *base, size_t at, const float (&f)[V], float inv) {
@@ -155,7 +173,7 @@ __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const Nor
   }
   float rstd = 1.f;
   if (NORM) {
-    ss = row_reduce<false>(ss, p.tpr, slots[0]);
+    ss = row_sum(ss, p.tpr, slots[0], BlockSync());
     rstd = 1.f / sqrtf(ss / p.n + p.eps);
     if (on && li == 0 && p.rstd) p.rstd[row] = rstd;
   }
@@ -168,16 +186,16 @@ __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const Nor
   };
   float inv = 0.f;
   if (QUANT) {
-    float top = 0.f;
+    unsigned bits = 0;
 #pragma unroll
     for (int k = 0; k < (NV ? NV : loops); ++k)
       if (on && at(k) < p.n) {
         float y[V];
         result(k, y);
 #pragma unroll
-        for (int j = 0; j < V; ++j) top = join<true>(top, fabsf(y[j]));
+        for (int j = 0; j < V; ++j) bits = max(bits, magnitude(y[j]));
       }
-    top = row_reduce<true>(top, p.tpr, slots[1]);
+    const float top = row_top(bits, p.tpr, slots[1], BlockSync());
     // a row of zeros has scale 0 and zeros; a scale below what has a reciprocal is held there
     inv = top > 0.f ? fminf(E4M3_MAX / top, 3.4e38f) : top;
     if (on && li == 0) p.scale[row] = top / E4M3_MAX;
@@ -249,7 +267,7 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
           else if (p.part) sdw[c + j] = fmaf(d, xh, sdw[c + j]);
         }
       }
-    dot = row_reduce<false>(dot, p.tpr, slots[par]) / p.n;
+    dot = row_sum(dot, p.tpr, slots[par], BlockSync()) / p.n;
 #pragma unroll
     for (int k = 0; k < (NV ? NV : loops); ++k)
       if (on && at(k) < p.n) {
@@ -278,6 +296,200 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
   for (int c = threadIdx.x; c < p.n; c += blockDim.x) {
     float t = 0.f;
     for (int i = 0; i < groups; ++i) t += sdw[(size_t)i * p.n + c];
+    p.part[(size_t)blockIdx.x * p.n + c] = t;
+  }
+}
+
+// ---- many rows: a persistent block, rows by bulk copies -----------------------------------------------------------------
+// A group of TPR threads walks rows through a ring of shared-memory stages that its first thread keeps filled, so that loads
+// stay in flight over the reductions and stores of the rows before; a thread holds its columns' weights (and, in backward, their
+// dw) in registers for all its rows.  The barrier of a row's reduction is also the point behind which its stage may be refilled.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(tc::smem_u32(bar))
+               : "memory");
+}
+
+constexpr int RING_THREADS = 512, MAX_STAGES = 8;
+
+struct RingShape {
+  int tpr, groups, stages, row_bytes;
+};
+
+// the barrier of a group's threads
+struct GroupSync {
+  int tpr, group;
+  __device__ __forceinline__ void operator()() const {
+    if (tpr == RING_THREADS) __syncthreads();
+    else tc::named_barrier(1 + group, tpr);
+  }
+};
+
+template <typename T, typename S, int RES, int NV, bool QUANT>
+__global__ void __launch_bounds__(RING_THREADS, 1) rms_norm_fwd_ring_kernel(const NormParams p, const RingShape q) {
+  typedef typename std::conditional<RES == 2, float, T>::type R;
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ __align__(128) char ring[];
+  __shared__ uint64_t full[16][MAX_STAGES];
+  __shared__ float slots[4][RING_THREADS / 32];
+  const int group = threadIdx.x / q.tpr, li = threadIdx.x % q.tpr;
+  char *const mine = ring + (size_t)group * q.stages * q.row_bytes;
+  if (li == 0)
+    for (int i = 0; i < q.stages; ++i) tc::mbar_init(&full[group][i], 1);
+  tc::fence_barrier_init();
+  __syncthreads();
+  const long long row0 = (long long)blockIdx.x * q.groups + group, stride = (long long)gridDim.x * q.groups;
+  const uint32_t x_bytes = p.n * sizeof(T), r_bytes = RES ? p.n * sizeof(R) : 0;
+  auto fill = [&](int st, long long row) {
+    char *dst = mine + (size_t)st * q.row_bytes;
+    tc::mbar_expect_tx(&full[group][st], x_bytes + r_bytes);
+    bulk_load(dst, reinterpret_cast<const T *>(p.x) + row * p.n, x_bytes, &full[group][st]);
+    if (RES) bulk_load(dst + x_bytes, reinterpret_cast<const R *>(p.res) + row * p.n, r_bytes, &full[group][st]);
+  };
+  if (li == 0)
+    for (int i = 0; i < q.stages; ++i)
+      if (row0 + i * stride < p.rows) fill(i, row0 + i * stride);
+  auto at = [&](int k) { return (k * q.tpr + li) * V; };
+  float w[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (at(k) < p.n) load_w<V>(p.w, p.w_type, at(k), w[k]);
+  bool dead = false;
+  int st = 0, phase = 0, par = 0;
+  for (long long row = row0; row < p.rows; row += stride, par ^= 1) {
+    const char *src = mine + (size_t)st * q.row_bytes;
+    if (!dead && !tc::mbar_wait(&full[group][st], phase)) tu_tc_error = 720, dead = true;
+    const size_t base = (size_t)row * p.n;
+    Vec<S, V> s[NV];
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at(k) < p.n) {
+        const Vec<T, V> x = *reinterpret_cast<const Vec<T, V> *>(src + at(k) * sizeof(T));
+        Vec<R, V> r;
+        if (RES) r = *reinterpret_cast<const Vec<R, V> *>(src + x_bytes + at(k) * sizeof(R));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s[k].v[j] = Num<S>::t(RES ? Num<T>::f(x.v[j]) + Num<R>::f(r.v[j]) : Num<T>::f(x.v[j]));
+          const float f = Num<S>::f(s[k].v[j]);
+          ss = fmaf(f, f, ss);
+        }
+      }
+    ss = row_sum(ss, q.tpr, slots[par], GroupSync{q.tpr, group});
+    if (li == 0 && !dead && row + q.stages * stride < p.rows) fill(st, row + q.stages * stride);
+    if (++st == q.stages) st = 0, phase ^= 1;
+    const float rstd = 1.f / sqrtf(ss / p.n + p.eps);
+    if (li == 0 && p.rstd) p.rstd[row] = rstd;
+    if (p.sum) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (at(k) < p.n) *reinterpret_cast<Vec<S, V> *>(reinterpret_cast<S *>(p.sum) + base + at(k)) = s[k];
+    }
+    float inv = 0.f;
+    if (QUANT) {
+      unsigned bits = 0;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (at(k) < p.n) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) bits = max(bits, magnitude(Num<S>::f(s[k].v[j]) * rstd * w[k][j]));
+        }
+      const float top = row_top(bits, q.tpr, slots[2 + par], GroupSync{q.tpr, group});
+      inv = top > 0.f ? fminf(E4M3_MAX / top, 3.4e38f) : top;
+      if (li == 0) p.scale[row] = top / E4M3_MAX;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at(k) < p.n) {
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = Num<S>::f(s[k].v[j]) * rstd * w[k][j];
+        if constexpr (QUANT) store_e4m3<V>(p.y, base + at(k), y, inv);
+        else store_f<T, V>(p.y, base + at(k), y);
+      }
+  }
+}
+
+template <typename T, typename S, int NV> __global__ void __launch_bounds__(RING_THREADS, 1) rms_norm_bwd_ring_kernel(const NormBwdParams p, const RingShape q) {
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ __align__(128) char ring[];
+  __shared__ uint64_t full[16][MAX_STAGES];
+  __shared__ float slots[2][RING_THREADS / 32];
+  const int group = threadIdx.x / q.tpr, li = threadIdx.x % q.tpr;
+  char *const mine = ring + (size_t)group * q.stages * q.row_bytes;
+  if (li == 0)
+    for (int i = 0; i < q.stages; ++i) tc::mbar_init(&full[group][i], 1);
+  tc::fence_barrier_init();
+  __syncthreads();
+  const long long row0 = (long long)blockIdx.x * q.groups + group, stride = (long long)gridDim.x * q.groups;
+  const uint32_t s_bytes = p.n * sizeof(S), y_bytes = p.n * sizeof(T);
+  auto fill = [&](int st, long long row) {
+    char *dst = mine + (size_t)st * q.row_bytes;
+    tc::mbar_expect_tx(&full[group][st], y_bytes + (p.ds ? 2 : 1) * s_bytes);
+    bulk_load(dst, reinterpret_cast<const S *>(p.s) + row * p.n, s_bytes, &full[group][st]);
+    bulk_load(dst + s_bytes, reinterpret_cast<const T *>(p.dy) + row * p.n, y_bytes, &full[group][st]);
+    if (p.ds) bulk_load(dst + s_bytes + y_bytes, reinterpret_cast<const S *>(p.ds) + row * p.n, s_bytes, &full[group][st]);
+  };
+  if (li == 0)
+    for (int i = 0; i < q.stages; ++i)
+      if (row0 + i * stride < p.rows) fill(i, row0 + i * stride);
+  auto at = [&](int k) { return (k * q.tpr + li) * V; };
+  float w[NV][V], acc[NV][V] = {};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (at(k) < p.n) load_w<V>(p.w, p.w_type, at(k), w[k]);
+  bool dead = false;
+  int st = 0, phase = 0, par = 0;
+  for (long long row = row0; row < p.rows; row += stride, par ^= 1) {
+    const char *src = mine + (size_t)st * q.row_bytes;
+    const float rstd = p.rstd[row];
+    if (!dead && !tc::mbar_wait(&full[group][st], phase)) tu_tc_error = 721, dead = true;
+    const size_t base = (size_t)row * p.n;
+    Vec<S, V> s[NV], ds[NV];
+    Vec<T, V> dy[NV];
+    float dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at(k) < p.n) {
+        s[k] = *reinterpret_cast<const Vec<S, V> *>(src + at(k) * sizeof(S));
+        dy[k] = *reinterpret_cast<const Vec<T, V> *>(src + s_bytes + at(k) * sizeof(T));
+        if (p.ds) ds[k] = *reinterpret_cast<const Vec<S, V> *>(src + s_bytes + y_bytes + at(k) * sizeof(S));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = Num<S>::f(s[k].v[j]) * rstd, d = Num<T>::f(dy[k].v[j]);
+          dot = fmaf(xh, w[k][j] * d, dot);
+          acc[k][j] = fmaf(d, xh, acc[k][j]);
+        }
+      }
+    dot = row_sum(dot, q.tpr, slots[par], GroupSync{q.tpr, group}) / p.n;
+    if (li == 0 && !dead && row + q.stages * stride < p.rows) fill(st, row + q.stages * stride);
+    if (++st == q.stages) st = 0, phase ^= 1;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at(k) < p.n) {
+        float d[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          d[j] = (w[k][j] * Num<T>::f(dy[k].v[j]) - Num<S>::f(s[k].v[j]) * rstd * dot) * rstd;
+          if (p.ds) d[j] += Num<S>::f(ds[k].v[j]);
+        }
+        if (p.dx) store_f<T, V>(p.dx, base + at(k), d);
+        if (p.dr) store_f<S, V>(p.dr, base + at(k), d);
+      }
+  }
+  if (!p.part) return;
+  __syncthreads();  // the ring is empty: every row that was asked for has been read
+  float *const sdw = reinterpret_cast<float *>(ring);
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (at(k) < p.n) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) sdw[(size_t)group * p.n + at(k) + j] = acc[k][j];
+    }
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.n; c += RING_THREADS) {
+    float t = 0.f;
+    for (int i = 0; i < q.groups; ++i) t += sdw[(size_t)i * p.n + c];
     p.part[(size_t)blockIdx.x * p.n + c] = t;
   }
 }
@@ -318,10 +530,40 @@ bool aligned16(std::initializer_list<const void *> ptrs) {
   return true;
 }
 
+// The ring's shape for rows of n elements (V a vector) of which a stage holds row_bytes; nv = 0: not for this row.  It pays where
+// every group has several rows to walk (measured at 2048 columns of bf16: ring 95 against 110 us at 32768 rows, the direct kernel
+// ahead below four rows a group, where filling the ring is all there is).
+bool ring_shape(long long rows, int n, int V, int row_bytes, RingShape &q, int &nv, int &grid) {
+  const int vecs = n / V;
+  q.tpr = 32;
+  while (2 * q.tpr < vecs && q.tpr < RING_THREADS) q.tpr *= 2;
+  nv = (vecs + q.tpr - 1) / q.tpr;
+  q.groups = RING_THREADS / q.tpr;
+  q.row_bytes = row_bytes;
+  q.stages = (int)(200 * 1024 / ((size_t)q.groups * row_bytes));
+  if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
+  grid = sm_count();
+  return nv <= 2 && q.stages >= 2 && rows >= 4ll * q.groups * grid;
+}
+
 template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_norm_fwd(NormParams p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   int nv = 0;
-  if (p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum})) norm_split(p.rows, p.n / V, 8, p.tpr, nv);
+  const bool aligned = p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum});
+  RingShape q;
+  int grid_ring;
+  if (NORM && aligned && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0)), q, nv, grid_ring)) {
+    const size_t bytes = (size_t)q.groups * q.stages * q.row_bytes;
+    auto launch = [&](auto kernel) {
+      const int rc = set_smem(kernel, bytes);
+      if (rc) return rc;
+      kernel<<<grid_ring, RING_THREADS, bytes, st>>>(p, q);
+      return check_launch("rms_norm_fwd");
+    };
+    return nv == 1 ? launch(rms_norm_fwd_ring_kernel<T, S, RES, 1, QUANT>) : launch(rms_norm_fwd_ring_kernel<T, S, RES, 2, QUANT>);
+  }
+  nv = 0;
+  if (aligned) norm_split(p.rows, p.n / V, 8, p.tpr, nv);
   const bool vec = nv > 0;
   if (!vec) norm_split(p.rows, p.n, 8, p.tpr, nv);
   const int block = p.tpr < 128 ? 128 : p.tpr;
@@ -382,7 +624,22 @@ NormBwdPlan norm_bwd_plan(long long rows, int n, int esize, bool vec) {
 
 template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStream_t st, int &parts) {
   constexpr int V = 16 / sizeof(T);
-  const NormBwdPlan q = norm_bwd_plan(p.rows, p.n, sizeof(T), aligned16({p.s, p.dy, p.ds, p.w, p.dx, p.dr}));
+  const bool aligned = aligned16({p.s, p.dy, p.ds, p.w, p.dx, p.dr});
+  RingShape r;
+  int nv;
+  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + 2 * sizeof(S)), r, nv, parts)) {
+    size_t bytes = (size_t)r.groups * r.stages * r.row_bytes;
+    const size_t sums = (size_t)r.groups * p.n * sizeof(float);
+    if (bytes < sums) bytes = sums;
+    auto launch = [&](auto kernel) {
+      const int rc = set_smem(kernel, bytes);
+      if (rc) return rc;
+      kernel<<<parts, RING_THREADS, bytes, st>>>(p, r);
+      return check_launch("rms_norm_bwd");
+    };
+    return nv == 1 ? launch(rms_norm_bwd_ring_kernel<T, S, 1>) : launch(rms_norm_bwd_ring_kernel<T, S, 2>);
+  }
+  const NormBwdPlan q = norm_bwd_plan(p.rows, p.n, sizeof(T), aligned);
   p.tpr = q.tpr;
   parts = q.grid;
   const size_t bytes = p.part ? (size_t)(q.block / q.tpr) * p.n * sizeof(float) : 0;
@@ -453,7 +710,8 @@ int flab_rms_norm_partials(long long rows, int n, int dtype) {
   if (rows <= 0 || n <= 0) return 1;
   const int e = dtype == FLAB_FP32 ? 4 : 2;
   const int a = flab::norm_bwd_plan(rows, n, e, true).grid, b = flab::norm_bwd_plan(rows, n, e, false).grid;
-  return a > b ? a : b;
+  const int sms = flab::sm_count();  // the ring's grid
+  return a > b ? (a > sms ? a : sms) : b > sms ? b : sms;
 }
 
 int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const void *weight, const float *rstd, void *dx, void *dresidual, void *dweight,
