@@ -1,0 +1,494 @@
+// Products with an epilogue, for the projections either side of the recurrences (nn.Linear in fla/layers; the epilogue's parts are
+// separate PyTorch kernels there):
+//   y = act(x W^T + b) + r            x [M, K], W [N, K] bf16 / fp16, or e4m3 bytes with a scale a row of each
+//   backward:  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum over rows of dz;  dr = dy
+// One tcgen05 kernel computes all three products, C[m, n] = sum_k A(m, k) B(n, k), with either operand stored row by row
+// (K-major) or column by column (MN-major: W in dx, dz and x in dW), so nothing is transposed in memory.  Accumulation fp32 in TMEM;
+// the epilogue is fp32 and rounds once.  z is kept for backward in the type of x (one rounding of the argument of act', whose effect
+// is below the rounding of dz), and dz is rounded to that type because it is an operand of both products.
+//
+// Layout: a pair of CTAs works on a 256 x BN tile (cta_group::2), each CTA loading its 128 rows of A and its half of B, S stages of
+// 128-byte rows by TMA; the accumulator is double buffered in TMEM so that a tile's epilogue runs under the next tile's products.
+// The epilogue turns 32 x 64 blocks in shared memory, so that a warp's global reads and writes are whole rows of 128 bytes whatever
+// the row pitch of the outputs.
+#include "tc.cuh"
+
+FLAB_TC_DEFINE_ERROR_WORD(linear_error)
+
+namespace flab {
+namespace {
+
+enum { ACT_NONE = 0, ACT_SILU = 1, ACT_SIGMOID = 2, ACT_LOGSIGMOID = 3, ACT_GELU = 4 };
+
+__device__ __forceinline__ float act_fwd(float z, int act) {
+  switch (act) {
+    case ACT_SILU: return __fdividef(z, 1.f + __expf(-z));
+    case ACT_SIGMOID: return __fdividef(1.f, 1.f + __expf(-z));
+    case ACT_LOGSIGMOID: return fminf(z, 0.f) - log1pf(__expf(-fabsf(z)));
+    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+  switch (act) {
+    case ACT_SILU: {
+      const float s = __fdividef(1.f, 1.f + __expf(-z));
+      return s * (1.f + z * (1.f - s));
+    }
+    case ACT_SIGMOID: {
+      const float s = __fdividef(1.f, 1.f + __expf(-z));
+      return s * (1.f - s);
+    }
+    case ACT_LOGSIGMOID: return __fdividef(1.f, 1.f + __expf(z));
+    case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    default: return 1.f;
+  }
+}
+
+struct GemmParams {
+  int M, N, K;          // C [M, N]; K: the summed extent
+  int tiles_n, tiles;
+  void *c;              // [M, N]
+  void *z;              // z before the activation, same type, or null
+  const void *bias;     // [N] or null
+  const void *res;      // [M, N] or null
+  const float *row_scale, *col_scale;  // e4m3 operands
+  int act;
+  int pairs;            // rows of c, z, res and bias begin on 4-byte boundaries
+};
+
+template <int BN> struct GemmShape {
+  static constexpr int S = BN == 256 ? 5 : BN == 128 ? 6 : 7;
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
+  static constexpr int TURN = 32 * 64 * 4;  // a warp's block of 32 x 64 floats; 16-byte piece c of row r lies at c ^ (r & 7)
+  static constexpr int BYTES = S * STAGE + EPI_WARPS * TURN + 1024;
+};
+
+// TO: type of c, z, bias, residual.  F8: e4m3 operands, else 16 bits of type T16 (0 fp16, 1 bf16).  AMN / BMN: MN-major operands.
+template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREADS, 1)
+    gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb) {
+  typedef GemmShape<BN> Z;
+  constexpr int S = Z::S, BK = F8 ? 128 : 64;  // 128 bytes of each row
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  uint8_t *const buf = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_rank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  constexpr uint32_t COLS = 2 * BN;
+
+  if (warp == 2) tc::tmem_alloc_pair(&tmem_base, COLS);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) tc::mbar_init(&full[i], 1), tc::mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&acc_full[i], 1), tc::mbar_init(&acc_empty[i], 2 * Z::EPI_WARPS);
+    tc::fence_barrier_init();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const int kblocks = (p.K + BK - 1) / BK;
+
+  if (warp == 0) {  // ---- loads
+    if (lane == 0) {
+      tc::tma_prefetch_desc(&ma);
+      tc::tma_prefetch_desc(&mb);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < p.tiles && ok; tile += clusters) {
+        const int m0 = tile / p.tiles_n * 256 + rank * 128, n0 = tile % p.tiles_n * BN + rank * (BN / 2);
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % S;
+          if (it >= S && !tc::mbar_wait(&empty[s], (it / S - 1) & 1)) {
+            tu_tc_error = 730;
+            ok = false;
+            break;
+          }
+          const uint32_t bar = tc::peer_addr(&full[s], 0);
+          if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * Z::STAGE);
+          uint8_t *const a = buf + s * Z::STAGE, *const b = a + Z::A_BYTES;
+          if constexpr (AMN) {
+            for (int i = 0; i < 2; ++i) tc::tma_load_2d_pair(a + i * 8192, &ma, bar, m0 + i * 64, kb * BK);
+          } else {
+            tc::tma_load_2d_pair(a, &ma, bar, kb * BK, m0);
+          }
+          if constexpr (BMN) {
+            for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(b + i * 8192, &mb, bar, n0 + i * 64, kb * BK);
+          } else {
+            tc::tma_load_2d_pair(b, &mb, bar, kb * BK, n0);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {  // ---- products
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = F8 ? tc::instr_desc(256, BN, 0, 0, 0) : tc::instr_desc(256, BN, T16, AMN, BMN);
+      uint32_t it = 0;
+      int n = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < p.tiles && ok; tile += clusters, ++n) {
+        const int half = n & 1;
+        if (n >= 2 && !tc::mbar_wait(&acc_empty[half], (n / 2 - 1) & 1)) {
+          tu_tc_error = 731;
+          break;
+        }
+        tc::fence_after_sync();
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % S;
+          if (!tc::mbar_wait(&full[s], (it / S) & 1)) {
+            tu_tc_error = 732;
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+          const uint32_t a = tc::smem_u32(buf + s * Z::STAGE), b = a + Z::A_BYTES;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc::umma_pair<F8>(tmem + half * BN, AMN ? tc::desc_mnmajor(a, k, 8192) : tc::desc_kmajor(a, k, 0),
+                              BMN ? tc::desc_mnmajor(b, k, 8192) : tc::desc_kmajor(b, k, 0), idesc, kb > 0 || k > 0);
+          tc::umma_commit_pair(&empty[s]);
+        }
+        if (ok) tc::umma_commit_pair(&acc_full[half]);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 64 columns in turn
+    const int w = warp - 4, quarter = w & 3, side = w >> 2;
+    float *const turn = reinterpret_cast<float *>(buf + S * Z::STAGE + w * Z::TURN);
+    int n = 0;
+    for (int tile = cluster; tile < p.tiles; tile += clusters, ++n) {
+      const int half = n & 1;
+      if (!tc::mbar_wait(&acc_full[half], (n / 2) & 1)) {
+        tu_tc_error = 733;
+        break;
+      }
+      tc::fence_after_sync();
+      const int m0 = tile / p.tiles_n * 256 + rank * 128 + quarter * 32, n0 = tile % p.tiles_n * BN;
+      const uint32_t from = tmem + half * BN + ((uint32_t)(quarter * 32) << 16);
+      const int rows = min(32, p.M - m0);
+      for (int cb = side; cb < BN / 64; cb += 2) {
+        float v[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tc::tmem_ld_32x32b_x32(from + cb * 64 + h * 32, v);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4 *>(turn + lane * 64 + (((h * 8 + j) ^ (lane & 7)) << 2)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+        __syncwarp();
+        const int c0 = n0 + cb * 64 + lane * 2;  // this lane's two columns
+        const bool on0 = c0 < p.N, on1 = c0 + 1 < p.N;
+        float2 bias = make_float2(0.f, 0.f), scale = make_float2(1.f, 1.f);
+        if (EPI && p.bias) {
+          if (on0) bias.x = Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c0]);
+          if (on1) bias.y = Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c0 + 1]);
+        }
+        if (F8) {
+          if (on0) scale.x = p.col_scale[c0];
+          if (on1) scale.y = p.col_scale[c0 + 1];
+        }
+        struct alignas(2 * sizeof(TO)) Two {
+          TO v[2];
+        };
+        auto get = [&](const void *q, size_t at) {
+          const TO *const e = reinterpret_cast<const TO *>(q) + at;
+          Two t;
+          if (p.pairs && on1) {
+            t = *reinterpret_cast<const Two *>(e);
+          } else {
+            if (on0) t.v[0] = e[0];
+            if (on1) t.v[1] = e[1];
+          }
+          return t;
+        };
+        auto set = [&](void *q, size_t at, float2 f) {
+          TO *const e = reinterpret_cast<TO *>(q) + at;
+          Two t;
+          t.v[0] = Num<TO>::t(f.x), t.v[1] = Num<TO>::t(f.y);
+          if (p.pairs && on1) {
+            *reinterpret_cast<Two *>(e) = t;
+          } else {
+            if (on0) e[0] = t.v[0];
+            if (on1) e[1] = t.v[1];
+          }
+        };
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          Two res[8];
+          if (EPI && p.res) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (r0 + i < rows) res[i] = get(p.res, (size_t)(m0 + r0 + i) * p.N + c0);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (r0 + i >= rows) break;
+            float2 f = *reinterpret_cast<const float2 *>(turn + (r0 + i) * 64 + (((lane >> 1) ^ i) << 2) + (lane & 1) * 2);  // r0 % 8 == 0
+            const size_t at = (size_t)(m0 + r0 + i) * p.N + c0;
+            if (F8) {
+              const float rs = p.row_scale[m0 + r0 + i];
+              f.x = f.x * rs * scale.x, f.y = f.y * rs * scale.y;
+            }
+            if (EPI) {
+              f.x += bias.x, f.y += bias.y;
+              if (p.z) set(p.z, at, f);
+              if (p.act) f.x = act_fwd(f.x, p.act), f.y = act_fwd(f.y, p.act);
+              if (p.res) f.x += Num<TO>::f(res[i].v[0]), f.y += Num<TO>::f(res[i].v[1]);
+            }
+            set(p.c, at, f);
+          }
+        }
+        __syncwarp();
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();
+  tc::fence_after_sync();
+  if (warp == 2) tc::tmem_dealloc_pair(tmem, COLS);
+}
+
+// ---- dz = dy act'(z), and the column sums of dz ---------------------------------------------------------------------------
+// A block takes 32 V columns x a run of rows; dz may have a row pitch of its own.  Partial column sums, one row a run.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) act_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ z, T *__restrict__ dz, float *__restrict__ part, int M,
+                                                      int N, int pitch, int run, int act) {
+  __shared__ float s[8][32 * V];
+  struct alignas(V * sizeof(T)) Pack {
+    T v[V];
+  };
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (blockIdx.x * 32 + lane) * V;
+  const int end = min(M, (int)(blockIdx.y + 1) * run);
+  float sum[V] = {};
+  if (c < N) {
+#pragma unroll 4
+    for (int r = blockIdx.y * run + w; r < end; r += 8) {
+      const size_t at = (size_t)r * N + c;
+      const Pack d = *reinterpret_cast<const Pack *>(dy + at);
+      Pack u, o;
+      if (z) u = *reinterpret_cast<const Pack *>(z + at);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float f = Num<T>::f(d.v[j]);
+        if (z) f *= act_slope(Num<T>::f(u.v[j]), act);
+        sum[j] += f;
+        o.v[j] = Num<T>::t(f);
+      }
+      if (dz) *reinterpret_cast<Pack *>(dz + (size_t)r * pitch + c) = o;
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[w][lane * V + j] = sum[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 256)
+    if (blockIdx.x * 32 * V + i < N) {
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += s[k][i];
+      part[(size_t)blockIdx.y * N + blockIdx.x * 32 * V + i] = t;
+    }
+}
+
+constexpr int RUN = 256;  // rows of a partial column sum
+
+template <typename T>
+int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, int N, int pitch, int act, cudaStream_t st) {
+  const T *d = reinterpret_cast<const T *>(dy), *u = act ? reinterpret_cast<const T *>(z) : nullptr;
+  T *o = reinterpret_cast<T *>(dz);
+  const unsigned runs = (M + RUN - 1) / RUN;
+  FLAB_REQUIRE(runs < 65536, FLAB_E_UNSUPPORTED, "linear_bwd: too many rows (%d)", M);
+  bool wide = N % 8 == 0;
+  for (const void *q : {(const void *)d, (const void *)u, (const void *)o}) wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+  if (wide) act_bwd_kernel<T, 8><<<dim3((N + 255) / 256, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, RUN, act);
+  else act_bwd_kernel<T, 1><<<dim3((N + 31) / 32, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, RUN, act);
+  return check_launch("linear_bwd");
+}
+
+// rows of `n` elements to rows of `pitch`
+template <typename T> __global__ void __launch_bounds__(256) repitch_kernel(const T *__restrict__ from, T *__restrict__ to, int rows, int n, int pitch) {
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+#pragma unroll 4
+    for (int c = lane; c < n; c += 32) to[(size_t)r * pitch + c] = from[(size_t)r * n + c];
+  }
+}
+
+int operand_map(CUtensorMap *map, const void *base, int dtype, long long rows, int cols, int pitch, int box_cols, int box_rows) {
+  const CUtensorMapDataType type = dtype == FLAB_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == FLAB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)pitch * (dtype == FLAB_E4M3 ? 1 : 2)};
+  const uint32_t box[2] = {(uint32_t)box_cols, (uint32_t)box_rows};
+  return make_tensor_map(map, base, type, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI>
+int launch_gemm_bn(GemmParams p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
+  typedef GemmShape<BN> Z;
+  const int bk = F8 ? 128 : 64;
+  CUtensorMap ma, mb;
+  int rc = AMN ? operand_map(&ma, a, dtype, p.K, p.M, a_pitch, 64, 64) : operand_map(&ma, a, dtype, p.M, p.K, a_pitch, bk, 128);
+  if (rc) return rc;
+  rc = BMN ? operand_map(&mb, b, dtype, p.K, p.N, b_pitch, 64, 64) : operand_map(&mb, b, dtype, p.N, p.K, b_pitch, bk, BN / 2);
+  if (rc) return rc;
+  p.tiles_n = (p.N + BN - 1) / BN;
+  const long long tiles = (long long)((p.M + 255) / 256) * p.tiles_n;
+  FLAB_REQUIRE(tiles < (1 << 30), FLAB_E_UNSUPPORTED, "linear: %d x %d is too large", p.M, p.N);
+  p.tiles = (int)tiles;
+  auto kernel = gemm_kernel<TO, F8, T16, AMN, BMN, BN, EPI>;
+  if ((rc = set_smem(kernel, Z::BYTES))) return rc;
+  const int clusters = sm_count() / 2;
+  kernel<<<2 * (p.tiles < clusters ? p.tiles : clusters), Z::THREADS, Z::BYTES, st>>>(p, ma, mb);
+  return check_launch("linear");
+}
+
+// The widest tile that still gives every pair of SMs one: with fewer tiles than pairs the time is the length of one tile, and a
+// narrower one is shorter.
+template <typename TO, bool F8, int T16, bool AMN, bool BMN, bool EPI>
+int launch_gemm(const GemmParams &p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
+  const long long rows = (p.M + 255) / 256;
+  const int clusters = sm_count() / 2;
+  if (rows * ((p.N + 255) / 256) >= clusters) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 256, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
+  if (BMN || rows * ((p.N + 127) / 128) >= clusters) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 128, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
+  if constexpr (!BMN) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 64, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
+  return FLAB_E_UNSUPPORTED;
+}
+
+template <typename... Ptr> bool four(int n, Ptr... ptr) {
+  bool ok = n % 2 == 0;
+  for (const void *q : {(const void *)ptr...}) ok = ok && reinterpret_cast<uintptr_t>(q) % 4 == 0;
+  return ok;
+}
+
+// An operand's rows as TMA needs them (16-byte address and pitch): where they lie, or copied into the caller's scratch.
+struct Scratch {
+  char *at;
+  size_t left;
+};
+int pitch_of(int n) { return (n + 7) / 8 * 8; }
+bool as_is(const void *p, int n) { return n % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+size_t copy_bytes(long long rows, int n) { return ((size_t)rows * pitch_of(n) * 2 + 255) / 256 * 256; }
+int operand(const void *&p, int &pitch, int rows, int n, Scratch &ws, cudaStream_t st) {
+  pitch = pitch_of(n);
+  if (as_is(p, n)) return FLAB_OK;
+  const size_t need = copy_bytes(rows, n);
+  FLAB_REQUIRE(ws.at && ws.left >= need, FLAB_E_BADARG, "linear needs a workspace of flab_linear_workspace() bytes");
+  const int blocks = rows / 8 + 1, cap = sm_count() * 8;
+  repitch_kernel<unsigned short><<<blocks < cap ? blocks : cap, 256, 0, st>>>(reinterpret_cast<const unsigned short *>(p),
+                                                                             reinterpret_cast<unsigned short *>(ws.at), rows, n, pitch);
+  p = ws.at;
+  ws.at += need, ws.left -= need;
+  return check_launch("linear repitch");
+}
+
+}  // namespace
+
+int sum_partials(const float *part, void *out, int parts, int n, int dtype, cudaStream_t st);
+
+}  // namespace flab
+
+extern "C" {
+
+// scratch of the forward product (backward = 0), or of the backward ones
+size_t flab_linear_workspace(const void *x, const void *weight, int M, int N, int K, int backward) {
+  using namespace flab;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  size_t n = (as_is(x, K) ? 0 : copy_bytes(M, K)) + (as_is(weight, K) ? 0 : copy_bytes(N, K));
+  if (backward) n += copy_bytes(M, N);
+  return n;
+}
+
+int flab_linear_fwd(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *z, int M, int N, int K, int act, int dtype,
+                    void *ws, size_t ws_bytes, void *stream) {
+  using namespace flab;
+  cudaStream_t st = (cudaStream_t)stream;
+  FLAB_REQUIRE(M >= 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_fwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
+  FLAB_REQUIRE(dtype == FLAB_BF16 || dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_fwd: element type %d is not supported", dtype);
+  if (M == 0) return FLAB_OK;
+  FLAB_REQUIRE(x && weight && y, FLAB_E_BADARG, "linear_fwd needs x, weight, y");
+  FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0, FLAB_E_BADARG, "linear_fwd: ws must be 256-byte aligned");
+  Scratch s = {reinterpret_cast<char *>(ws), ws_bytes};
+  GemmParams p = {};
+  p.M = M, p.N = N, p.K = K, p.c = y, p.z = z, p.bias = bias, p.res = residual, p.act = act;
+  p.pairs = four(N, y, z, residual);
+  int xp, wp, rc;
+  if ((rc = operand(x, xp, M, K, s, st)) || (rc = operand(weight, wp, N, K, s, st))) return rc;
+  return dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, false, true>(p, x, xp, weight, wp, dtype, st)
+                            : launch_gemm<__half, false, 0, false, false, true>(p, x, xp, weight, wp, dtype, st);
+}
+
+int flab_linear_bwd_partials(int M) { return M <= 0 ? 1 : (M + flab::RUN - 1) / flab::RUN; }
+
+int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *dy, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
+                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *stream) {
+  using namespace flab;
+  cudaStream_t st = (cudaStream_t)stream;
+  FLAB_REQUIRE(M > 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_bwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
+  FLAB_REQUIRE(dtype == FLAB_BF16 || dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_bwd: element type %d is not supported", dtype);
+  FLAB_REQUIRE(dy && (!dx || weight) && (!dweight || x) && (act == ACT_NONE || z) && (!dbias || db_partial), FLAB_E_BADARG,
+               "linear_bwd needs dy, weight for dx, x for dweight, z for an activation, db_partial for dbias");
+  FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0, FLAB_E_BADARG, "linear_bwd: ws must be 256-byte aligned");
+  Scratch s = {reinterpret_cast<char *>(ws), ws_bytes};
+  const void *dz = dy;
+  int zp = pitch_of(N), rc;
+  const bool make_dz = (dx || dweight) && (act != ACT_NONE || !as_is(dy, N));
+  if (make_dz || dbias) {
+    void *out = nullptr;
+    if (make_dz) {
+      const size_t need = copy_bytes(M, N);
+      FLAB_REQUIRE(s.at && s.left >= need, FLAB_E_BADARG, "linear_bwd needs a workspace of flab_linear_workspace() bytes");
+      dz = out = s.at;
+      s.at += need, s.left -= need;
+    }
+    rc = dtype == FLAB_BF16 ? launch_act_bwd<bf16>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st)
+                            : launch_act_bwd<__half>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st);
+    if (rc) return rc;
+    if (dbias && (rc = sum_partials(db_partial, dbias, flab_linear_bwd_partials(M), N, dtype, st))) return rc;
+  }
+  GemmParams p = {};
+  if (dx) {
+    int wp;
+    if ((rc = operand(weight, wp, N, K, s, st))) return rc;
+    p.M = M, p.N = K, p.K = N, p.c = dx, p.pairs = four(K, dx);
+    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, true, false>(p, dz, zp, weight, wp, dtype, st)
+                            : launch_gemm<__half, false, 0, false, true, false>(p, dz, zp, weight, wp, dtype, st);
+    if (rc) return rc;
+  }
+  if (dweight) {
+    int xp;
+    if ((rc = operand(x, xp, M, K, s, st))) return rc;
+    p.M = N, p.N = K, p.K = M, p.c = dweight, p.pairs = four(K, dweight);
+    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, true, true, false>(p, dz, zp, x, xp, dtype, st)
+                            : launch_gemm<__half, false, 0, true, true, false>(p, dz, zp, x, xp, dtype, st);
+    if (rc) return rc;
+  }
+  return FLAB_OK;
+}
+
+int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, const float *w_scale, const void *bias, const void *residual, void *y, int M,
+                     int N, int K, int act, int out_dtype, void *stream) {
+  using namespace flab;
+  cudaStream_t st = (cudaStream_t)stream;
+  FLAB_REQUIRE(M >= 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_e4m3: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
+  FLAB_REQUIRE(out_dtype == FLAB_BF16 || out_dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_e4m3: output type %d is not supported", out_dtype);
+  if (M == 0) return FLAB_OK;
+  FLAB_REQUIRE(x && x_scale && weight && w_scale && y, FLAB_E_BADARG, "linear_e4m3 needs x, weight, their scales and y");
+  FLAB_REQUIRE(K % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0, FLAB_E_UNSUPPORTED,
+               "linear_e4m3: K = %d must be a multiple of 16 and the operands 16-byte aligned", K);
+  GemmParams p = {};
+  p.M = M, p.N = N, p.K = K, p.c = y, p.bias = bias, p.res = residual, p.act = act, p.row_scale = x_scale, p.col_scale = w_scale;
+  p.pairs = four(N, y, residual);
+  return out_dtype == FLAB_BF16 ? launch_gemm<bf16, true, 0, false, false, true>(p, x, K, weight, K, FLAB_E4M3, st)
+                                : launch_gemm<__half, true, 0, false, false, true>(p, x, K, weight, K, FLAB_E4M3, st);
+}
+}

@@ -79,7 +79,7 @@ int make_state_map(CUtensorMap *map, const void *base, const flab_args *a, int b
   return make_tensor_map_bf16(map, base, 2, dims, str, box, a->dtype == FLAB_FP16);
 }
 
-#define FLAB_ERROR_UNITS(X) X(hgrn_error) X(rms_norm_error) X(tc_chunk_o_error) X(recurrent_error) X(tc_delta_h_error) X(tc_dqkwg_error) X(tc_wy_bwd_error) X(tc_wy_fwd_error) X(tc_selftest_error)
+#define FLAB_ERROR_UNITS(X) X(hgrn_error) X(linear_error) X(rms_norm_error) X(tc_chunk_o_error) X(recurrent_error) X(tc_delta_h_error) X(tc_dqkwg_error) X(tc_wy_bwd_error) X(tc_wy_fwd_error) X(tc_selftest_error)
 #define FLAB_DECLARE_UNIT(name) \
   int name();                   \
   int name##_clear();

@@ -116,6 +116,16 @@ def load() -> ctypes.CDLL:
     lib.flab_rms_norm_bwd.restype = ci
     lib.flab_rms_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ll, ci, ci, ci, ci, vp]
     sz = ctypes.c_size_t
+    lib.flab_linear_workspace.restype = sz
+    lib.flab_linear_workspace.argtypes = [vp, vp, ci, ci, ci, ci]
+    lib.flab_linear_fwd.restype = ci
+    lib.flab_linear_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp]
+    lib.flab_linear_bwd_partials.restype = ci
+    lib.flab_linear_bwd_partials.argtypes = [ci]
+    lib.flab_linear_bwd.restype = ci
+    lib.flab_linear_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp]
+    lib.flab_linear_e4m3.restype = ci
+    lib.flab_linear_e4m3.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp]
     lib.flab_hgrn_workspace.restype = sz
     lib.flab_hgrn_workspace.argtypes = [ci, ll, ci]
     lib.flab_hgrn_fwd.restype = ci

@@ -1,0 +1,150 @@
+# -*- coding: utf-8 -*-
+"""Projections as one kernel each: a product with bias, activation and residual in its epilogue (`linear`), and the same for e4m3
+tokens and weights with a scale a row (`linear_fp8`; `rms_norm_quant` and `quantize_rows` make them). They stand for nn.Linear and the
+elementwise steps around it in fla/layers (gate and input projections in front of a recurrence, the output projection onto the
+residual stream). The kernels are in csrc/linear.cu."""
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .._lib import _DTYPES
+
+ACTIVATIONS = {None: 0, "silu": 1, "swish": 1, "sigmoid": 2, "logsigmoid": 3, "gelu": 4}
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    if x.dim() == 2:
+        return x.contiguous()
+    return x.reshape(math.prod(x.shape[:-1]), x.shape[-1]).contiguous()
+
+
+def _workspace(n: int, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _forward(x2, w, b, r2, act, want_z):
+    (M, K), N = x2.shape, w.shape[0]
+    y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
+    z = torch.empty_like(y) if want_z else None
+    if M:
+        lib = _lib.load()
+        n = lib.flab_linear_workspace(x2.data_ptr(), w.data_ptr(), M, N, K, 0)
+        ws = _workspace(n, x2.device)
+        with _lib.device_of(x2):
+            rc = lib.flab_linear_fwd(x2.data_ptr(), w.data_ptr(), _p(b), _p(r2), y.data_ptr(), _p(z), M, N, K, act, _DTYPES[x2.dtype], _p(ws), n,
+                                     _lib.stream_of(x2))
+        _lib.finish("flab_linear_fwd", rc)
+    return y, z
+
+
+class LinearFunction(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        x2, w = _rows(x), weight.contiguous()
+        need_x, need_w, need_b, _ = ctx.needs_input_grad[:4]
+        y, z = _forward(x2, w, None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act,
+                        act != 0 and (need_x or need_w or need_b))
+        ctx.save_for_backward(x2 if need_w else None, w if need_x else None, z)
+        ctx.act, ctx.sizes, ctx.x_shape = act, (x2.shape[0], w.shape[0], w.shape[1]), x.shape
+        return y.reshape(x.shape[:-1] + (w.shape[0],))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2, w, z = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        M, N, K = ctx.sizes
+        d2, dev = _rows(dy), dy.device
+        dx = torch.empty(M, K, dtype=dy.dtype, device=dev) if need_x else None
+        dw = torch.empty(N, K, dtype=dy.dtype, device=dev) if need_w else None
+        db = torch.empty(N, dtype=dy.dtype, device=dev) if need_b else None
+        if M == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        elif need_x or need_w or need_b:
+            lib = _lib.load()
+            n = lib.flab_linear_workspace(_p(x2), _p(w), M, N, K, 1)
+            ws = _workspace(n, dev)
+            part = torch.empty(lib.flab_linear_bwd_partials(M), N, dtype=torch.float32, device=dev) if need_b else None
+            with _lib.device_of(d2):
+                rc = lib.flab_linear_bwd(_p(x2), _p(w), _p(z), d2.data_ptr(), _p(dx), _p(dw), _p(db), _p(part), M, N, K, ctx.act, _DTYPES[dy.dtype],
+                                         _p(ws), n, _lib.stream_of(d2))
+            _lib.finish("flab_linear_bwd", rc)
+        return (None if dx is None else dx.reshape(ctx.x_shape)), dw, db, (dy if need_r else None), None
+
+
+def _check(x, weight, bias, residual, activation, dtype):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"Activation `{activation}` not supported: one of None, silu (swish), sigmoid, logsigmoid and gelu.")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"x must be [..., K] and weight [N, K] with N, K > 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != dtype):
+        raise ValueError(f"bias must be [{N}] in {dtype}, got {bias.dtype} {tuple(bias.shape)}")
+    if residual is not None and (residual.shape != x.shape[:-1] + (N,) or residual.dtype != dtype):
+        raise ValueError(f"residual must be {tuple(x.shape[:-1]) + (N,)} in {dtype}, got {residual.dtype} {tuple(residual.shape)}")
+    if not x.is_cuda:
+        raise RuntimeError("flab200 kernels run on CUDA tensors only (no CPU fallback)")
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"{name} is on {t.device}, expected {x.device}")
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+           activation: Optional[str] = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual, differentiable in all four tensors.
+
+    x `[..., K]`, weight `[N, K]`, bias `[N]`, residual `[..., N]`, all of one type, bf16 or fp16 (fp32 is refused: the tensor
+    cores would round it); activation None, "silu" (or "swish"), "sigmoid", "logsigmoid" (a log forget gate) or "gelu" (erf)."""
+    if x.dtype not in _HALF or weight.dtype != x.dtype:
+        raise ValueError(f"x and weight must both be bfloat16 or both float16, got {x.dtype} and {weight.dtype}")
+    _check(x, weight, bias, residual, activation, x.dtype)
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return LinearFunction.apply(x, weight, bias, residual, act)
+    y, _ = _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False)
+    return y.reshape(x.shape[:-1] + (weight.shape[0],))
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, activation: Optional[str] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """act((x x_scale)(weight weight_scale)^T + bias) + residual for float8_e4m3fn x `[..., K]` and weight `[N, K]` with fp32 scales
+    `[...]` and `[N]`, as `rms_norm_quant` and `quantize_rows` return them. K a multiple of 16; bias, residual and the result in
+    out_dtype, bf16 or fp16. For inference: no backward."""
+    e4m3 = torch.float8_e4m3fn
+    if x.dtype != e4m3 or weight.dtype != e4m3 or out_dtype not in _HALF:
+        raise ValueError(f"x and weight must be float8_e4m3fn and out_dtype bfloat16 or float16, got {x.dtype}, {weight.dtype} and {out_dtype}")
+    for name, s, shape in (("x_scale", x_scale, x.shape[:-1]), ("weight_scale", weight_scale, weight.shape[:1])):
+        if s.dtype != torch.float32 or s.shape != shape or s.device != x.device:
+            raise ValueError(f"{name} must be {tuple(shape)} in float32 on {x.device}, got {s.dtype} {tuple(s.shape)} on {s.device}")
+    _check(x, weight, bias, residual, activation, out_dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, weight_scale, bias, residual)):
+        raise NotImplementedError("linear_fp8 has no backward: call it under torch.no_grad()")
+    if x.shape[-1] % 16:
+        raise ValueError(f"linear_fp8: K = {x.shape[-1]} must be a multiple of 16")
+    x2, w = _rows(x), weight.contiguous()
+    if x2.data_ptr() % 16:
+        x2 = x2.clone()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    b, r2 = None if bias is None else bias.contiguous(), None if residual is None else _rows(residual)
+    xs, ws = x_scale.contiguous(), weight_scale.contiguous()
+    (M, K), N = x2.shape, w.shape[0]
+    y = torch.empty(M, N, dtype=out_dtype, device=x.device)
+    if M:
+        lib = _lib.load()
+        with _lib.device_of(x2):
+            rc = lib.flab_linear_e4m3(x2.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), _p(b), _p(r2), y.data_ptr(), M, N, K,
+                                      ACTIVATIONS[activation], _DTYPES[out_dtype], _lib.stream_of(x2))
+        _lib.finish("flab_linear_e4m3", rc)
+    return y.reshape(x.shape[:-1] + (N,))

@@ -34,7 +34,7 @@ extern "C" {
 #define FLAB_ABI_VERSION 1
 #define FLAB_CHUNK 64
 
-enum { FLAB_BF16 = 0, FLAB_FP16 = 1, FLAB_FP32 = 2 };
+enum { FLAB_BF16 = 0, FLAB_FP16 = 1, FLAB_FP32 = 2, FLAB_E4M3 = 3 /* operands of flab_linear_e4m3 only */ };
 
 enum {
   FLAB_OK = 0,
@@ -142,6 +142,25 @@ int flab_rms_norm_fwd(const void *x, const void *residual, const void *weight, v
 int flab_rms_norm_partials(long long rows, int n, int dtype);
 int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const void *weight, const float *rstd, void *dx, void *dresidual, void *dweight,
                       float *dw_partial, long long rows, int n, int dtype, int sum_dtype, int weight_dtype, void *stream);
+
+/* ---- projections: a product with bias, activation and residual in its epilogue -----------------
+ * What nn.Linear and the elementwise kernels around it do in the reference's layers, and its gradients:
+ *   z = x weight^T + bias;  y = act(z) + residual;   dz = d_y act'(z);  dx = dz weight;  dweight = dz^T x;  dbias = sum of dz over rows
+ * x, dx: [M, K]; weight, dweight: [N, K]; bias, dbias: [N]; y, z, residual, d_y: [M, N]; contiguous, of type dtype (bf16 or fp16).
+ * act: 0 none, 1 silu, 2 sigmoid, 3 log sigmoid, 4 gelu (erf). bias, residual may be NULL; z (NULL: not wanted) is what backward
+ * needs with an activation. Each of dx, dweight, dbias may be NULL; db_partial: fp32 [flab_linear_bwd_partials(M), N], summed in a
+ * fixed order. ws: 256-byte aligned, flab_linear_workspace() bytes (it holds operands whose rows do not begin on 16-byte boundaries,
+ * and dz); 0 bytes: NULL. M == 0 is a no-op in forward.
+ * flab_linear_e4m3: operands of e4m3 bytes that stand for x * x_scale[row] and weight * w_scale[row] (fp32 [M], [N]); bias, residual
+ * and y of type out_dtype (bf16 or fp16); K a multiple of 16, operands 16-byte aligned. */
+size_t flab_linear_workspace(const void *x, const void *weight, int M, int N, int K, int backward);
+int flab_linear_fwd(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *z, int M, int N, int K, int act, int dtype,
+                    void *ws, size_t ws_bytes, void *stream);
+int flab_linear_bwd_partials(int M);
+int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *d_y, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
+                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *stream);
+int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, const float *w_scale, const void *bias, const void *residual, void *y, int M,
+                     int N, int K, int act, int out_dtype, void *stream);
 
 /* ---- causal depthwise short convolution (q, k, v of the reference's layers pass through it first) ----
  * Replaces the convolution of ShortConvolution.forward / .step (fla/modules/convolution.py:142-216):
