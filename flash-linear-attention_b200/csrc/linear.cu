@@ -9,8 +9,10 @@
 //
 // Layout: a pair of CTAs works on a 256 x BN tile (cta_group::2), each CTA loading its 128 rows of A and its half of B, S stages of
 // 128-byte rows by TMA; the accumulator is double buffered in TMEM so that a tile's epilogue runs under the next tile's products.
-// The epilogue turns 32 x 64 blocks in shared memory, so that a warp's global reads and writes are whole rows of 128 bytes whatever
-// the row pitch of the outputs.
+// An epilogue thread holds a row of the accumulator; its results go through swizzled shared memory to TMA tile stores, and the
+// residual comes in the same way, a block ahead.  Outputs whose rows do not begin on 16-byte boundaries go through a transposition in
+// shared memory instead, so that a warp reads and writes runs of 64 bytes.  Tiles go in groups of 8 rows of tiles, so that what the
+// pairs work on at one time shares operands in L2.
 #include "tc.cuh"
 
 FLAB_TC_DEFINE_ERROR_WORD(linear_error)
@@ -47,7 +49,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 
 struct GemmParams {
   int M, N, K;          // C [M, N]; K: the summed extent
-  int tiles_n, tiles;
+  int tiles_m, tiles_n, tiles;
   void *c;              // [M, N]
   void *z;              // z before the activation, same type, or null
   const void *bias;     // [N] or null
@@ -58,21 +60,22 @@ struct GemmParams {
 };
 
 template <int BN> struct GemmShape {
-  static constexpr int S = BN == 256 ? 5 : BN == 128 ? 6 : 7;
+  static constexpr int S = BN == 256 ? 5 : 6;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
-  static constexpr int TURN = 32 * 64 * 4;  // a warp's block of 32 x 64 floats; 16-byte piece c of row r lies at c ^ (r & 7)
+  static constexpr int TURN = 2 * 4096;  // a warp's two blocks of 32 rows of 128 bytes; 16-byte piece c of row r lies at c ^ (r & 7)
   static constexpr int BYTES = S * STAGE + EPI_WARPS * TURN + 1024;
 };
 
-// TO: type of c, z, bias, residual.  F8: e4m3 operands, else 16 bits of type T16 (0 fp16, 1 bf16).  AMN / BMN: MN-major operands.
-template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI>
+// TS: outputs by tile stores.  TO: type of c, z, bias, residual.  F8: e4m3 operands, else 16 bits of type T16 (0 fp16, 1 bf16).  AMN / BMN: MN-major operands.
+template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI, bool TS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREADS, 1)
-    gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb) {
+    gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc,
+                const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap mr) {
   typedef GemmShape<BN> Z;
   constexpr int S = Z::S, BK = F8 ? 128 : 64;  // 128 bytes of each row
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2], res_full[Z::EPI_WARPS][2];
   __shared__ uint32_t tmem_base;
   uint8_t *const buf = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -84,6 +87,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) tc::mbar_init(&full[i], 1), tc::mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(&acc_full[i], 1), tc::mbar_init(&acc_empty[i], 2 * Z::EPI_WARPS);
+    for (int i = 0; i < Z::EPI_WARPS; ++i) tc::mbar_init(&res_full[i][0], 1), tc::mbar_init(&res_full[i][1], 1);
     tc::fence_barrier_init();
   }
   tc::fence_before_sync();
@@ -92,6 +96,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
   const int kblocks = (p.K + BK - 1) / BK;
+  auto place = [&](int tile, int &tm, int &tn) {  // groups of 8 rows of tiles, down the group's columns
+    const int group = tile / (8 * p.tiles_n), in = tile - group * 8 * p.tiles_n, high = min(8, p.tiles_m - group * 8);
+    tn = in / high;
+    tm = group * 8 + in - tn * high;
+  };
 
   if (warp == 0) {  // ---- loads
     if (lane == 0) {
@@ -100,7 +109,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       uint32_t it = 0;
       bool ok = true;
       for (int tile = cluster; tile < p.tiles && ok; tile += clusters) {
-        const int m0 = tile / p.tiles_n * 256 + rank * 128, n0 = tile % p.tiles_n * BN + rank * (BN / 2);
+        int tm, tn;
+        place(tile, tm, tn);
+        const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % S;
           if (it >= S && !tc::mbar_wait(&empty[s], (it / S - 1) & 1)) {
@@ -157,57 +168,229 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       }
     }
     __syncwarp();
-  } else if (warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 64 columns in turn
+  } else if (TS && warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 64 columns in turn
     const int w = warp - 4, quarter = w & 3, side = w >> 2;
-    float *const turn = reinterpret_cast<float *>(buf + S * Z::STAGE + w * Z::TURN);
+    uint8_t *const stage = buf + S * Z::STAGE + w * Z::TURN;
+    constexpr int BLOCKS = BN / 128;  // of this warp (with 64 columns, only side 0 has one)
+    const bool mine = BN > 64 || side == 0, two = !EPI || !p.z;  // two buffers in turn; with z the second one is z's
+    uint32_t seen = 0;  // parity of the residual blocks taken, a bit a buffer
     int n = 0;
     for (int tile = cluster; tile < p.tiles; tile += clusters, ++n) {
       const int half = n & 1;
+      int tm, tn;
+      place(tile, tm, tn);
+      const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN;
+      auto column = [&](int b) { return n0 + (2 * b + side) * 64; };
+      auto ask = [&](int b) {  // lane 0
+        const int q = two ? b & 1 : 0;
+        tc::mbar_expect_tx(&res_full[w][q], 4096);
+        tc::tma_load_2d(stage + q * 4096, &mr, &res_full[w][q], column(b), m0);
+      };
+      if (mine && lane == 0) {
+        tc::tma_store_wait_read();
+        if (EPI && p.res) {
+          ask(0);
+          if (two && BLOCKS > 1) ask(1);
+        }
+      }
+      __syncwarp();
+      float row_scale = 1.f;
+      if (F8 && m0 + lane < p.M) row_scale = p.row_scale[m0 + lane];
       if (!tc::mbar_wait(&acc_full[half], (n / 2) & 1)) {
         tu_tc_error = 733;
         break;
       }
       tc::fence_after_sync();
-      const int m0 = tile / p.tiles_n * 256 + rank * 128 + quarter * 32, n0 = tile % p.tiles_n * BN;
       const uint32_t from = tmem + half * BN + ((uint32_t)(quarter * 32) << 16);
-      const int rows = min(32, p.M - m0);
-      for (int cb = side; cb < BN / 64; cb += 2) {
-        float v[32];
+      bool ok = true;
+      if (mine) {
+#pragma unroll 1
+        for (int b = 0; b < (BLOCKS ? BLOCKS : 1); ++b) {
+          const int q = two ? b & 1 : 0, c0 = column(b);
+          uint8_t *const ybuf = stage + q * 4096 + lane * 128, *const zbuf = stage + 4096 + lane * 128;
+          if (b > 0 && !two) {
+            if (lane == 0) {
+              tc::tma_store_wait_read();
+              if (EPI && p.res) ask(b);
+            }
+            __syncwarp();
+          }
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            tc::tmem_ld_32x32b_x32(from + (2 * b + side) * 64 + h * 32, v);
+            const int c = c0 + h * 32;
+            float cs[F8 ? 32 : 1];
+            if (F8) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tc::tmem_ld_32x32b_x32(from + cb * 64 + h * 32, v);
-          tc::tmem_ld_wait();
+              for (int j = 0; j < 8; ++j) {
+                const float4 s = c + 4 * j < p.N ? *reinterpret_cast<const float4 *>(p.col_scale + c + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                cs[4 * j] = s.x, cs[4 * j + 1] = s.y, cs[4 * j + 2] = s.z, cs[4 * j + 3] = s.w;
+              }
+            }
+            struct alignas(16) Eight {
+              TO v[8];
+            };
+            Eight bias[4];
+            if (EPI && p.bias) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4 *>(turn + lane * 64 + (((h * 8 + j) ^ (lane & 7)) << 2)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              for (int j = 0; j < 4; ++j)
+                if (c + 8 * j < p.N) bias[j] = *reinterpret_cast<const Eight *>(reinterpret_cast<const TO *>(p.bias) + c + 8 * j);
+            }
+            tc::tmem_ld_wait();
+            if (F8) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = v[j] * row_scale * cs[j];
+            }
+            if (EPI && p.bias) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] += Num<TO>::f(bias[j >> 3].v[j & 7]);
+            }
+            auto piece = [&](uint8_t *row, int j) { return reinterpret_cast<Eight *>(row + (((h * 4 + j) ^ (lane & 7)) << 4)); };
+            if (EPI && p.z) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                Eight o;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
+                *piece(zbuf, j) = o;
+              }
+            }
+            if (EPI && p.act) {
+              switch (p.act) {  // one loop an activation: the choice is made once
+                case ACT_SILU:
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SILU);
+                  break;
+                case ACT_SIGMOID:
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SIGMOID);
+                  break;
+                case ACT_LOGSIGMOID:
+#pragma unroll 4
+                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_LOGSIGMOID);
+                  break;
+                default:
+#pragma unroll 4
+                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_GELU);
+                  break;
+              }
+            }
+            if (EPI && p.res) {
+              if (h == 0 && ok) {
+                ok = tc::mbar_wait(&res_full[w][q], (seen >> q) & 1);
+                if (!ok) tu_tc_error = 734;
+                seen ^= 1u << q;
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const Eight r = *piece(ybuf, j);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[8 * j + i] += Num<TO>::f(r.v[i]);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              Eight o;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
+              *piece(ybuf, j) = o;
+            }
+          }
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tc::tma_store_2d(&mc, stage + q * 4096, c0, m0);
+            if (EPI && p.z) tc::tma_store_2d(&mz, stage + 4096, c0, m0);
+            tc::tma_store_commit();
+          }
         }
-        __syncwarp();
-        const int c0 = n0 + cb * 64 + lane * 2;  // this lane's two columns
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
+      if (!__all_sync(0xffffffffu, ok)) break;
+    }
+    if (lane == 0) tc::tma_store_wait_all();
+    __syncwarp();
+  } else if (!TS && warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 32 columns in turn
+    const int w = warp - 4, quarter = w & 3, side = w >> 2;
+    float *const turn = reinterpret_cast<float *>(buf + S * Z::STAGE + w * Z::TURN);
+    const int odd = lane >> 4, pair = lane & 15;  // this lane's rows 2 i + odd and columns 2 pair, 2 pair + 1 of a block
+    struct alignas(2 * sizeof(TO)) Two {
+      TO v[2];
+    };
+    struct Ahead {  // what a block needs from memory
+      uint32_t res[16];  // two elements as they lie: nothing waits for a load before the block needs it
+      float2 bias, scale;
+    };
+    int n = 0;
+    for (int tile = cluster; tile < p.tiles; tile += clusters, ++n) {
+      const int half = n & 1;
+      int tm, tn;
+      place(tile, tm, tn);
+      const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN;
+      const int rows = min(32, p.M - m0);
+      auto ask = [&](int cb, Ahead &a) {
+        const int c0 = n0 + cb * 32 + pair * 2;
         const bool on0 = c0 < p.N, on1 = c0 + 1 < p.N;
-        float2 bias = make_float2(0.f, 0.f), scale = make_float2(1.f, 1.f);
+        a.bias = make_float2(0.f, 0.f), a.scale = make_float2(1.f, 1.f);
         if (EPI && p.bias) {
-          if (on0) bias.x = Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c0]);
-          if (on1) bias.y = Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c0 + 1]);
+          if (on0) a.bias.x = Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c0]);
+          if (on1) a.bias.y = Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c0 + 1]);
         }
         if (F8) {
-          if (on0) scale.x = p.col_scale[c0];
-          if (on1) scale.y = p.col_scale[c0 + 1];
+          if (on0) a.scale.x = p.col_scale[c0];
+          if (on1) a.scale.y = p.col_scale[c0 + 1];
         }
-        struct alignas(2 * sizeof(TO)) Two {
-          TO v[2];
-        };
-        auto get = [&](const void *q, size_t at) {
-          const TO *const e = reinterpret_cast<const TO *>(q) + at;
-          Two t;
-          if (p.pairs && on1) {
-            t = *reinterpret_cast<const Two *>(e);
+        if (EPI && p.res) {
+          const unsigned short *e = reinterpret_cast<const unsigned short *>(p.res) + (size_t)(m0 + odd) * p.N + c0;
+          if (p.pairs) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (2 * i + odd < rows && on0) a.res[i] = *reinterpret_cast<const uint32_t *>(e + 2 * i * (size_t)p.N);
           } else {
-            if (on0) t.v[0] = e[0];
-            if (on1) t.v[1] = e[1];
+            unsigned short lo[16], hi[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (2 * i + odd < rows && on0) lo[i] = e[2 * i * (size_t)p.N];
+              if (2 * i + odd < rows && on1) hi[i] = e[2 * i * (size_t)p.N + 1];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a.res[i] = lo[i] | (uint32_t)hi[i] << 16;
           }
-          return t;
-        };
-        auto set = [&](void *q, size_t at, float2 f) {
+        }
+      };
+      Ahead now, next;
+      ask(side, now);
+      float row_scale = 0.f;
+      if (F8 && lane < rows) row_scale = p.row_scale[m0 + lane];
+      if (!tc::mbar_wait(&acc_full[half], (n / 2) & 1)) {
+        tu_tc_error = 733;
+        break;
+      }
+      tc::fence_after_sync();
+      const uint32_t from = tmem + half * BN + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int cb = side; cb < BN / 32; cb += 2) {
+        float v[32];
+        tc::tmem_ld_32x32b_x32(from + cb * 32, v);
+        tc::tmem_ld_wait();
+        if (cb + 2 >= BN / 32) {  // the warp has taken its last block: the products may use this half again
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
+        } else {
+          ask(cb + 2, next);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4 *>(turn + lane * 32 + ((j ^ (lane & 7)) << 2)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        __syncwarp();
+        const int c0 = n0 + cb * 32 + pair * 2;
+        const bool on0 = c0 < p.N, on1 = c0 + 1 < p.N;
+        size_t at = (size_t)(m0 + odd) * p.N + c0;
+        auto set = [&](void *q, float2 f) {
           TO *const e = reinterpret_cast<TO *>(q) + at;
           Two t;
           t.v[0] = Num<TO>::t(f.x), t.v[1] = Num<TO>::t(f.y);
@@ -218,36 +401,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
             if (on1) e[1] = t.v[1];
           }
         };
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-          Two res[8];
-          if (EPI && p.res) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (r0 + i < rows) res[i] = get(p.res, (size_t)(m0 + r0 + i) * p.N + c0);
+        for (int i = 0; i < 16; ++i, at += 2 * (size_t)p.N) {
+          const int r = 2 * i + odd;
+          float2 f = *reinterpret_cast<const float2 *>(turn + r * 32 + (((pair >> 1) ^ (r & 7)) << 2) + (pair & 1) * 2);
+          if (F8) {
+            const float rs = __shfl_sync(0xffffffffu, row_scale, r);
+            f.x = f.x * rs * now.scale.x, f.y = f.y * rs * now.scale.y;
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (r0 + i >= rows) break;
-            float2 f = *reinterpret_cast<const float2 *>(turn + (r0 + i) * 64 + (((lane >> 1) ^ i) << 2) + (lane & 1) * 2);  // r0 % 8 == 0
-            const size_t at = (size_t)(m0 + r0 + i) * p.N + c0;
-            if (F8) {
-              const float rs = p.row_scale[m0 + r0 + i];
-              f.x = f.x * rs * scale.x, f.y = f.y * rs * scale.y;
+          if (r >= rows) continue;
+          if (EPI) {
+            f.x += now.bias.x, f.y += now.bias.y;
+            if (p.z) set(p.z, f);
+            if (p.act) f.x = act_fwd(f.x, p.act), f.y = act_fwd(f.y, p.act);
+            if (p.res) {
+              const Two r2 = *reinterpret_cast<const Two *>(&now.res[i]);
+              f.x += Num<TO>::f(r2.v[0]), f.y += Num<TO>::f(r2.v[1]);
             }
-            if (EPI) {
-              f.x += bias.x, f.y += bias.y;
-              if (p.z) set(p.z, at, f);
-              if (p.act) f.x = act_fwd(f.x, p.act), f.y = act_fwd(f.y, p.act);
-              if (p.res) f.x += Num<TO>::f(res[i].v[0]), f.y += Num<TO>::f(res[i].v[1]);
-            }
-            set(p.c, at, f);
           }
+          set(p.c, f);
         }
         __syncwarp();
+        now = next;
       }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
+      if (side >= BN / 32) {  // no block of this tile is this warp's
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
+      }
     }
   }
   tc::fence_before_sync();
@@ -332,8 +512,8 @@ int operand_map(CUtensorMap *map, const void *base, int dtype, long long rows, i
   return make_tensor_map(map, base, type, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI>
-int launch_gemm_bn(GemmParams p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
+template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI, bool TS>
+int launch_gemm_ts(GemmParams p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
   typedef GemmShape<BN> Z;
   const int bk = F8 ? 128 : 64;
   CUtensorMap ma, mb;
@@ -342,24 +522,41 @@ int launch_gemm_bn(GemmParams p, const void *a, int a_pitch, const void *b, int 
   rc = BMN ? operand_map(&mb, b, dtype, p.K, p.N, b_pitch, 64, 64) : operand_map(&mb, b, dtype, p.N, p.K, b_pitch, bk, BN / 2);
   if (rc) return rc;
   p.tiles_n = (p.N + BN - 1) / BN;
-  const long long tiles = (long long)((p.M + 255) / 256) * p.tiles_n;
+  p.tiles_m = (p.M + 255) / 256;
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
   FLAB_REQUIRE(tiles < (1 << 30), FLAB_E_UNSUPPORTED, "linear: %d x %d is too large", p.M, p.N);
   p.tiles = (int)tiles;
-  auto kernel = gemm_kernel<TO, F8, T16, AMN, BMN, BN, EPI>;
+  CUtensorMap mc = ma, mz = ma, mr = ma;  // (a map that is not used may be any)
+  if (TS) {
+    const int out = Num<TO>::id;
+    if ((rc = operand_map(&mc, p.c, out, p.M, p.N, p.N, 64, 32))) return rc;
+    if (p.z && (rc = operand_map(&mz, p.z, out, p.M, p.N, p.N, 64, 32))) return rc;
+    if (p.res && (rc = operand_map(&mr, p.res, out, p.M, p.N, p.N, 64, 32))) return rc;
+  }
+  auto kernel = gemm_kernel<TO, F8, T16, AMN, BMN, BN, EPI, TS>;
   if ((rc = set_smem(kernel, Z::BYTES))) return rc;
   const int clusters = sm_count() / 2;
-  kernel<<<2 * (p.tiles < clusters ? p.tiles : clusters), Z::THREADS, Z::BYTES, st>>>(p, ma, mb);
+  kernel<<<2 * (p.tiles < clusters ? p.tiles : clusters), Z::THREADS, Z::BYTES, st>>>(p, ma, mb, mc, mz, mr);
   return check_launch("linear");
 }
 
-// The widest tile that still gives every pair of SMs one: with fewer tiles than pairs the time is the length of one tile, and a
-// narrower one is shorter.
+template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI>
+int launch_gemm_bn(const GemmParams &p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
+  bool ts = p.N % 8 == 0;
+  for (const void *q : {(const void *)p.c, (const void *)p.z, p.res, p.bias, (const void *)p.col_scale}) ts = ts && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+  return ts ? launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, true>(p, a, a_pitch, b, b_pitch, dtype, st)
+            : launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, false>(p, a, a_pitch, b, b_pitch, dtype, st);
+}
+
+// The tile's width by the time of the rounds it takes: a round of 256 columns costs 256, of 128 columns 160 and of 64 columns 110
+// (a narrower tile reads the same rows of A for fewer products; measured on 4096 x 4096 x 4096 and 256 x 2048 x 2048, bf16).
 template <typename TO, bool F8, int T16, bool AMN, bool BMN, bool EPI>
 int launch_gemm(const GemmParams &p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
-  const long long rows = (p.M + 255) / 256;
-  const int clusters = sm_count() / 2;
-  if (rows * ((p.N + 255) / 256) >= clusters) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 256, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
-  if (BMN || rows * ((p.N + 127) / 128) >= clusters) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 128, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
+  const long long rows = (p.M + 255) / 256, clusters = sm_count() / 2;
+  auto cost = [&](int bn, int each) { return (rows * ((p.N + bn - 1) / bn) + clusters - 1) / clusters * each; };
+  const long long c256 = cost(256, 256), c128 = cost(128, 160), c64 = BMN ? c256 + c128 : cost(64, 110);
+  if (c256 <= c128 && c256 <= c64) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 256, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
+  if (c128 <= c64) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 128, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
   if constexpr (!BMN) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 64, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
   return FLAB_E_UNSUPPORTED;
 }
