@@ -257,7 +257,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
               }
             }
             if (EPI && p.act) {
-              switch (p.act) {  // one loop an activation: the choice is made once
+              switch (p.act) {  // one loop an activation, unrolled whole: a loop over v would put it in local memory
                 case ACT_SILU:
 #pragma unroll
                   for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SILU);
@@ -267,11 +267,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
                   for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SIGMOID);
                   break;
                 case ACT_LOGSIGMOID:
-#pragma unroll 4
+#pragma unroll
                   for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_LOGSIGMOID);
                   break;
                 default:
-#pragma unroll 4
+#pragma unroll
                   for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_GELU);
                   break;
               }
