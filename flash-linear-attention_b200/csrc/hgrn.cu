@@ -339,6 +339,27 @@ template <typename T> __device__ __forceinline__ void pack2(T *s, float a, float
   v.v[0] = Num<T>::t(a), v.v[1] = Num<T>::t(b);
   *reinterpret_cast<Pack<T, 2> *>(s) = v;
 }
+// The codes of the L rows from t0 on, by a warp: `n` is the last sequence that begins at or before t0 (-1: none).  Only the sequences
+// that lie in the tile are looked at; a row between two edges has code 0.
+template <int L> __device__ __forceinline__ void tile_codes(const HgrnParams &p, long long t0, int n, int *code, int lane) {
+  const long long begin = cu_at(p, 0), end = cu_at(p, p.N) < p.T ? cu_at(p, p.N) : p.T;
+  for (int r = lane; r < L; r += 32) code[r] = t0 + r < begin || t0 + r >= end ? ROW_OUT : 0;
+  __syncwarp();
+  for (int j0 = n < 0 ? 0 : n;; j0 += 32) {
+    const int j = j0 + lane;
+    bool inside = false;
+    if (j < p.N) {
+      const long long s = cu_at(p, j) - t0, e = cu_at(p, j + 1) - t0;  // first row, and the one behind the last
+      inside = s < L;
+      if (inside && s < e) {
+        if (s >= 0) code[s] = (j << ROW_SHIFT) | ROW_START | (e == s + 1 ? ROW_END : 0);
+        if (e > 0 && e <= L && e != s + 1) code[e - 1] = (j << ROW_SHIFT) | ROW_END;
+      }
+    }
+    if (!__all_sync(0xffffffffu, inside)) break;
+  }
+}
+
 template <typename T, int R, int S, bool BWD> struct Stream {
   static constexpr int V = 2, C = 32 * V, W = 8, L = W * R;
   static constexpr int TILE = L * C, TENSORS = BWD ? 3 : 2;
@@ -359,6 +380,8 @@ template <typename T, int R, int S, bool BWD> struct Stream {
     uint64_t full[S], mapped[S], ready[S], done[S], empty[S];
   };
 };
+
+template <bool BWD, int L, int R> __device__ __forceinline__ int row_of(int w, int r) { return BWD ? L - 1 - (w * R + r) : w * R + r; }
 
 template <typename T, int R, int S, bool BWD, bool VAR>
 __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
@@ -384,8 +407,13 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
     tc::fence_barrier_init();
   }
   __syncthreads();
+  // the codes of warp w's rows: bit r of the result where position r has one, lane r holds it
+  auto codes_of = [&](int edges, const int *code, int w, int &mine) {
+    mine = edges ? code[row_of<BWD, L, R>(w, lane % R)] : 0;
+    return __ballot_sync(0xffffffffu, mine != 0) & ((1u << R) - 1);
+  };
   // position r of warp w's rows is this row of the tile
-  auto row = [&](int w, int r) -> int { return BWD ? L - 1 - (w * R + r) : w * R + r; };
+  auto row = [&](int w, int r) -> int { return row_of<BWD, L, R>(w, r); };
 
   if (warp < W) {  // ---- map warps
     const int w = warp;
@@ -405,20 +433,27 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         Q.y = BWD ? a.y * (Q.y + x.y) : fmaf(a.y, Q.y, x.y);
         P.x *= a.x, P.y *= a.y;
       };
-      if (!VAR || !sh.at[s].edges) {
+      int mine = 0;
+      const unsigned codes = VAR ? codes_of(sh.at[s].edges, st.code, w, mine) : 0;
+      if (!VAR || codes == 0) {
 #pragma unroll
         for (int r = 0; r < R; ++r) take(unpack2(gs + row(w, r) * C), unpack2(xs + row(w, r) * C));
       } else {
+        // kept short: unrolled, this rarely run code cost more in instruction fetches than it saved
         const int ch = sh.at[s].cg * C + lane * 2;
-#pragma unroll 4
+#pragma unroll 1
         for (int r = 0; r < R; ++r) {
-          const int code = st.code[row(w, r)];
-          const bool out = code & ROW_OUT;
-          if (code & (ROW_OUT | AHEAD)) {
-            P = make_float2(CUT, CUT);
-            Q = out || !edge || ch >= p.D ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2 *>(edge + (size_t)(code >> ROW_SHIFT) * p.D + ch);
+          const float2 g = unpack2(gs + row(w, r) * C), x = unpack2(xs + row(w, r) * C);
+          bool out = false;
+          if (codes >> r & 1) {
+            const int code = __shfl_sync(0xffffffffu, mine, r);
+            out = code & ROW_OUT;
+            if (code & (ROW_OUT | AHEAD)) {
+              P = make_float2(CUT, CUT);
+              Q = out || !edge || ch >= p.D ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2 *>(edge + (size_t)(code >> ROW_SHIFT) * p.D + ch);
+            }
           }
-          if (!out) take(unpack2(gs + row(w, r) * C), unpack2(xs + row(w, r) * C));
+          if (!out) take(g, x);
         }
       }
       st.P[w][lane] = P;
@@ -459,7 +494,9 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         }
       };
       const float2 none = make_float2(0.f, 0.f);
-      if (!VAR || !sh.at[s].edges) {
+      int mine = 0;
+      const unsigned codes = VAR ? codes_of(z.edges, st.code, w, mine) : 0;
+      if (!VAR || codes == 0) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const int at = row(w, r) * C;
@@ -469,21 +506,26 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
           take(at, unpack2(gs + at), unpack2(xs + at), h);
         }
       } else {
-#pragma unroll 2
+#pragma unroll 1
         for (int r = 0; r < R; ++r) {
-          const int at = row(w, r) * C, code = st.code[row(w, r)];
-          const size_t of = (size_t)(code >> ROW_SHIFT) * p.D + ch;
+          const int at = row(w, r) * C;
+          const float2 g = unpack2(gs + at), x = unpack2(xs + at);
+          float2 h = BWD ? unpack2(os + at) : none;
+          int code = 0;
+          if (codes >> r & 1) {
+            code = __shfl_sync(0xffffffffu, mine, r);
+            const size_t of = (size_t)(code >> ROW_SHIFT) * p.D + ch;
+            if (code & AHEAD) c = edge && on ? *reinterpret_cast<const float2 *>(edge + of) : none;
+            if (BWD && (code & ROW_START)) h = p.h0 && on ? *reinterpret_cast<const float2 *>(p.h0 + of) : none;
+          }
           if (code & ROW_OUT) {
             c = none;
             pack2(xs + at, 0.f, 0.f);
             if (BWD) pack2(gs + at, 0.f, 0.f);
-            continue;
+          } else {
+            take(at, g, x, h);
+            if ((code & (BWD ? ROW_START : ROW_END)) && p.ht && on) *reinterpret_cast<float2 *>(p.ht + (size_t)(code >> ROW_SHIFT) * p.D + ch) = c;
           }
-          if (code & AHEAD) c = edge && on ? *reinterpret_cast<const float2 *>(edge + of) : none;
-          float2 h = BWD ? unpack2(os + at) : none;
-          if (BWD && (code & ROW_START)) h = p.h0 && on ? *reinterpret_cast<const float2 *>(p.h0 + of) : none;
-          take(at, unpack2(gs + at), unpack2(xs + at), h);
-          if ((code & (BWD ? ROW_START : ROW_END)) && p.ht && on) *reinterpret_cast<float2 *>(p.ht + of) = c;
         }
       }
       // rows past T are the identity, so the last warp's last value is the sequence's
@@ -534,65 +576,71 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       float2 c = make_float2(0.f, 0.f);
       if (group > 0) e[0] = look(words(p.ends, group - 1)), e[1] = look(words(p.ends, group - 1) + 1);
       else if (!VAR && edge && ch < p.D) c = *reinterpret_cast<const float2 *>(edge + (size_t)z.b * p.D + ch);
+      // the group's earlier tiles as one map, so that little is left to do once the end of the group before is there: that end to
+      // the next one is what is serial along time
+      float2 gP = make_float2(1.f, 1.f), gQ = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < G - 1; ++i)
-        if (i < before) m[i][0] = await(words(p.maps, first + i), m[i][0]), m[i][1] = await(words(p.maps, first + i) + 1, m[i][1]);
+        if (i < before) {
+          const float2 mx = map_of(await(words(p.maps, first + i), m[i][0])), my = map_of(await(words(p.maps, first + i) + 1, m[i][1]));
+          gQ.x = through(mx.x, mx.y, gQ.x), gQ.y = through(my.x, my.y, gQ.y);
+          gP.x = is_cut(mx.x) ? CUT : gP.x * mx.x, gP.y = is_cut(my.x) ? CUT : gP.y * my.x;
+        }
       if (group > 0) {
         c.x = end_of(await(words(p.ends, group - 1), e[0]));
         c.y = end_of(await(words(p.ends, group - 1) + 1, e[1]));
       }
-#pragma unroll
-      for (int i = 0; i < G - 1; ++i)
-        if (i < before) {
-          const float2 mx = map_of(m[i][0]), my = map_of(m[i][1]);
-          c.x = through(mx.x, mx.y, c.x), c.y = through(my.x, my.y, c.y);
-        }
+      c.x = through(gP.x, gQ.x, c.x), c.y = through(gP.y, gQ.y, c.y);
+      if (leader) {
+        put(words(p.ends, group), end_word(through(jP.x, jQ.x, c.x)));
+        put(words(p.ends, group) + 1, end_word(through(jP.y, jQ.y, c.y)));
+      }
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float2 P = st.P[i][lane], Q = st.Q[i][lane];
         st.P[i][lane] = c;
         c.x = through(P.x, Q.x, c.x), c.y = through(P.y, Q.y, c.y);
       }
-      if (leader) {
-        put(words(p.ends, group), end_word(c.x));
-        put(words(p.ends, group) + 1, end_word(c.y));
-      }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sh.ready[s]);
     }
   } else if (warp == 2 * W + Z::CHAINS) {  // ---- load warp
+    int tile = 0;
+    if (lane == 0) tile = atomicAdd(p.ticket, 1);
+    tile = __shfl_sync(0xffffffffu, tile, 0);
     for (int it = 0;; ++it) {
       const int s = it % S;
-      int tile = 0;
-      if (lane == 0) tile = atomicAdd(p.ticket, 1);  // its way to L2 falls into the wait for the stage
-      if (it >= S && !tc::mbar_wait(&sh.empty[s], (it / S - 1) & 1)) {
-        tu_tc_error = 707;
-        break;
-      }
-      __syncwarp();
-      tile = __shfl_sync(0xffffffffu, tile, 0);
+      // what the tile's place takes (and the next ticket) falls into the wait for the stage
       const bool more = tile < tiles;
       typename Z::Shared::Place z;
       z.step = -1;
+      int following = 0, first_seq = 0;
       if (more) {
-        typename Z::Stage &st = sh.st[s];
+        if (lane == 0) following = atomicAdd(p.ticket, 1);
         z.step = tile / chains;
         z.chain = tile - z.step * chains;
         z.b = z.chain / p.nCG;
         z.cg = z.chain - z.b * p.nCG;
         z.t0 = (BWD ? p.nT - 1 - z.step : z.step) * L;
         z.edges = 0;
+        if (VAR) {  // most tiles lie inside one sequence
+          first_seq = warp_count(p, z.t0, lane) - 1;
+          z.edges = first_seq < 0 || first_seq >= p.N || cu_at(p, first_seq) == z.t0 || cu_at(p, first_seq + 1) <= z.t0 + L;
+        }
+      }
+      if (it >= S && !tc::mbar_wait(&sh.empty[s], (it / S - 1) & 1)) {
+        tu_tc_error = 707;
+        break;
+      }
+      __syncwarp();
+      if (more) {
+        typename Z::Stage &st = sh.st[s];
         if (lane == 0) {
           tc::tma_load_3d(st.buf[1], &mg, &sh.full[s], z.cg * C, z.t0, z.b);
           tc::tma_load_3d(st.buf[0], &mx, &sh.full[s], z.cg * C, z.t0, z.b);
           if (BWD) tc::tma_load_3d(st.buf[Z::TENSORS - 1], &mo, &sh.full[s], z.cg * C, z.t0 - 1, z.b);
         }
-        if (VAR) {  // most tiles lie inside one sequence
-          const int n = warp_count(p, z.t0, lane) - 1;
-          z.edges = n < 0 || n >= p.N || cu_at(p, n) == z.t0 || cu_at(p, n + 1) <= z.t0 + L;
-          if (z.edges)
-            for (int r = lane; r < L; r += 32) st.code[r] = z.t0 + r < p.T ? row_code(p, z.t0 + r) : ROW_OUT;
-        }
+        if (VAR && z.edges) tile_codes<L>(p, z.t0, first_seq, st.code, lane);
       }
       __syncwarp();
       if (lane == 0) {
@@ -615,6 +663,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         }
         break;
       }
+      tile = __shfl_sync(0xffffffffu, following, 0);
     }
   } else if (lane == 0) {  // ---- store warp
     for (int it = 0;; ++it) {
@@ -748,7 +797,7 @@ template <typename T, bool BWD, bool VAR> int launch_stream(HgrnParams p, void *
   CUtensorMap m[5];
   const void *base[5] = {p.x, p.g, BWD ? p.o_in : p.x, p.o, BWD ? p.dg : p.o};
   for (int i = 0; i < 5; ++i)
-    if ((rc = make_tensor_map(&m[i], base[i], type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE))) return rc;
+    if ((rc = make_tensor_map(&m[i], base[i], type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))) return rc;
   auto kernel = hgrn_stream_kernel<T, R, S, BWD, VAR>;
   const int bytes = (int)sizeof(typename Z::Shared);
   if ((rc = set_smem(kernel, bytes))) return rc;

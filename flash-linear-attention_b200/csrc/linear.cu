@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T *__restrict__ dy, 
     }
 }
 
-constexpr int RUN = 256;  // rows of a partial column sum
+constexpr int RUN = 128;  // rows of a partial column sum
 
 template <typename T>
 int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, int N, int pitch, int act, cudaStream_t st) {

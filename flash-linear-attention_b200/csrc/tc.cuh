@@ -324,7 +324,7 @@ int make_state_map(CUtensorMap *map, const void *base, const flab_args *a, int b
 
 // host: tensor-map construction without linking libcuda (entry point fetched from the runtime)
 int make_tensor_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
-                    const uint32_t *box, CUtensorMapSwizzle swizzle);
+                    const uint32_t *box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 int make_tensor_map_bf16(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
                          const uint32_t *box, int elem_fp16);
 

@@ -23,7 +23,7 @@ static EncodeTiledFn encode_fn() {
 
 // rank <= 4; dims[0] is the contiguous extent; strides_bytes[i] is the stride of dims[i+1].  Zero fill outside the tensor.
 int make_tensor_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
-                    const uint32_t *box, CUtensorMapSwizzle swizzle) {
+                    const uint32_t *box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   EncodeTiledFn fn = encode_fn();
   // A driver-API call needs a current context; a thread that has only used the runtime lazily (an
   // autograd worker thread, say) may not have bound the primary context yet.  cudaSetDevice binds it
@@ -45,7 +45,7 @@ int make_tensor_map(CUtensorMap *map, const void *base, CUtensorMapDataType type
     if (i + 1 < rank) gstr[i] = strides_bytes[i];
   }
   CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void *>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   FLAB_REQUIRE(r == CUDA_SUCCESS, FLAB_E_BADARG, "cuTensorMapEncodeTiled failed with code %d (base %p must be 16-byte aligned, strides multiples of 16)",
                (int)r, base);
   return 0;

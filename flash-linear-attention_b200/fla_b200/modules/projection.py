@@ -26,8 +26,16 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x.reshape(math.prod(x.shape[:-1]), x.shape[-1]).contiguous()
 
 
-def _workspace(n: int, dev):
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+def _like(t: torch.Tensor, shape) -> torch.Tensor:
+    return t if t.shape == shape else t.reshape(shape)
+
+
+def _workspace(lib, x2, w, M, N, K, backward):
+    """(scratch, its bytes): none where the operands lie as the kernel reads them."""
+    if not backward and K % 8 == 0 and x2.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0:
+        return None, 0
+    n = lib.flab_linear_workspace(_p(x2), _p(w), M, N, K, backward)
+    return (torch.empty(n, dtype=torch.uint8, device=(w if x2 is None else x2).device) if n else None), n
 
 
 def _forward(x2, w, b, r2, act, want_z):
@@ -36,8 +44,7 @@ def _forward(x2, w, b, r2, act, want_z):
     z = torch.empty_like(y) if want_z else None
     if M:
         lib = _lib.load()
-        n = lib.flab_linear_workspace(x2.data_ptr(), w.data_ptr(), M, N, K, 0)
-        ws = _workspace(n, x2.device)
+        ws, n = _workspace(lib, x2, w, M, N, K, 0)
         with _lib.device_of(x2):
             rc = lib.flab_linear_fwd(x2.data_ptr(), w.data_ptr(), _p(b), _p(r2), y.data_ptr(), _p(z), M, N, K, act, _DTYPES[x2.dtype], _p(ws), n,
                                      _lib.stream_of(x2))
@@ -55,7 +62,7 @@ class LinearFunction(torch.autograd.Function):
                         act != 0 and (need_x or need_w or need_b))
         ctx.save_for_backward(x2 if need_w else None, w if need_x else None, z)
         ctx.act, ctx.sizes, ctx.x_shape = act, (x2.shape[0], w.shape[0], w.shape[1]), x.shape
-        return y.reshape(x.shape[:-1] + (w.shape[0],))
+        return _like(y, x.shape[:-1] + (w.shape[0],))
 
     @staticmethod
     @once_differentiable
@@ -73,14 +80,15 @@ class LinearFunction(torch.autograd.Function):
                     t.zero_()
         elif need_x or need_w or need_b:
             lib = _lib.load()
-            n = lib.flab_linear_workspace(_p(x2), _p(w), M, N, K, 1)
-            ws = _workspace(n, dev)
+            # dz is a tensor of its own where an activation or dy's rows make one
+            own_dz = (need_x or need_w) and (ctx.act != 0 or N % 8 != 0 or d2.data_ptr() % 16 != 0)
+            ws, n = _workspace(lib, x2, w, M, N, K, 1) if own_dz or K % 8 or x2 is not None and x2.data_ptr() % 16 or w is not None and w.data_ptr() % 16 else (None, 0)
             part = torch.empty(lib.flab_linear_bwd_partials(M), N, dtype=torch.float32, device=dev) if need_b else None
             with _lib.device_of(d2):
                 rc = lib.flab_linear_bwd(_p(x2), _p(w), _p(z), d2.data_ptr(), _p(dx), _p(dw), _p(db), _p(part), M, N, K, ctx.act, _DTYPES[dy.dtype],
                                          _p(ws), n, _lib.stream_of(d2))
             _lib.finish("flab_linear_bwd", rc)
-        return (None if dx is None else dx.reshape(ctx.x_shape)), dw, db, (dy if need_r else None), None
+        return (None if dx is None else _like(dx, ctx.x_shape)), dw, db, (dy if need_r else None), None
 
 
 def _check(x, weight, bias, residual, activation, dtype):
@@ -113,7 +121,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LinearFunction.apply(x, weight, bias, residual, act)
     y, _ = _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False)
-    return y.reshape(x.shape[:-1] + (weight.shape[0],))
+    return _like(y, x.shape[:-1] + (weight.shape[0],))
 
 
 def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -147,4 +155,4 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
             rc = lib.flab_linear_e4m3(x2.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), _p(b), _p(r2), y.data_ptr(), M, N, K,
                                       ACTIVATIONS[activation], _DTYPES[out_dtype], _lib.stream_of(x2))
         _lib.finish("flab_linear_e4m3", rc)
-    return y.reshape(x.shape[:-1] + (N,))
+    return _like(y, x.shape[:-1] + (N,))
