@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       if (lane == 0) tc::mbar_arrive(&sh.ready[s]);
     }
   } else if (warp == 2 * W + Z::CHAINS) {  // ---- load warp
-    int tile = 0;
+    int tile = 0, first_seq = BWD ? p.N : 0;  // the last sequence that begins at or before the tile (packed batches)
     if (lane == 0) tile = atomicAdd(p.ticket, 1);
     tile = __shfl_sync(0xffffffffu, tile, 0);
     for (int it = 0;; ++it) {
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       const bool more = tile < tiles;
       typename Z::Shared::Place z;
       z.step = -1;
-      int following = 0, first_seq = 0;
+      int following = 0;
       if (more) {
         if (lane == 0) following = atomicAdd(p.ticket, 1);
         z.step = tile / chains;
@@ -624,8 +624,18 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         z.t0 = (BWD ? p.nT - 1 - z.step : z.step) * L;
         z.edges = 0;
         if (VAR) {  // most tiles lie inside one sequence
-          first_seq = warp_count(p, z.t0, lane) - 1;
-          z.edges = first_seq < 0 || first_seq >= p.N || cu_at(p, first_seq) == z.t0 || cu_at(p, first_seq + 1) <= z.t0 + L;
+          // tickets go along time: the sequence is found among the 32 next to the last tile's, with one load
+          const int from = max(BWD ? first_seq - 30 : first_seq, 0);
+          const long long v = cu_at(p, min(from + lane, p.N));
+          const int below = __popc(__ballot_sync(0xffffffffu, from + lane <= p.N && v <= z.t0));
+          if ((below > 0 || from == 0) && below < 32) {
+            first_seq = from + below - 1;
+            const long long b0 = __shfl_sync(0xffffffffu, v, max(below - 1, 0)), b1 = __shfl_sync(0xffffffffu, v, below);
+            z.edges = first_seq < 0 || first_seq >= p.N || b0 == z.t0 || b1 <= z.t0 + L;
+          } else {
+            first_seq = warp_count(p, z.t0, lane) - 1;
+            z.edges = first_seq < 0 || first_seq >= p.N || cu_at(p, first_seq) == z.t0 || cu_at(p, first_seq + 1) <= z.t0 + L;
+          }
         }
       }
       if (it >= S && !tc::mbar_wait(&sh.empty[s], (it / S - 1) & 1)) {

@@ -494,12 +494,21 @@ int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, 
   return check_launch("linear_bwd");
 }
 
-// rows of `n` elements to rows of `pitch`
-template <typename T> __global__ void __launch_bounds__(256) repitch_kernel(const T *__restrict__ from, T *__restrict__ to, int rows, int n, int pitch) {
+// Rows of n elements to rows of `pitch`, for one or two matrices in a launch.
+struct Repitch {
+  const unsigned short *from;
+  unsigned short *to;
+  int rows, n, pitch;
+};
+__global__ void __launch_bounds__(256) repitch_kernel(const Repitch a, const Repitch b) {
   const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows + b.rows; r += gridDim.x * 8) {
+    const bool second = r >= a.rows;
+    const int row = second ? r - a.rows : r, n = second ? b.n : a.n;
+    const unsigned short *from = (second ? b.from : a.from) + (size_t)row * n;
+    unsigned short *to = (second ? b.to : a.to) + (size_t)row * (second ? b.pitch : a.pitch);
 #pragma unroll 4
-    for (int c = lane; c < n; c += 32) to[(size_t)r * pitch + c] = from[(size_t)r * n + c];
+    for (int c = lane; c < n; c += 32) to[c] = from[c];
   }
 }
 
@@ -567,24 +576,29 @@ template <typename... Ptr> bool four(int n, Ptr... ptr) {
   return ok;
 }
 
-// An operand's rows as TMA needs them (16-byte address and pitch): where they lie, or copied into the caller's scratch.
-struct Scratch {
-  char *at;
-  size_t left;
-};
+// Operands' rows as TMA needs them (16-byte address and pitch): where they lie, or copied into the caller's scratch.
 int pitch_of(int n) { return (n + 7) / 8 * 8; }
 bool as_is(const void *p, int n) { return n % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 size_t copy_bytes(long long rows, int n) { return ((size_t)rows * pitch_of(n) * 2 + 255) / 256 * 256; }
-int operand(const void *&p, int &pitch, int rows, int n, Scratch &ws, cudaStream_t st) {
-  pitch = pitch_of(n);
-  if (as_is(p, n)) return FLAB_OK;
-  const size_t need = copy_bytes(rows, n);
-  FLAB_REQUIRE(ws.at && ws.left >= need, FLAB_E_BADARG, "linear needs a workspace of flab_linear_workspace() bytes");
-  const int blocks = rows / 8 + 1, cap = sm_count() * 8;
-  repitch_kernel<unsigned short><<<blocks < cap ? blocks : cap, 256, 0, st>>>(reinterpret_cast<const unsigned short *>(p),
-                                                                             reinterpret_cast<unsigned short *>(ws.at), rows, n, pitch);
-  p = ws.at;
-  ws.at += need, ws.left -= need;
+struct Operands {
+  const void *x, *w;
+  size_t bytes;  // of copies in the scratch
+};
+// x [M, K] and weight [N, K]; with `copied` the scratch holds the copies already (of the forward call)
+int operands(Operands &o, const void *x, const void *w, int M, int N, int K, void *ws, size_t ws_bytes, bool copied, cudaStream_t st) {
+  o.x = x, o.w = w, o.bytes = 0;
+  const size_t xb = as_is(x, K) ? 0 : copy_bytes(M, K), wb = as_is(w, K) ? 0 : copy_bytes(N, K);
+  if (xb + wb == 0) return FLAB_OK;
+  FLAB_REQUIRE(ws && ws_bytes >= xb + wb, FLAB_E_BADARG, "linear needs a workspace of flab_linear_workspace() bytes");
+  char *const at = reinterpret_cast<char *>(ws);
+  const Repitch a = {(const unsigned short *)x, (unsigned short *)at, xb ? M : 0, K, pitch_of(K)};
+  const Repitch b = {(const unsigned short *)w, (unsigned short *)(at + xb), wb ? N : 0, K, pitch_of(K)};
+  o.bytes = xb + wb;
+  if (xb) o.x = a.to;
+  if (wb) o.w = b.to;
+  if (copied) return FLAB_OK;
+  const int blocks = (a.rows + b.rows + 7) / 8, cap = sm_count() * 8;
+  repitch_kernel<<<blocks < cap ? blocks : cap, 256, 0, st>>>(a, b);
   return check_launch("linear repitch");
 }
 
@@ -596,13 +610,16 @@ int sum_partials(const float *part, void *out, int parts, int n, int dtype, cuda
 
 extern "C" {
 
-// scratch of the forward product (backward = 0), or of the backward ones
-size_t flab_linear_workspace(const void *x, const void *weight, int M, int N, int K, int backward) {
+size_t flab_linear_workspace(const void *x, const void *weight, int M, int N, int K) {
   using namespace flab;
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  size_t n = (as_is(x, K) ? 0 : copy_bytes(M, K)) + (as_is(weight, K) ? 0 : copy_bytes(N, K));
-  if (backward) n += copy_bytes(M, N);
-  return n;
+  return (as_is(x, K) ? 0 : copy_bytes(M, K)) + (as_is(weight, K) ? 0 : copy_bytes(N, K));
+}
+
+size_t flab_linear_bwd_workspace(const void *dy, int M, int N, int act) {
+  using namespace flab;
+  if (M <= 0 || N <= 0) return 0;
+  return act == ACT_NONE && as_is(dy, N) ? 0 : copy_bytes(M, N);
 }
 
 int flab_linear_fwd(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *z, int M, int N, int K, int act, int dtype,
@@ -614,38 +631,41 @@ int flab_linear_fwd(const void *x, const void *weight, const void *bias, const v
   if (M == 0) return FLAB_OK;
   FLAB_REQUIRE(x && weight && y, FLAB_E_BADARG, "linear_fwd needs x, weight, y");
   FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0, FLAB_E_BADARG, "linear_fwd: ws must be 256-byte aligned");
-  Scratch s = {reinterpret_cast<char *>(ws), ws_bytes};
+  Operands o;
+  int rc = operands(o, x, weight, M, N, K, ws, ws_bytes, false, st);
+  if (rc) return rc;
   GemmParams p = {};
   p.M = M, p.N = N, p.K = K, p.c = y, p.z = z, p.bias = bias, p.res = residual, p.act = act;
   p.pairs = four(N, y, z, residual);
-  int xp, wp, rc;
-  if ((rc = operand(x, xp, M, K, s, st)) || (rc = operand(weight, wp, N, K, s, st))) return rc;
-  return dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, false, true>(p, x, xp, weight, wp, dtype, st)
-                            : launch_gemm<__half, false, 0, false, false, true>(p, x, xp, weight, wp, dtype, st);
+  const int kp = pitch_of(K);
+  return dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, false, true>(p, o.x, kp, o.w, kp, dtype, st)
+                            : launch_gemm<__half, false, 0, false, false, true>(p, o.x, kp, o.w, kp, dtype, st);
 }
 
 int flab_linear_bwd_partials(int M) { return M <= 0 ? 1 : (M + flab::RUN - 1) / flab::RUN; }
 
 int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *dy, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
-                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *stream) {
+                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *bwd_ws, size_t bwd_ws_bytes, void *stream) {
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M > 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_bwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
   FLAB_REQUIRE(dtype == FLAB_BF16 || dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_bwd: element type %d is not supported", dtype);
-  FLAB_REQUIRE(dy && (!dx || weight) && (!dweight || x) && (act == ACT_NONE || z) && (!dbias || db_partial), FLAB_E_BADARG,
-               "linear_bwd needs dy, weight for dx, x for dweight, z for an activation, db_partial for dbias");
-  FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0, FLAB_E_BADARG, "linear_bwd: ws must be 256-byte aligned");
-  Scratch s = {reinterpret_cast<char *>(ws), ws_bytes};
+  FLAB_REQUIRE(dy && ((!dx && !dweight) || (x && weight)) && (act == ACT_NONE || z) && (!dbias || db_partial), FLAB_E_BADARG,
+               "linear_bwd needs dy, x and weight for dx or dweight, z for an activation, db_partial for dbias");
+  FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0 && reinterpret_cast<uintptr_t>(bwd_ws) % 256 == 0, FLAB_E_BADARG,
+               "linear_bwd: ws and bwd_ws must be 256-byte aligned");
+  Operands o = {x, weight, 0};
+  int rc = dx || dweight ? operands(o, x, weight, M, N, K, ws, ws_bytes, true, st) : FLAB_OK;
+  if (rc) return rc;
   const void *dz = dy;
-  int zp = pitch_of(N), rc;
-  const bool make_dz = (dx || dweight) && (act != ACT_NONE || !as_is(dy, N));
+  const int zp = pitch_of(N), kp = pitch_of(K);
+  const size_t dz_bytes = flab_linear_bwd_workspace(dy, M, N, act);
+  const bool make_dz = (dx || dweight) && dz_bytes;
   if (make_dz || dbias) {
     void *out = nullptr;
     if (make_dz) {
-      const size_t need = copy_bytes(M, N);
-      FLAB_REQUIRE(s.at && s.left >= need, FLAB_E_BADARG, "linear_bwd needs a workspace of flab_linear_workspace() bytes");
-      dz = out = s.at;
-      s.at += need, s.left -= need;
+      FLAB_REQUIRE(bwd_ws && bwd_ws_bytes >= dz_bytes, FLAB_E_BADARG, "linear_bwd needs a workspace of flab_linear_bwd_workspace() bytes");
+      dz = out = bwd_ws;
     }
     rc = dtype == FLAB_BF16 ? launch_act_bwd<bf16>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st)
                             : launch_act_bwd<__half>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st);
@@ -654,19 +674,15 @@ int flab_linear_bwd(const void *x, const void *weight, const void *z, const void
   }
   GemmParams p = {};
   if (dx) {
-    int wp;
-    if ((rc = operand(weight, wp, N, K, s, st))) return rc;
     p.M = M, p.N = K, p.K = N, p.c = dx, p.pairs = four(K, dx);
-    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, true, false>(p, dz, zp, weight, wp, dtype, st)
-                            : launch_gemm<__half, false, 0, false, true, false>(p, dz, zp, weight, wp, dtype, st);
+    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, true, false>(p, dz, zp, o.w, kp, dtype, st)
+                            : launch_gemm<__half, false, 0, false, true, false>(p, dz, zp, o.w, kp, dtype, st);
     if (rc) return rc;
   }
   if (dweight) {
-    int xp;
-    if ((rc = operand(x, xp, M, K, s, st))) return rc;
     p.M = N, p.N = K, p.K = M, p.c = dweight, p.pairs = four(K, dweight);
-    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, true, true, false>(p, dz, zp, x, xp, dtype, st)
-                            : launch_gemm<__half, false, 0, true, true, false>(p, dz, zp, x, xp, dtype, st);
+    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, true, true, false>(p, dz, zp, o.x, kp, dtype, st)
+                            : launch_gemm<__half, false, 0, true, true, false>(p, dz, zp, o.x, kp, dtype, st);
     if (rc) return rc;
   }
   return FLAB_OK;

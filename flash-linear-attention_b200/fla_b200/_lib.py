@@ -11,6 +11,7 @@ from contextlib import nullcontext
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FLA_B200_LIB", os.path.join(_HERE, "libflab200.so"))
@@ -117,13 +118,15 @@ def load() -> ctypes.CDLL:
     lib.flab_rms_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ll, ci, ci, ci, ci, vp]
     sz = ctypes.c_size_t
     lib.flab_linear_workspace.restype = sz
-    lib.flab_linear_workspace.argtypes = [vp, vp, ci, ci, ci, ci]
+    lib.flab_linear_workspace.argtypes = [vp, vp, ci, ci, ci]
+    lib.flab_linear_bwd_workspace.restype = sz
+    lib.flab_linear_bwd_workspace.argtypes = [vp, ci, ci, ci]
     lib.flab_linear_fwd.restype = ci
     lib.flab_linear_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp]
     lib.flab_linear_bwd_partials.restype = ci
     lib.flab_linear_bwd_partials.argtypes = [ci]
     lib.flab_linear_bwd.restype = ci
-    lib.flab_linear_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp]
+    lib.flab_linear_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp, sz, vp]
     lib.flab_linear_e4m3.restype = ci
     lib.flab_linear_e4m3.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp]
     lib.flab_hgrn_workspace.restype = sz
@@ -195,6 +198,12 @@ def call(entry: str, ref: torch.Tensor, **kw):
 def device_of(t: torch.Tensor):
     """Context in which `t`'s device is the current one; nothing to enter where it already is."""
     return nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+
+def once(backward):
+    """A Function's backward body that is not differentiable itself. The marking (which costs 3 us a call) is only needed where a
+    second derivative could be asked for."""
+    return once_differentiable(backward) if torch.is_grad_enabled() else backward
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -7,7 +7,6 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import _DTYPES
@@ -48,6 +47,34 @@ def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=T
     return y, scale, total, rstd
 
 
+def _backward(ctx, dy, dsum=None):
+    total, rstd, w = ctx.saved_tensors
+    rows, n = total.shape
+    dev = total.device
+    need_x, need_w, need_r = ctx.needs_input_grad[:3]
+    dy = torch.zeros(rows, n, dtype=ctx.x_dtype, device=dev) if dy is None else _rows(dy.to(ctx.x_dtype))
+    dsum = None if dsum is None else _rows(dsum.to(total.dtype))
+    wide = need_r and ctx.r_dtype != ctx.x_dtype  # the residual's gradient has a type of its own (the sum's)
+    dx = torch.empty(rows, n, dtype=ctx.x_dtype, device=dev) if need_x or (need_r and not wide) else None
+    dr = torch.empty(rows, n, dtype=total.dtype, device=dev) if wide else None
+    dw = torch.empty_like(w) if w is not None and need_w else None
+    if rows and n:
+        lib = _lib.load()
+        part = None
+        if dw is not None:
+            part = torch.empty(lib.flab_rms_norm_partials(rows, n, _DTYPES[ctx.x_dtype]), n, dtype=torch.float32, device=dev)
+        with _lib.device_of(total):
+            rc = lib.flab_rms_norm_bwd(total.data_ptr(), dy.data_ptr(), _p(dsum), _p(w), rstd.data_ptr(), _p(dx), _p(dr), _p(dw), _p(part),
+                                       rows, n, _DTYPES[ctx.x_dtype], _DTYPES[total.dtype],
+                                       _DTYPES[torch.float32 if w is None else w.dtype], _lib.stream_of(total))
+        _lib.finish("flab_rms_norm_bwd", rc)
+    elif dw is not None:
+        dw.zero_()
+    dx = None if dx is None else _like(dx, ctx.x_shape)
+    dr = _like(dr, ctx.x_shape) if wide else dx
+    return dx if need_x else None, dw, dr if need_r else None, None, None, None
+
+
 class RMSNormFunction(torch.autograd.Function):
     """(y, sum) or y alone; `sum` is x itself, and not among the outputs, where there is neither a residual nor a wider type."""
 
@@ -65,33 +92,8 @@ class RMSNormFunction(torch.autograd.Function):
         return (y, _like(total, x.shape)) if prenorm else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dsum=None):
-        total, rstd, w = ctx.saved_tensors
-        rows, n = total.shape
-        dev = total.device
-        need_x, need_w, need_r = ctx.needs_input_grad[:3]
-        dy = torch.zeros(rows, n, dtype=ctx.x_dtype, device=dev) if dy is None else _rows(dy.to(ctx.x_dtype))
-        dsum = None if dsum is None else _rows(dsum.to(total.dtype))
-        wide = need_r and ctx.r_dtype != ctx.x_dtype  # the residual's gradient has a type of its own (the sum's)
-        dx = torch.empty(rows, n, dtype=ctx.x_dtype, device=dev) if need_x or (need_r and not wide) else None
-        dr = torch.empty(rows, n, dtype=total.dtype, device=dev) if wide else None
-        dw = torch.empty_like(w) if w is not None and need_w else None
-        if rows and n:
-            lib = _lib.load()
-            part = None
-            if dw is not None:
-                part = torch.empty(lib.flab_rms_norm_partials(rows, n, _DTYPES[ctx.x_dtype]), n, dtype=torch.float32, device=dev)
-            with _lib.device_of(total):
-                rc = lib.flab_rms_norm_bwd(total.data_ptr(), dy.data_ptr(), _p(dsum), _p(w), rstd.data_ptr(), _p(dx), _p(dr), _p(dw), _p(part),
-                                           rows, n, _DTYPES[ctx.x_dtype], _DTYPES[total.dtype],
-                                           _DTYPES[torch.float32 if w is None else w.dtype], _lib.stream_of(total))
-            _lib.finish("flab_rms_norm_bwd", rc)
-        elif dw is not None:
-            dw.zero_()
-        dx = None if dx is None else _like(dx, ctx.x_shape)
-        dr = _like(dr, ctx.x_shape) if wide else dx
-        return dx if need_x else None, dw, dr if need_r else None, None, None, None
+        return _lib.once(_backward)(ctx, dy, dsum)
 
 
 def _check(x, weight, residual, residual_in_fp32):

@@ -7,7 +7,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import _DTYPES
@@ -30,26 +29,53 @@ def _like(t: torch.Tensor, shape) -> torch.Tensor:
     return t if t.shape == shape else t.reshape(shape)
 
 
-def _workspace(lib, x2, w, M, N, K, backward):
-    """(scratch, its bytes): none where the operands lie as the kernel reads them."""
-    if not backward and K % 8 == 0 and x2.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0:
-        return None, 0
-    n = lib.flab_linear_workspace(_p(x2), _p(w), M, N, K, backward)
-    return (torch.empty(n, dtype=torch.uint8, device=(w if x2 is None else x2).device) if n else None), n
+def _as_is(t: torch.Tensor, n: int) -> bool:
+    """Whether rows of n elements begin on 16-byte boundaries, as the kernel reads its operands."""
+    return n % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 def _forward(x2, w, b, r2, act, want_z):
+    """(y, z or None, the operands' copies or None)"""
     (M, K), N = x2.shape, w.shape[0]
     y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
     z = torch.empty_like(y) if want_z else None
+    copies = None
     if M:
         lib = _lib.load()
-        ws, n = _workspace(lib, x2, w, M, N, K, 0)
+        n = 0 if _as_is(x2, K) and _as_is(w, K) else lib.flab_linear_workspace(x2.data_ptr(), w.data_ptr(), M, N, K)
+        if n:
+            copies = torch.empty(n, dtype=torch.uint8, device=x2.device)
         with _lib.device_of(x2):
-            rc = lib.flab_linear_fwd(x2.data_ptr(), w.data_ptr(), _p(b), _p(r2), y.data_ptr(), _p(z), M, N, K, act, _DTYPES[x2.dtype], _p(ws), n,
+            rc = lib.flab_linear_fwd(x2.data_ptr(), w.data_ptr(), _p(b), _p(r2), y.data_ptr(), _p(z), M, N, K, act, _DTYPES[x2.dtype], _p(copies), n,
                                      _lib.stream_of(x2))
         _lib.finish("flab_linear_fwd", rc)
-    return y, z
+    return y, z, copies
+
+
+def _backward(ctx, dy):
+    x2, w, z, copies = ctx.saved_tensors
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    M, N, K = ctx.sizes
+    d2, dev = _rows(dy), dy.device
+    dx = torch.empty(M, K, dtype=dy.dtype, device=dev) if need_x else None
+    dw = torch.empty(N, K, dtype=dy.dtype, device=dev) if need_w else None
+    db = torch.empty(N, dtype=dy.dtype, device=dev) if need_b else None
+    if M == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    elif need_x or need_w or need_b:
+        lib = _lib.load()
+        n = lib.flab_linear_bwd_workspace(d2.data_ptr(), M, N, ctx.act) if need_x or need_w else 0
+        dz = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        part = torch.empty(lib.flab_linear_bwd_partials(M), N, dtype=torch.float32, device=dev) if need_b else None
+        # (an operand that was copied, or whose product is not wanted, is not kept: its address only says how the copies lie)
+        x_at, w_at = ctx.places
+        with _lib.device_of(d2):
+            rc = lib.flab_linear_bwd(x_at, w_at, _p(z), d2.data_ptr(), _p(dx), _p(dw), _p(db), _p(part), M, N, K, ctx.act, _DTYPES[dy.dtype],
+                                     _p(copies), 0 if copies is None else copies.numel(), _p(dz), n, _lib.stream_of(d2))
+        _lib.finish("flab_linear_bwd", rc)
+    return (None if dx is None else _like(dx, ctx.x_shape)), dw, db, (dy if need_r else None), None
 
 
 class LinearFunction(torch.autograd.Function):
@@ -58,37 +84,17 @@ class LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         x2, w = _rows(x), weight.contiguous()
         need_x, need_w, need_b, _ = ctx.needs_input_grad[:4]
-        y, z = _forward(x2, w, None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act,
-                        act != 0 and (need_x or need_w or need_b))
-        ctx.save_for_backward(x2 if need_w else None, w if need_x else None, z)
-        ctx.act, ctx.sizes, ctx.x_shape = act, (x2.shape[0], w.shape[0], w.shape[1]), x.shape
+        y, z, copies = _forward(x2, w, None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act,
+                                act != 0 and (need_x or need_w or need_b))
+        K = w.shape[1]
+        ctx.save_for_backward(x2 if need_w and _as_is(x2, K) else None, w if need_x and _as_is(w, K) else None, z, copies if need_x or need_w else None)
+        ctx.places = x2.data_ptr(), w.data_ptr()
+        ctx.act, ctx.sizes, ctx.x_shape = act, (x2.shape[0], w.shape[0], K), x.shape
         return _like(y, x.shape[:-1] + (w.shape[0],))
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x2, w, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        M, N, K = ctx.sizes
-        d2, dev = _rows(dy), dy.device
-        dx = torch.empty(M, K, dtype=dy.dtype, device=dev) if need_x else None
-        dw = torch.empty(N, K, dtype=dy.dtype, device=dev) if need_w else None
-        db = torch.empty(N, dtype=dy.dtype, device=dev) if need_b else None
-        if M == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        elif need_x or need_w or need_b:
-            lib = _lib.load()
-            # dz is a tensor of its own where an activation or dy's rows make one
-            own_dz = (need_x or need_w) and (ctx.act != 0 or N % 8 != 0 or d2.data_ptr() % 16 != 0)
-            ws, n = _workspace(lib, x2, w, M, N, K, 1) if own_dz or K % 8 or x2 is not None and x2.data_ptr() % 16 or w is not None and w.data_ptr() % 16 else (None, 0)
-            part = torch.empty(lib.flab_linear_bwd_partials(M), N, dtype=torch.float32, device=dev) if need_b else None
-            with _lib.device_of(d2):
-                rc = lib.flab_linear_bwd(_p(x2), _p(w), _p(z), d2.data_ptr(), _p(dx), _p(dw), _p(db), _p(part), M, N, K, ctx.act, _DTYPES[dy.dtype],
-                                         _p(ws), n, _lib.stream_of(d2))
-            _lib.finish("flab_linear_bwd", rc)
-        return (None if dx is None else _like(dx, ctx.x_shape)), dw, db, (dy if need_r else None), None
+        return _lib.once(_backward)(ctx, dy)
 
 
 def _check(x, weight, bias, residual, activation, dtype):
@@ -120,7 +126,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LinearFunction.apply(x, weight, bias, residual, act)
-    y, _ = _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False)
+    y, _, _ = _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False)
     return _like(y, x.shape[:-1] + (weight.shape[0],))
 
 

@@ -5,7 +5,6 @@ differentiable in x, g and the initial state, and both take packed sequences. Th
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import _DTYPES
@@ -16,15 +15,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _launch(entry, ref, *args):
-    """One call of the C ABI on the current stream of `ref`'s device, with a workspace from that stream's allocator."""
-    lib = _lib.load()
+def _workspace(lib, ref):
+    """(scratch from the current stream's allocator, its bytes); none for what one tile holds."""
     B, T, D = ref.shape
-    ws_bytes = lib.flab_hgrn_workspace(B, T, D)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ref.device) if ws_bytes else None
-    with _lib.device_of(ref):
-        rc = getattr(lib, entry)(*args, _p(ws), ws_bytes, _lib.stream_of(ref))
-    _lib.finish(entry, rc)
+    n = lib.flab_hgrn_workspace(B, T, D) if T > 64 else 0
+    return (torch.empty(n, dtype=torch.uint8, device=ref.device) if n else None), n
 
 
 def hgrn_fwd(x, g, h0, output_final_state, cu):
@@ -38,8 +33,12 @@ def hgrn_fwd(x, g, h0, output_final_state, cu):
         if ht is not None:
             ht.zero_() if h0 is None else ht.copy_(h0)
         return o, ht
-    _launch("flab_hgrn_fwd", x, x.data_ptr(), g.data_ptr(), _p(h0), o.data_ptr(), _p(ht), _p(cu),
-            int(cu is not None and cu.dtype == torch.int64), B, T, D, N, _DTYPES[x.dtype])
+    lib = _lib.load()
+    ws, n = _workspace(lib, x)
+    with _lib.device_of(x):
+        rc = lib.flab_hgrn_fwd(x.data_ptr(), g.data_ptr(), _p(h0), o.data_ptr(), _p(ht), _p(cu), cu is not None and cu.dtype == torch.int64, B, T, D, N,
+                               _DTYPES[x.dtype], _p(ws), n, _lib.stream_of(x))
+    _lib.finish("flab_hgrn_fwd", rc)
     return o, ht
 
 
@@ -53,9 +52,21 @@ def hgrn_bwd(g, o, h0, do, dht, want_dh0, cu):
         if dh0 is not None:
             dh0.zero_() if dht is None else dh0.copy_(dht)
         return dx, dg, dh0
-    _launch("flab_hgrn_bwd", g, g.data_ptr(), o.data_ptr(), _p(h0), do.data_ptr(), _p(dht), dx.data_ptr(), dg.data_ptr(), _p(dh0), _p(cu),
-            int(cu is not None and cu.dtype == torch.int64), B, T, D, N, _DTYPES[g.dtype])
+    lib = _lib.load()
+    ws, n = _workspace(lib, g)
+    with _lib.device_of(g):
+        rc = lib.flab_hgrn_bwd(g.data_ptr(), o.data_ptr(), _p(h0), do.data_ptr(), _p(dht), dx.data_ptr(), dg.data_ptr(), _p(dh0), _p(cu),
+                               cu is not None and cu.dtype == torch.int64, B, T, D, N, _DTYPES[g.dtype], _p(ws), n, _lib.stream_of(g))
+    _lib.finish("flab_hgrn_bwd", rc)
     return dx, dg, dh0
+
+
+def _backward(ctx, do, dht):
+    g, o, h0, cu = ctx.saved_tensors
+    do = torch.zeros_like(g) if do is None else do.to(g.dtype).contiguous()
+    dht = None if dht is None else dht.float().contiguous()
+    dx, dg, dh0 = hgrn_bwd(g, o, h0, do, dht, ctx.needs_input_grad[2], cu)
+    return dx, dg, None if dh0 is None else dh0.to(ctx.h0_dtype), None, None
 
 
 class HGRNFunction(torch.autograd.Function):
@@ -71,13 +82,8 @@ class HGRNFunction(torch.autograd.Function):
         return o, ht
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do, dht):
-        g, o, h0, cu = ctx.saved_tensors
-        do = torch.zeros_like(g) if do is None else do.to(g.dtype).contiguous()
-        dht = None if dht is None else dht.float().contiguous()
-        dx, dg, dh0 = hgrn_bwd(g, o, h0, do, dht, ctx.needs_input_grad[2], cu)
-        return dx, dg, None if dh0 is None else dh0.to(ctx.h0_dtype), None, None
+        return _lib.once(_backward)(ctx, do, dht)
 
 
 def _hgrn(x, g, initial_state, output_final_state, offsets):
@@ -96,16 +102,17 @@ def _hgrn(x, g, initial_state, output_final_state, offsets):
             raise ValueError(f"`offsets` must be a one-dimensional int32 or int64 tensor, got {offsets.dtype} {tuple(offsets.shape)}")
         offsets = offsets.to(x.device).contiguous()
         N = offsets.numel() - 1
-    for name, t in (("g", g), ("initial_state", initial_state)):
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{name} is on {t.device}, expected {x.device}")
+    if g.device != x.device:
+        raise RuntimeError(f"g is on {g.device}, expected {x.device}")
+    if initial_state is not None and initial_state.device != x.device:
+        raise RuntimeError(f"initial_state is on {initial_state.device}, expected {x.device}")
     if initial_state is not None and tuple(initial_state.shape) != (N, x.shape[2]):
         raise ValueError(f"The number of initial states is expected to be equal to the number of input sequences, "
                          f"i.e., a shape of {(N, x.shape[2])} rather than {tuple(initial_state.shape)}.")
     if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or (initial_state is not None and initial_state.requires_grad)):
         return HGRNFunction.apply(x, g, initial_state, bool(output_final_state), offsets)
-    h0 = None if initial_state is None else initial_state.detach().float().contiguous()
-    return hgrn_fwd(x.detach().contiguous(), g.detach().contiguous(), h0, bool(output_final_state), offsets)
+    h0 = None if initial_state is None else initial_state.float().contiguous()
+    return hgrn_fwd(x.contiguous(), g.contiguous(), h0, bool(output_final_state), offsets)
 
 
 def chunk_hgrn(

@@ -312,12 +312,17 @@ def test_abi_refusals():
     assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 5, 0, None, 0, None) == -1
     assert b"activation" in lib.flab_last_error()
     assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 0, 2, None, 0, None) == -2
-    assert lib.flab_linear_workspace(16, 16, 8, 8, 8, 0) == 0
-    assert lib.flab_linear_workspace(16, 18, 8, 8, 8, 0) == 256 and lib.flab_linear_workspace(16, 16, 8, 8, 7, 0) == 512
+    assert lib.flab_linear_workspace(16, 16, 8, 8, 8) == 0
+    assert lib.flab_linear_workspace(16, 18, 8, 8, 8) == 256 and lib.flab_linear_workspace(16, 16, 8, 8, 7) == 512
+    assert lib.flab_linear_bwd_workspace(16, 8, 8, 0) == 0 and lib.flab_linear_bwd_workspace(16, 8, 8, 1) == 256
+    assert lib.flab_linear_bwd_workspace(18, 8, 8, 0) == 256
     assert lib.flab_linear_fwd(16, 18, None, None, 16, None, 8, 8, 8, 0, 0, None, 0, None) == -1
     assert b"workspace" in lib.flab_last_error()
-    assert lib.flab_linear_bwd(16, 16, None, 16, 16, None, None, None, 8, 8, 8, 1, 0, None, 0, None) == -1
-    assert lib.flab_linear_bwd(16, 16, 16, 16, 16, None, None, None, 8, 8, 8, 1, 0, None, 0, None) == -1
+    assert lib.flab_linear_bwd(16, 16, None, 16, 16, None, None, None, 8, 8, 8, 1, 0, None, 0, None, 0, None) == -1
+    assert lib.flab_linear_bwd(None, 16, None, 16, 16, None, None, None, 8, 8, 8, 0, 0, None, 0, None, 0, None) == -1
+    assert lib.flab_linear_bwd(16, 18, None, 16, 16, None, None, None, 8, 8, 8, 0, 0, None, 0, None, 0, None) == -1
+    assert b"flab_linear_workspace" in lib.flab_last_error()
+    assert lib.flab_linear_bwd(16, 16, 16, 16, 16, None, None, None, 8, 8, 8, 1, 0, None, 0, None, 0, None) == -1
     assert b"workspace" in lib.flab_last_error()
     assert lib.flab_linear_e4m3(16, 16, 16, 16, None, None, 16, 8, 8, 24, 0, 0, None) == -2
     assert b"multiple of 16" in lib.flab_last_error()
