@@ -63,7 +63,7 @@ template <int BN> struct GemmShape {
   static constexpr int S = BN == 256 ? 5 : 6;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
-  static constexpr int TURN = 2 * 4096;  // a warp's two blocks of 32 rows of 128 bytes; 16-byte piece c of row r lies at c ^ (r & 7)
+  static constexpr int TURN = 8192;  // a warp's staging: four blocks of 32 rows of 64 bytes, or one of 32 x 32 floats to turn
   static constexpr int BYTES = S * STAGE + EPI_WARPS * TURN + 1024;
 };
 
@@ -168,30 +168,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       }
     }
     __syncwarp();
-  } else if (TS && warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 64 columns in turn
+  } else if (TS && warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 32 columns in turn
     const int w = warp - 4, quarter = w & 3, side = w >> 2;
-    uint8_t *const stage = buf + S * Z::STAGE + w * Z::TURN;
-    constexpr int BLOCKS = BN / 128;  // of this warp (with 64 columns, only side 0 has one)
-    const bool mine = BN > 64 || side == 0, two = !EPI || !p.z;  // two buffers in turn; with z the second one is z's
+    uint8_t *const stage = buf + S * Z::STAGE + w * Z::TURN;  // y, y, z, z
+    constexpr int BLOCKS = BN / 64;  // of this warp
     uint32_t seen = 0;  // parity of the residual blocks taken, a bit a buffer
     int n = 0;
     for (int tile = cluster; tile < p.tiles; tile += clusters, ++n) {
       const int half = n & 1;
       int tm, tn;
       place(tile, tm, tn);
-      const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN;
-      auto column = [&](int b) { return n0 + (2 * b + side) * 64; };
-      auto ask = [&](int b) {  // lane 0
-        const int q = two ? b & 1 : 0;
-        tc::mbar_expect_tx(&res_full[w][q], 4096);
-        tc::tma_load_2d(stage + q * 4096, &mr, &res_full[w][q], column(b), m0);
+      const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN + side * 32;
+      auto ask = [&](int b) {  // lane 0: the residual of block b, into the buffer that its result will leave from
+        tc::mbar_expect_tx(&res_full[w][b & 1], 2048);
+        tc::tma_load_2d(stage + (b & 1) * 2048, &mr, &res_full[w][b & 1], n0 + b * 64, m0);
       };
-      if (mine && lane == 0) {
+      if (lane == 0) {
         tc::tma_store_wait_read();
-        if (EPI && p.res) {
-          ask(0);
-          if (two && BLOCKS > 1) ask(1);
-        }
+        if (EPI && p.res) ask(0);
       }
       __syncwarp();
       float row_scale = 1.f;
@@ -201,114 +195,112 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         break;
       }
       tc::fence_after_sync();
-      const uint32_t from = tmem + half * BN + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t from = tmem + half * BN + side * 32 + ((uint32_t)(quarter * 32) << 16);
       bool ok = true;
-      if (mine) {
 #pragma unroll 1
-        for (int b = 0; b < (BLOCKS ? BLOCKS : 1); ++b) {
-          const int q = two ? b & 1 : 0, c0 = column(b);
-          uint8_t *const ybuf = stage + q * 4096 + lane * 128, *const zbuf = stage + 4096 + lane * 128;
-          if (b > 0 && !two) {
-            if (lane == 0) {
-              tc::tma_store_wait_read();
-              if (EPI && p.res) ask(b);
-            }
-            __syncwarp();
+      for (int b = 0; b < BLOCKS; ++b) {
+        const int q = b & 1, c = n0 + b * 64;
+        float v[32];
+        tc::tmem_ld_32x32b_x32(from + b * 64, v);
+        if (EPI && p.res) {
+          if (b + 1 < BLOCKS && lane == 0) {
+            tc::tma_store_wait_read();  // of block b - 1, a block's work ago
+            ask(b + 1);
           }
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            float v[32];
-            tc::tmem_ld_32x32b_x32(from + (2 * b + side) * 64 + h * 32, v);
-            const int c = c0 + h * 32;
-            float cs[F8 ? 32 : 1];
-            if (F8) {
+        } else {
+          if (lane == 0) tc::tma_store_wait_read_but_one();  // of block b - 2
+        }
+        float cs[F8 ? 32 : 1];
+        if (F8) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 s = c + 4 * j < p.N ? *reinterpret_cast<const float4 *>(p.col_scale + c + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                cs[4 * j] = s.x, cs[4 * j + 1] = s.y, cs[4 * j + 2] = s.z, cs[4 * j + 3] = s.w;
-              }
-            }
-            struct alignas(16) Eight {
-              TO v[8];
-            };
-            Eight bias[4];
-            if (EPI && p.bias) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c + 8 * j < p.N) bias[j] = *reinterpret_cast<const Eight *>(reinterpret_cast<const TO *>(p.bias) + c + 8 * j);
-            }
-            tc::tmem_ld_wait();
-            if (F8) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = v[j] * row_scale * cs[j];
-            }
-            if (EPI && p.bias) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] += Num<TO>::f(bias[j >> 3].v[j & 7]);
-            }
-            auto piece = [&](uint8_t *row, int j) { return reinterpret_cast<Eight *>(row + (((h * 4 + j) ^ (lane & 7)) << 4)); };
-            if (EPI && p.z) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                Eight o;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
-                *piece(zbuf, j) = o;
-              }
-            }
-            if (EPI && p.act) {
-              switch (p.act) {  // one loop an activation, unrolled whole: a loop over v would put it in local memory
-                case ACT_SILU:
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SILU);
-                  break;
-                case ACT_SIGMOID:
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SIGMOID);
-                  break;
-                case ACT_LOGSIGMOID:
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_LOGSIGMOID);
-                  break;
-                default:
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_GELU);
-                  break;
-              }
-            }
-            if (EPI && p.res) {
-              if (h == 0 && ok) {
-                ok = tc::mbar_wait(&res_full[w][q], (seen >> q) & 1);
-                if (!ok) tu_tc_error = 734;
-                seen ^= 1u << q;
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const Eight r = *piece(ybuf, j);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[8 * j + i] += Num<TO>::f(r.v[i]);
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              Eight o;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
-              *piece(ybuf, j) = o;
-            }
-          }
-          tc::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            tc::tma_store_2d(&mc, stage + q * 4096, c0, m0);
-            if (EPI && p.z) tc::tma_store_2d(&mz, stage + 4096, c0, m0);
-            tc::tma_store_commit();
+          for (int j = 0; j < 8; ++j) {
+            const float4 s = c + 4 * j < p.N ? *reinterpret_cast<const float4 *>(p.col_scale + c + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+            cs[4 * j] = s.x, cs[4 * j + 1] = s.y, cs[4 * j + 2] = s.z, cs[4 * j + 3] = s.w;
           }
         }
+        struct alignas(16) Eight {
+          TO v[8];
+        };
+        Eight bias[4];
+        if (EPI && p.bias) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + 8 * j < p.N) bias[j] = *reinterpret_cast<const Eight *>(reinterpret_cast<const TO *>(p.bias) + c + 8 * j);
+        }
+        tc::tmem_ld_wait();
+        __syncwarp();
+        if (b + 1 == BLOCKS) {  // the warp has taken its last block: the products may use this half again
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
+        }
+        if (F8) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = v[j] * row_scale * cs[j];
+        }
+        if (EPI && p.bias) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += Num<TO>::f(bias[j >> 3].v[j & 7]);
+        }
+        // rows of 64 bytes, 64-byte swizzle: 16-byte piece j of row r lies at j ^ (r / 2 % 4)
+        auto piece = [&](int buffer, int j) { return reinterpret_cast<Eight *>(stage + buffer * 2048 + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)); };
+        if (EPI && p.z) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            Eight o;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
+            *piece(2 + q, j) = o;
+          }
+        }
+        if (EPI && p.act) {
+          switch (p.act) {  // one loop an activation, unrolled whole: a loop over v would put it in local memory
+            case ACT_SILU:
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SILU);
+              break;
+            case ACT_SIGMOID:
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_SIGMOID);
+              break;
+            case ACT_LOGSIGMOID:
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_LOGSIGMOID);
+              break;
+            default:
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = act_fwd(v[j], ACT_GELU);
+              break;
+          }
+        }
+        if (EPI && p.res) {
+          if (ok) {
+            ok = tc::mbar_wait(&res_full[w][q], (seen >> q) & 1);
+            if (!ok) tu_tc_error = 734;
+            seen ^= 1u << q;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Eight r = *piece(q, j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[8 * j + i] += Num<TO>::f(r.v[i]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Eight o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
+          *piece(q, j) = o;
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          tc::tma_store_2d(&mc, stage + q * 2048, c, m0);
+          if (EPI && p.z) tc::tma_store_2d(&mz, stage + (2 + q) * 2048, c, m0);
+          tc::tma_store_commit();
+        }
       }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
       if (!__all_sync(0xffffffffu, ok)) break;
     }
     if (lane == 0) tc::tma_store_wait_all();
@@ -518,7 +510,8 @@ int operand_map(CUtensorMap *map, const void *base, int dtype, long long rows, i
                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)pitch * (dtype == FLAB_E4M3 ? 1 : 2)};
   const uint32_t box[2] = {(uint32_t)box_cols, (uint32_t)box_rows};
-  return make_tensor_map(map, base, type, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const int row = box_cols * (dtype == FLAB_E4M3 ? 1 : 2);  // bytes of a box row: the swizzle's span
+  return make_tensor_map(map, base, type, 2, dims, strides, box, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI, bool TS>
@@ -538,9 +531,9 @@ int launch_gemm_ts(GemmParams p, const void *a, int a_pitch, const void *b, int 
   CUtensorMap mc = ma, mz = ma, mr = ma;  // (a map that is not used may be any)
   if (TS) {
     const int out = Num<TO>::id;
-    if ((rc = operand_map(&mc, p.c, out, p.M, p.N, p.N, 64, 32))) return rc;
-    if (p.z && (rc = operand_map(&mz, p.z, out, p.M, p.N, p.N, 64, 32))) return rc;
-    if (p.res && (rc = operand_map(&mr, p.res, out, p.M, p.N, p.N, 64, 32))) return rc;
+    if ((rc = operand_map(&mc, p.c, out, p.M, p.N, p.N, 32, 32))) return rc;
+    if (p.z && (rc = operand_map(&mz, p.z, out, p.M, p.N, p.N, 32, 32))) return rc;
+    if (p.res && (rc = operand_map(&mr, p.res, out, p.M, p.N, p.N, 32, 32))) return rc;
   }
   auto kernel = gemm_kernel<TO, F8, T16, AMN, BMN, BN, EPI, TS>;
   if ((rc = set_smem(kernel, Z::BYTES))) return rc;
