@@ -490,7 +490,7 @@ template <typename KernelT> inline int set_smem(KernelT kernel, size_t bytes) {
     set_error("kernel needs %zu bytes of shared memory (limit 232448)", bytes);
     return FLAB_E_UNSUPPORTED;
   }
-  if (bytes > 48 * 1024) {
+  if (bytes > 32 * 1024) {  // (the 48 KB that need no asking include the kernel's static shared memory)
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) {
       set_error("cudaFuncSetAttribute(%zu): %s", bytes, cudaGetErrorString(e));
