@@ -699,8 +699,8 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
   __syncthreads();
 }
 
-// ---- a few tokens a sequence (decode) ---------------------------------------------------------------------------------
-// A thread walks the tokens of 16 bytes of channels; nothing is shared.
+// ---- a few tokens a sequence (decode, short windows) --------------------------------------------------------------------
+// A thread walks the tokens of its channels; nothing is shared.
 template <typename T, int V, bool BWD> __global__ void __launch_bounds__(256) hgrn_step_kernel(const HgrnParams p) {
   const int per = p.D / V;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -715,28 +715,41 @@ template <typename T, int V, bool BWD> __global__ void __launch_bounds__(256) hg
   const size_t state = (size_t)b * p.D + ch;
   if (edge) c = *reinterpret_cast<const PF *>(edge + state);
   if (BWD && p.h0) h = *reinterpret_cast<const PF *>(p.h0 + state);
-  for (int k = 0; k < (int)p.T; ++k) {
-    const int t = BWD ? (int)p.T - 1 - k : k;
-    const size_t at = ((size_t)b * p.T + t) * p.D + ch;
-    const PV g = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.g) + at);
-    const PV x = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.x) + at);
-    PV y, z, o;
-    if (BWD && t > 0) o = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.o_in) + at - p.D);
+  constexpr int U = BWD ? 4 : 8;  // tokens whose loads are in flight together
+  const int last = (int)p.T - 1;
+  for (int k0 = 0; k0 <= last; k0 += U) {
+    PV g[U], x[U], o[BWD ? U : 1];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float a = gate(Num<T>::f(g.v[j]));
-      if (!BWD) {
-        c.v[j] = fmaf(a, c.v[j], Num<T>::f(x.v[j]));
-        y.v[j] = Num<T>::t(c.v[j]);
-      } else {
-        const float d = Num<T>::f(x.v[j]) + c.v[j];
-        c.v[j] = a * d;
-        y.v[j] = Num<T>::t(d);
-        z.v[j] = Num<T>::t(c.v[j] * (t > 0 ? Num<T>::f(o.v[j]) : h.v[j]));
+    for (int u = 0; u < U; ++u)
+      if (k0 + u <= last) {
+        const int t = BWD ? last - (k0 + u) : k0 + u;
+        const size_t at = ((size_t)b * p.T + t) * p.D + ch;
+        g[u] = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.g) + at);
+        x[u] = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.x) + at);
+        if (BWD && t > 0) o[u] = *reinterpret_cast<const PV *>(reinterpret_cast<const T *>(p.o_in) + at - p.D);
       }
-    }
-    *reinterpret_cast<PV *>(reinterpret_cast<T *>(p.o) + at) = y;
-    if (BWD) *reinterpret_cast<PV *>(reinterpret_cast<T *>(p.dg) + at) = z;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u <= last) {
+        const int t = BWD ? last - (k0 + u) : k0 + u;
+        const size_t at = ((size_t)b * p.T + t) * p.D + ch;
+        PV y, z;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float a = gate(Num<T>::f(g[u].v[j]));
+          if (!BWD) {
+            c.v[j] = fmaf(a, c.v[j], Num<T>::f(x[u].v[j]));
+            y.v[j] = Num<T>::t(c.v[j]);
+          } else {
+            const float d = Num<T>::f(x[u].v[j]) + c.v[j];
+            c.v[j] = a * d;
+            y.v[j] = Num<T>::t(d);
+            z.v[j] = Num<T>::t(c.v[j] * (t > 0 ? Num<T>::f(o[BWD ? u : 0].v[j]) : h.v[j]));
+          }
+        }
+        *reinterpret_cast<PV *>(reinterpret_cast<T *>(p.o) + at) = y;
+        if (BWD) *reinterpret_cast<PV *>(reinterpret_cast<T *>(p.dg) + at) = z;
+      }
   }
   if (p.ht) *reinterpret_cast<PF *>(p.ht + state) = c;
 }
@@ -817,8 +830,12 @@ template <typename T, bool BWD, bool VAR> int launch_stream(HgrnParams p, void *
   return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
 }
 
-// Sequences of up to this many tokens are walked by one thread a channel group: shorter than that, a tile is mostly empty rows.
-constexpr int STEPS = 8;
+// Fixed-length sequences that are walked by one thread a channel group instead of being put into tiles: up to 32 tokens, of which a
+// tile would be mostly empty rows (62 x 15 x 1821 fp32: tiles 33 us forward, the walk 9), and up to a tile's 128 where the
+// channels alone fill the card (128 x 44 x 1284 bf16: 32 and 12 us).
+bool walks(const HgrnParams &p, int V) {
+  return !p.cu && (p.T <= 32 || (p.T <= 128 && (long long)p.B * p.D / V >= 512ll * sm_count()));
+}
 
 template <typename T, bool BWD, int V> int launch_step(const HgrnParams &p, cudaStream_t st) {
   const long long n = (long long)p.B * (p.D / V);
@@ -835,11 +852,14 @@ template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws,
     tma = tma && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   }
   for (const float *q : {p.h0, p.dht, (const float *)p.ht}) tma = tma && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  if (!p.cu && p.T <= STEPS) {
-    bool wide = tma && p.D % (16 / sizeof(T)) == 0;
-    for (const float *q : {p.h0, p.dht, (const float *)p.ht}) wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
-    return wide ? launch_step<T, BWD, 16 / sizeof(T)>(p, st) : launch_step<T, BWD, 1>(p, st);
+  constexpr int WIDE = 16 / sizeof(T);
+  bool wide = tma && p.D % WIDE == 0;
+  for (const float *q : {p.h0, p.dht, (const float *)p.ht}) {
+    wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    pair = pair && reinterpret_cast<uintptr_t>(q) % 8 == 0;
   }
+  if (walks(p, wide ? WIDE : pair ? 2 : 1))
+    return wide ? launch_step<T, BWD, WIDE>(p, st) : pair ? launch_step<T, BWD, 2>(p, st) : launch_step<T, BWD, 1>(p, st);
   if (tma && p.T > HgrnTile<T>::L)
     return p.cu ? launch_stream<T, BWD, true>(p, ws, ws_bytes, st) : launch_stream<T, BWD, false>(p, ws, ws_bytes, st);
   if (p.cu) return pair ? launch_hgrn<T, BWD, true, 2>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, true, 1>(p, ws, ws_bytes, st);

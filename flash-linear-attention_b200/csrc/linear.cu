@@ -13,6 +13,8 @@
 // residual comes in the same way, a block ahead.  Outputs whose rows do not begin on 16-byte boundaries go through a transposition in
 // shared memory instead, so that a warp reads and writes runs of 64 bytes.  Tiles go in groups of 8 rows of tiles, so that what the
 // pairs work on at one time shares operands in L2.
+#include <type_traits>
+
 #include "tc.cuh"
 
 FLAB_TC_DEFINE_ERROR_WORD(linear_error)
@@ -50,13 +52,14 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 struct GemmParams {
   int M, N, K;          // C [M, N]; K: the summed extent
   int tiles_m, tiles_n, tiles;
+  int splits, kper;     // the sum in `splits` runs of kper blocks of 128 bytes; each writes a matrix of its own behind the last one's
   void *c;              // [M, N]
   void *z;              // z before the activation, same type, or null
   const void *bias;     // [N] or null
   const void *res;      // [M, N] or null
   const float *row_scale, *col_scale;  // e4m3 operands
   int act;
-  int pairs;            // rows of c, z, res and bias begin on 4-byte boundaries
+  int pairs;            // rows of c, z and res begin on boundaries of two elements
 };
 
 template <int BN> struct GemmShape {
@@ -95,8 +98,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
   tc::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
-  const int kblocks = (p.K + BK - 1) / BK;
-  auto place = [&](int tile, int &tm, int &tn) {  // groups of 8 rows of tiles, down the group's columns
+  const int kblocks = (p.K + BK - 1) / BK, units = p.tiles * p.splits;
+  auto run = [&](int unit, int &from, int &to) {  // a unit's blocks of the sum
+    from = unit / p.tiles * p.kper;
+    to = min(kblocks, from + p.kper);
+  };
+  auto place = [&](int unit, int &tm, int &tn) {  // groups of 8 rows of tiles, down the group's columns
+    const int tile = unit % p.tiles;
     const int group = tile / (8 * p.tiles_n), in = tile - group * 8 * p.tiles_n, high = min(8, p.tiles_m - group * 8);
     tn = in / high;
     tm = group * 8 + in - tn * high;
@@ -108,11 +116,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       tc::tma_prefetch_desc(&mb);
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = cluster; tile < p.tiles && ok; tile += clusters) {
+      for (int unit = cluster; unit < units && ok; unit += clusters) {
         int tm, tn;
-        place(tile, tm, tn);
+        place(unit, tm, tn);
         const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        int k0, k1;
+        run(unit, k0, k1);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
           const int s = it % S;
           if (it >= S && !tc::mbar_wait(&empty[s], (it / S - 1) & 1)) {
             tu_tc_error = 730;
@@ -142,14 +152,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       uint32_t it = 0;
       int n = 0;
       bool ok = true;
-      for (int tile = cluster; tile < p.tiles && ok; tile += clusters, ++n) {
+      for (int unit = cluster; unit < units && ok; unit += clusters, ++n) {
         const int half = n & 1;
         if (n >= 2 && !tc::mbar_wait(&acc_empty[half], (n / 2 - 1) & 1)) {
           tu_tc_error = 731;
           break;
         }
         tc::fence_after_sync();
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        int k0, k1;
+        run(unit, k0, k1);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
           const int s = it % S;
           if (!tc::mbar_wait(&full[s], (it / S) & 1)) {
             tu_tc_error = 732;
@@ -161,7 +173,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             tc::umma_pair<F8>(tmem + half * BN, AMN ? tc::desc_mnmajor(a, k, 8192) : tc::desc_kmajor(a, k, 0),
-                              BMN ? tc::desc_mnmajor(b, k, 8192) : tc::desc_kmajor(b, k, 0), idesc, kb > 0 || k > 0);
+                              BMN ? tc::desc_mnmajor(b, k, 8192) : tc::desc_kmajor(b, k, 0), idesc, kb > k0 || k > 0);
           tc::umma_commit_pair(&empty[s]);
         }
         if (ok) tc::umma_commit_pair(&acc_full[half]);
@@ -174,10 +186,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
     constexpr int BLOCKS = BN / 64;  // of this warp
     uint32_t seen = 0;  // parity of the residual blocks taken, a bit a buffer
     int n = 0;
-    for (int tile = cluster; tile < p.tiles; tile += clusters, ++n) {
+    for (int unit = cluster; unit < units; unit += clusters, ++n) {
       const int half = n & 1;
       int tm, tn;
-      place(tile, tm, tn);
+      place(unit, tm, tn);
       const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN + side * 32;
       auto ask = [&](int b) {  // lane 0: the residual of block b, into the buffer that its result will leave from
         tc::mbar_expect_tx(&res_full[w][b & 1], 2048);
@@ -317,10 +329,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       float2 bias, scale;
     };
     int n = 0;
-    for (int tile = cluster; tile < p.tiles; tile += clusters, ++n) {
+    for (int unit = cluster; unit < units; unit += clusters, ++n) {
       const int half = n & 1;
       int tm, tn;
-      place(tile, tm, tn);
+      place(unit, tm, tn);
       const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN;
       const int rows = min(32, p.M - m0);
       auto ask = [&](int cb, Ahead &a) {
@@ -381,38 +393,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         __syncwarp();
         const int c0 = n0 + cb * 32 + pair * 2;
         const bool on0 = c0 < p.N, on1 = c0 + 1 < p.N;
-        size_t at = (size_t)(m0 + odd) * p.N + c0;
-        auto set = [&](void *q, float2 f) {
-          TO *const e = reinterpret_cast<TO *>(q) + at;
-          Two t;
-          t.v[0] = Num<TO>::t(f.x), t.v[1] = Num<TO>::t(f.y);
-          if (p.pairs && on1) {
-            *reinterpret_cast<Two *>(e) = t;
-          } else {
-            if (on0) e[0] = t.v[0];
-            if (on1) e[1] = t.v[1];
-          }
-        };
+        float2 f[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i, at += 2 * (size_t)p.N) {
+        for (int i = 0; i < 16; ++i) {
           const int r = 2 * i + odd;
-          float2 f = *reinterpret_cast<const float2 *>(turn + r * 32 + (((pair >> 1) ^ (r & 7)) << 2) + (pair & 1) * 2);
+          f[i] = *reinterpret_cast<const float2 *>(turn + r * 32 + (((pair >> 1) ^ (r & 7)) << 2) + (pair & 1) * 2);
           if (F8) {
             const float rs = __shfl_sync(0xffffffffu, row_scale, r);
-            f.x = f.x * rs * now.scale.x, f.y = f.y * rs * now.scale.y;
+            f[i].x = f[i].x * rs * now.scale.x, f[i].y = f[i].y * rs * now.scale.y;
           }
-          if (r >= rows) continue;
-          if (EPI) {
-            f.x += now.bias.x, f.y += now.bias.y;
-            if (p.z) set(p.z, f);
-            if (p.act) f.x = act_fwd(f.x, p.act), f.y = act_fwd(f.y, p.act);
-            if (p.res) {
-              const Two r2 = *reinterpret_cast<const Two *>(&now.res[i]);
-              f.x += Num<TO>::f(r2.v[0]), f.y += Num<TO>::f(r2.v[1]);
+          if (EPI) f[i].x += now.bias.x, f[i].y += now.bias.y;
+        }
+        auto store = [&](void *q) {
+          TO *e = reinterpret_cast<TO *>(q) + (size_t)(unit / p.tiles) * p.M * p.N + (size_t)(m0 + odd) * p.N + c0;
+          if (p.pairs) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i, e += 2 * (size_t)p.N)
+              if (2 * i + odd < rows && on0) {
+                Two t;
+                t.v[0] = Num<TO>::t(f[i].x), t.v[1] = Num<TO>::t(f[i].y);
+                *reinterpret_cast<Two *>(e) = t;
+              }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i, e += 2 * (size_t)p.N) {
+              if (2 * i + odd < rows && on0) e[0] = Num<TO>::t(f[i].x);
+              if (2 * i + odd < rows && on1) e[1] = Num<TO>::t(f[i].y);
             }
           }
-          set(p.c, f);
+        };
+        if (EPI && p.z) store(p.z);
+        if (EPI && p.act) {
+          switch (p.act) {  // the choice is made once a block
+            case ACT_SILU:
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i].x = act_fwd(f[i].x, ACT_SILU), f[i].y = act_fwd(f[i].y, ACT_SILU);
+              break;
+            case ACT_SIGMOID:
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i].x = act_fwd(f[i].x, ACT_SIGMOID), f[i].y = act_fwd(f[i].y, ACT_SIGMOID);
+              break;
+            case ACT_LOGSIGMOID:
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i].x = act_fwd(f[i].x, ACT_LOGSIGMOID), f[i].y = act_fwd(f[i].y, ACT_LOGSIGMOID);
+              break;
+            default:
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i].x = act_fwd(f[i].x, ACT_GELU), f[i].y = act_fwd(f[i].y, ACT_GELU);
+              break;
+          }
         }
+        if constexpr (EPI) {
+          if (p.res) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const Two r2 = *reinterpret_cast<const Two *>(&now.res[i]);
+              f[i].x += Num<TO>::f(r2.v[0]), f[i].y += Num<TO>::f(r2.v[1]);
+            }
+          }
+        }
+        store(p.c);
         __syncwarp();
         now = next;
       }
@@ -486,22 +526,72 @@ int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, 
   return check_launch("linear_bwd");
 }
 
-// Rows of n elements to rows of `pitch`, for one or two matrices in a launch.
+// Rows of n elements to rows of `pitch`, V elements at a time, for one or two matrices in a launch.
 struct Repitch {
   const unsigned short *from;
   unsigned short *to;
   int rows, n, pitch;
 };
-__global__ void __launch_bounds__(256) repitch_kernel(const Repitch a, const Repitch b) {
+template <int V> __global__ void __launch_bounds__(256) repitch_kernel(const Repitch a, const Repitch b) {
+  struct alignas(2 * V) Pack {
+    unsigned short v[V];
+  };
   const int lane = threadIdx.x & 31;
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows + b.rows; r += gridDim.x * 8) {
     const bool second = r >= a.rows;
     const int row = second ? r - a.rows : r, n = second ? b.n : a.n;
     const unsigned short *from = (second ? b.from : a.from) + (size_t)row * n;
     unsigned short *to = (second ? b.to : a.to) + (size_t)row * (second ? b.pitch : a.pitch);
-#pragma unroll 4
-    for (int c = lane; c < n; c += 32) to[c] = from[c];
+#pragma unroll 8
+    for (int c = lane * V; c < n; c += 32 * V) *reinterpret_cast<Pack *>(to + c) = *reinterpret_cast<const Pack *>(from + c);
   }
+}
+
+// The joined partial sums of a product in runs, with the epilogue: V elements a thread, the runs in order.
+template <typename TO, int V>
+__global__ void __launch_bounds__(256) join_kernel(const float *__restrict__ part, int splits, const GemmParams p) {
+  struct alignas(sizeof(TO) * V) Out {
+    TO v[V];
+  };
+  struct alignas(V == 1 ? 4 : 8) In {
+    float v[V < 2 ? 1 : 2];
+  };
+  const long long total = (long long)p.M * p.N, at = ((long long)blockIdx.x * 256 + threadIdx.x) * V;
+  if (at >= total) return;
+  float f[V] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float *const q = part + s * total + at;
+#pragma unroll
+    for (int j = 0; j < V; j += sizeof(In) / 4) {
+      const In in = *reinterpret_cast<const In *>(q + j);
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(In) / 4); ++i) f[j + i] += in.v[i];
+    }
+  }
+  if (p.bias) {
+    const int c = (int)(at % p.N);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] += Num<TO>::f(reinterpret_cast<const TO *>(p.bias)[c + j]);
+  }
+  Out o;
+  if (p.z) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = Num<TO>::t(f[j]);
+    *reinterpret_cast<Out *>(reinterpret_cast<TO *>(p.z) + at) = o;
+  }
+  if (p.act) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = act_fwd(f[j], p.act);
+  }
+  if (p.res) {
+    const Out r = *reinterpret_cast<const Out *>(reinterpret_cast<const TO *>(p.res) + at);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] += Num<TO>::f(r.v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) o.v[j] = Num<TO>::t(f[j]);
+  *reinterpret_cast<Out *>(reinterpret_cast<TO *>(p.c) + at) = o;
 }
 
 int operand_map(CUtensorMap *map, const void *base, int dtype, long long rows, int cols, int pitch, int box_cols, int box_rows) {
@@ -537,30 +627,75 @@ int launch_gemm_ts(GemmParams p, const void *a, int a_pitch, const void *b, int 
   }
   auto kernel = gemm_kernel<TO, F8, T16, AMN, BMN, BN, EPI, TS>;
   if ((rc = set_smem(kernel, Z::BYTES))) return rc;
-  const int clusters = sm_count() / 2;
-  kernel<<<2 * (p.tiles < clusters ? p.tiles : clusters), Z::THREADS, Z::BYTES, st>>>(p, ma, mb, mc, mz, mr);
+  const int clusters = sm_count() / 2, units = p.tiles * p.splits;
+  kernel<<<2 * (units < clusters ? units : clusters), Z::THREADS, Z::BYTES, st>>>(p, ma, mb, mc, mz, mr);
   return check_launch("linear");
 }
 
 template <typename TO, bool F8, int T16, bool AMN, bool BMN, int BN, bool EPI>
 int launch_gemm_bn(const GemmParams &p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
-  bool ts = p.N % 8 == 0;
+  bool ts = sizeof(TO) == 2 && p.N % 8 == 0;
   for (const void *q : {(const void *)p.c, (const void *)p.z, p.res, p.bias, (const void *)p.col_scale}) ts = ts && reinterpret_cast<uintptr_t>(q) % 16 == 0;
-  return ts ? launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, true>(p, a, a_pitch, b, b_pitch, dtype, st)
-            : launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, false>(p, a, a_pitch, b, b_pitch, dtype, st);
+  if constexpr (sizeof(TO) == 2) {
+    if (ts) return launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, true>(p, a, a_pitch, b, b_pitch, dtype, st);
+  }
+  return launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, false>(p, a, a_pitch, b, b_pitch, dtype, st);
 }
 
-// The tile's width by the time of the rounds it takes: a round of 256 columns costs 256, of 128 columns 160 and of 64 columns 110
-// (a narrower tile reads the same rows of A for fewer products; measured on 4096 x 4096 x 4096 and 256 x 2048 x 2048, bf16).
+// A product's tile width and the number of runs its sum is cut into, by an estimate of its time in us: rounds of tiles over the pairs
+// of SMs times the blocks of a run at 0.30, 0.22 and 0.20 us (256, 128 and 64 columns; measured on products of one round to forty),
+// and for a sum in runs the partial matrices' way through memory and the launch that joins them.  Cutting pays where few tiles have
+// a long sum: dW of 13943 x 192 x 64 was 73 us in one run a tile.
+struct GemmPlan {
+  int bn, splits, kper;
+  size_t bytes;  // of partial sums
+};
+GemmPlan gemm_plan(int M, int N, int K, bool f8, bool bmn) {
+  const long long rows = (M + 255) / 256, clusters = sm_count() / 2;
+  const int kb = (K + (f8 ? 127 : 63)) / (f8 ? 128 : 64);
+  GemmPlan best = {256, 1, kb, 0};
+  double least = 1e30;
+  for (int bn : {256, 128, 64}) {
+    if (bmn && bn == 64) continue;
+    const long long tiles = rows * ((N + bn - 1) / bn);
+    for (int want = 1; want <= 64; want *= 2) {
+      if (want > 1 && (tiles * want > clusters || kb < 4 * want)) break;
+      const int kper = (kb + want - 1) / want, splits = (kb + kper - 1) / kper;
+      double us = (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.30 : bn == 128 ? 0.22 : 0.20);
+      if (splits > 1) us += 6.0 + 8.0 * splits * M * N / 3.0e6;
+      if (us < least) least = us, best = {bn, splits, kper, splits > 1 ? (size_t)splits * M * N * 4 : 0};
+    }
+  }
+  return best;
+}
+
 template <typename TO, bool F8, int T16, bool AMN, bool BMN, bool EPI>
-int launch_gemm(const GemmParams &p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, cudaStream_t st) {
-  const long long rows = (p.M + 255) / 256, clusters = sm_count() / 2;
-  auto cost = [&](int bn, int each) { return (rows * ((p.N + bn - 1) / bn) + clusters - 1) / clusters * each; };
-  const long long c256 = cost(256, 256), c128 = cost(128, 160), c64 = BMN ? c256 + c128 : cost(64, 110);
-  if (c256 <= c128 && c256 <= c64) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 256, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
-  if (c128 <= c64) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 128, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
-  if constexpr (!BMN) return launch_gemm_bn<TO, F8, T16, AMN, BMN, 64, EPI>(p, a, a_pitch, b, b_pitch, dtype, st);
-  return FLAB_E_UNSUPPORTED;
+int launch_gemm(GemmParams p, const void *a, int a_pitch, const void *b, int b_pitch, int dtype, void *scratch, size_t scratch_bytes, cudaStream_t st) {
+  const GemmPlan q = gemm_plan(p.M, p.N, p.K, F8, BMN);
+  p.splits = q.splits, p.kper = q.kper;
+  auto widths = [&](auto to, auto epi, const GemmParams &g) {
+    typedef decltype(to) O;
+    constexpr bool E = decltype(epi)::value;
+    if (q.bn == 256) return launch_gemm_bn<O, F8, T16, AMN, BMN, 256, E>(g, a, a_pitch, b, b_pitch, dtype, st);
+    if constexpr (!BMN) {
+      if (q.bn == 64) return launch_gemm_bn<O, F8, T16, AMN, BMN, 64, E>(g, a, a_pitch, b, b_pitch, dtype, st);
+    }
+    return launch_gemm_bn<O, F8, T16, AMN, BMN, 128, E>(g, a, a_pitch, b, b_pitch, dtype, st);
+  };
+  if (q.splits == 1) return widths(TO(), std::integral_constant<bool, EPI>(), p);
+  FLAB_REQUIRE(scratch && scratch_bytes >= q.bytes && reinterpret_cast<uintptr_t>(scratch) % 256 == 0, FLAB_E_BADARG,
+               "linear needs a 256-byte aligned scratch of flab_linear_scratch() or flab_linear_bwd_scratch() bytes");
+  GemmParams g = p;
+  g.c = scratch, g.z = nullptr, g.bias = g.res = nullptr, g.act = 0, g.pairs = p.N % 2 == 0;
+  int rc = widths(float(), std::false_type(), g);
+  if (rc) return rc;
+  bool wide = p.N % 8 == 0;
+  for (const void *r : {(const void *)p.c, (const void *)p.z, p.res}) wide = wide && reinterpret_cast<uintptr_t>(r) % 16 == 0;
+  const long long total = (long long)p.M * p.N, per = wide ? 8 : 1;
+  const unsigned blocks = (unsigned)((total / per + 255) / 256);
+  if (wide) join_kernel<TO, 8><<<blocks, 256, 0, st>>>((const float *)scratch, q.splits, p);
+  else join_kernel<TO, 1><<<blocks, 256, 0, st>>>((const float *)scratch, q.splits, p);
+  return check_launch("linear join");
 }
 
 template <typename... Ptr> bool four(int n, Ptr... ptr) {
@@ -590,8 +725,12 @@ int operands(Operands &o, const void *x, const void *w, int M, int N, int K, voi
   if (xb) o.x = a.to;
   if (wb) o.w = b.to;
   if (copied) return FLAB_OK;
-  const int blocks = (a.rows + b.rows + 7) / 8, cap = sm_count() * 8;
-  repitch_kernel<<<blocks < cap ? blocks : cap, 256, 0, st>>>(a, b);
+  const int blocks = (a.rows + b.rows + 7) / 8, cap = sm_count() * 8, grid = blocks < cap ? blocks : cap;
+  int by = K % 4 == 0 ? 4 : K % 2 == 0 ? 2 : 1;
+  while (by > 1 && ((xb && reinterpret_cast<uintptr_t>(x) % (2 * by)) || (wb && reinterpret_cast<uintptr_t>(w) % (2 * by)))) by /= 2;
+  if (by == 4) repitch_kernel<4><<<grid, 256, 0, st>>>(a, b);
+  else if (by == 2) repitch_kernel<2><<<grid, 256, 0, st>>>(a, b);
+  else repitch_kernel<1><<<grid, 256, 0, st>>>(a, b);
   return check_launch("linear repitch");
 }
 
@@ -609,14 +748,20 @@ size_t flab_linear_workspace(const void *x, const void *weight, int M, int N, in
   return (as_is(x, K) ? 0 : copy_bytes(M, K)) + (as_is(weight, K) ? 0 : copy_bytes(N, K));
 }
 
-size_t flab_linear_bwd_workspace(const void *dy, int M, int N, int act) {
+size_t flab_linear_scratch(int M, int N, int K, int dtype) {
   using namespace flab;
-  if (M <= 0 || N <= 0) return 0;
-  return act == ACT_NONE && as_is(dy, N) ? 0 : copy_bytes(M, N);
+  return M <= 0 || N <= 0 || K <= 0 ? 0 : gemm_plan(M, N, K, dtype == FLAB_E4M3, false).bytes;
+}
+
+size_t flab_linear_bwd_scratch(const void *dy, int M, int N, int K, int act) {
+  using namespace flab;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const size_t a = gemm_plan(M, K, N, false, true).bytes, b = gemm_plan(N, K, M, false, true).bytes;
+  return (act == ACT_NONE && as_is(dy, N) ? 0 : copy_bytes(M, N)) + (a > b ? a : b);
 }
 
 int flab_linear_fwd(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *z, int M, int N, int K, int act, int dtype,
-                    void *ws, size_t ws_bytes, void *stream) {
+                    void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream) {
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M >= 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_fwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
@@ -631,34 +776,37 @@ int flab_linear_fwd(const void *x, const void *weight, const void *bias, const v
   p.M = M, p.N = N, p.K = K, p.c = y, p.z = z, p.bias = bias, p.res = residual, p.act = act;
   p.pairs = four(N, y, z, residual);
   const int kp = pitch_of(K);
-  return dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, false, true>(p, o.x, kp, o.w, kp, dtype, st)
-                            : launch_gemm<__half, false, 0, false, false, true>(p, o.x, kp, o.w, kp, dtype, st);
+  return dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, false, true>(p, o.x, kp, o.w, kp, dtype, scratch, scratch_bytes, st)
+                            : launch_gemm<__half, false, 0, false, false, true>(p, o.x, kp, o.w, kp, dtype, scratch, scratch_bytes, st);
 }
 
 int flab_linear_bwd_partials(int M) { return M <= 0 ? 1 : (M + flab::RUN - 1) / flab::RUN; }
 
 int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *dy, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
-                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *bwd_ws, size_t bwd_ws_bytes, void *stream) {
+                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream) {
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M > 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_bwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
   FLAB_REQUIRE(dtype == FLAB_BF16 || dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_bwd: element type %d is not supported", dtype);
   FLAB_REQUIRE(dy && ((!dx && !dweight) || (x && weight)) && (act == ACT_NONE || z) && (!dbias || db_partial), FLAB_E_BADARG,
                "linear_bwd needs dy, x and weight for dx or dweight, z for an activation, db_partial for dbias");
-  FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0 && reinterpret_cast<uintptr_t>(bwd_ws) % 256 == 0, FLAB_E_BADARG,
-               "linear_bwd: ws and bwd_ws must be 256-byte aligned");
+  FLAB_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0 && reinterpret_cast<uintptr_t>(scratch) % 256 == 0, FLAB_E_BADARG,
+               "linear_bwd: ws and scratch must be 256-byte aligned");
   Operands o = {x, weight, 0};
   int rc = dx || dweight ? operands(o, x, weight, M, N, K, ws, ws_bytes, true, st) : FLAB_OK;
   if (rc) return rc;
   const void *dz = dy;
   const int zp = pitch_of(N), kp = pitch_of(K);
-  const size_t dz_bytes = flab_linear_bwd_workspace(dy, M, N, act);
+  const size_t dz_bytes = act == ACT_NONE && as_is(dy, N) ? 0 : copy_bytes(M, N);
   const bool make_dz = (dx || dweight) && dz_bytes;
+  char *part = reinterpret_cast<char *>(scratch);  // of partial sums, behind dz
+  size_t part_bytes = scratch_bytes;
   if (make_dz || dbias) {
     void *out = nullptr;
     if (make_dz) {
-      FLAB_REQUIRE(bwd_ws && bwd_ws_bytes >= dz_bytes, FLAB_E_BADARG, "linear_bwd needs a workspace of flab_linear_bwd_workspace() bytes");
-      dz = out = bwd_ws;
+      FLAB_REQUIRE(scratch && scratch_bytes >= dz_bytes, FLAB_E_BADARG, "linear_bwd needs a scratch of flab_linear_bwd_scratch() bytes");
+      dz = out = scratch;
+      part += dz_bytes, part_bytes -= dz_bytes;
     }
     rc = dtype == FLAB_BF16 ? launch_act_bwd<bf16>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st)
                             : launch_act_bwd<__half>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st);
@@ -668,21 +816,21 @@ int flab_linear_bwd(const void *x, const void *weight, const void *z, const void
   GemmParams p = {};
   if (dx) {
     p.M = M, p.N = K, p.K = N, p.c = dx, p.pairs = four(K, dx);
-    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, true, false>(p, dz, zp, o.w, kp, dtype, st)
-                            : launch_gemm<__half, false, 0, false, true, false>(p, dz, zp, o.w, kp, dtype, st);
+    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, false, true, false>(p, dz, zp, o.w, kp, dtype, part, part_bytes, st)
+                            : launch_gemm<__half, false, 0, false, true, false>(p, dz, zp, o.w, kp, dtype, part, part_bytes, st);
     if (rc) return rc;
   }
   if (dweight) {
     p.M = N, p.N = K, p.K = M, p.c = dweight, p.pairs = four(K, dweight);
-    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, true, true, false>(p, dz, zp, o.x, kp, dtype, st)
-                            : launch_gemm<__half, false, 0, true, true, false>(p, dz, zp, o.x, kp, dtype, st);
+    rc = dtype == FLAB_BF16 ? launch_gemm<bf16, false, 1, true, true, false>(p, dz, zp, o.x, kp, dtype, part, part_bytes, st)
+                            : launch_gemm<__half, false, 0, true, true, false>(p, dz, zp, o.x, kp, dtype, part, part_bytes, st);
     if (rc) return rc;
   }
   return FLAB_OK;
 }
 
 int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, const float *w_scale, const void *bias, const void *residual, void *y, int M,
-                     int N, int K, int act, int out_dtype, void *stream) {
+                     int N, int K, int act, int out_dtype, void *scratch, size_t scratch_bytes, void *stream) {
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M >= 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_e4m3: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
@@ -694,7 +842,7 @@ int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, co
   GemmParams p = {};
   p.M = M, p.N = N, p.K = K, p.c = y, p.bias = bias, p.res = residual, p.act = act, p.row_scale = x_scale, p.col_scale = w_scale;
   p.pairs = four(N, y, residual);
-  return out_dtype == FLAB_BF16 ? launch_gemm<bf16, true, 0, false, false, true>(p, x, K, weight, K, FLAB_E4M3, st)
-                                : launch_gemm<__half, true, 0, false, false, true>(p, x, K, weight, K, FLAB_E4M3, st);
+  return out_dtype == FLAB_BF16 ? launch_gemm<bf16, true, 0, false, false, true>(p, x, K, weight, K, FLAB_E4M3, scratch, scratch_bytes, st)
+                                : launch_gemm<__half, true, 0, false, false, true>(p, x, K, weight, K, FLAB_E4M3, scratch, scratch_bytes, st);
 }
 }

@@ -524,11 +524,12 @@ void norm_split(long long rows, long long groups, int most, int &tpr, int &nv) {
   if (nv == 0) tpr = 1024;
 }
 
-bool aligned16(std::initializer_list<const void *> ptrs) {
+bool aligned_to(int bytes, std::initializer_list<const void *> ptrs) {
   for (const void *q : ptrs)
-    if (reinterpret_cast<uintptr_t>(q) % 16 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(q) % bytes != 0) return false;
   return true;
 }
+bool aligned16(std::initializer_list<const void *> ptrs) { return aligned_to(16, ptrs); }
 
 // The ring's shape for rows of n elements (V a vector) of which a stage holds row_bytes; nv = 0: not for this row.  It pays where
 // every group has several rows to walk (measured at 2048 columns of bf16: ring 95 against 110 us at 32768 rows, the direct kernel
@@ -538,12 +539,13 @@ bool ring_shape(long long rows, int n, int V, int row_bytes, RingShape &q, int &
   q.tpr = 32;
   while (2 * q.tpr < vecs && q.tpr < RING_THREADS) q.tpr *= 2;
   nv = (vecs + q.tpr - 1) / q.tpr;
+  if (nv == 3) nv = 4;
   q.groups = RING_THREADS / q.tpr;
   q.row_bytes = row_bytes;
   q.stages = (int)(200 * 1024 / ((size_t)q.groups * row_bytes));
   if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
   grid = sm_count();
-  return nv <= 2 && q.stages >= 2 && rows >= 4ll * q.groups * grid;
+  return nv <= (V == 4 ? 4 : 2) && q.stages >= 2 && rows >= 4ll * q.groups * grid;
 }
 
 template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_norm_fwd(NormParams p, cudaStream_t st) {
@@ -560,22 +562,27 @@ template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_nor
       kernel<<<grid_ring, RING_THREADS, bytes, st>>>(p, q);
       return check_launch("rms_norm_fwd");
     };
+    if constexpr (V == 4) {
+      if (nv == 4) return launch(rms_norm_fwd_ring_kernel<T, S, RES, 4, QUANT>);
+    }
     return nv == 1 ? launch(rms_norm_fwd_ring_kernel<T, S, RES, 1, QUANT>) : launch(rms_norm_fwd_ring_kernel<T, S, RES, 2, QUANT>);
   }
   nv = 0;
-  if (aligned) norm_split(p.rows, p.n / V, 8, p.tpr, nv);
-  const bool vec = nv > 0;
-  if (!vec) norm_split(p.rows, p.n, 8, p.tpr, nv);
+  int by = aligned ? V : p.n % 2 == 0 && aligned_to(8, {p.x, p.res, p.w, p.y, p.sum}) ? 2 : 1;  // elements a load
+  norm_split(p.rows, p.n / by, 8, p.tpr, nv);
+  if (nv == 0 && by > 1) by = 1, norm_split(p.rows, p.n, 8, p.tpr, nv);
   const int block = p.tpr < 128 ? 128 : p.tpr;
   const unsigned grid = (unsigned)((p.rows + block / p.tpr - 1) / (block / p.tpr));
 #define FLAB_NORM(VV, NN) rms_norm_fwd_kernel<T, S, RES, VV, NN, QUANT, NORM><<<grid, block, 0, st>>>(p)
-  if (vec) {
+  if (by == V) {
     switch (nv) {
       case 1: FLAB_NORM(V, 1); break;
       case 2: FLAB_NORM(V, 2); break;
       case 4: FLAB_NORM(V, 4); break;
       default: FLAB_NORM(V, 8); break;
     }
+  } else if (by == 2) {
+    FLAB_NORM(2, 8);
   } else if (nv) {
     FLAB_NORM(1, 8);
   } else {
@@ -601,20 +608,15 @@ template <typename T> int norm_fwd_typed(const NormParams &p, bool wide, bool qu
 
 // the shape of a backward launch: everything that its number of partial rows depends on
 struct NormBwdPlan {
-  int tpr, nv, block, grid;
-  bool vec;
+  int by, tpr, nv, block, grid;  // elements a load, threads a row, vectors a thread
 };
-NormBwdPlan norm_bwd_plan(long long rows, int n, int esize, bool vec) {
+NormBwdPlan norm_bwd_plan(long long rows, int n, int esize, int by) {
   NormBwdPlan q;
-  const int V = 16 / esize;
-  q.vec = vec && n % V == 0;
-  if (q.vec) {
-    norm_split(rows, n / V, 4, q.tpr, q.nv);
-    q.vec = q.nv > 0 && q.tpr <= 256;
-  }
-  if (!q.vec) {
-    norm_split(rows, n, 16, q.tpr, q.nv);
-    if (q.tpr > 256) q.tpr = 1024, q.nv = 0;
+  q.by = by;
+  norm_split(rows, n / by, by == 16 / esize ? 4 : by == 2 ? 8 : 16, q.tpr, q.nv);
+  if (q.nv == 0 || q.tpr > 256) {
+    if (by > 1) return norm_bwd_plan(rows, n, esize, 1);
+    q.tpr = 1024, q.nv = 0;
   }
   q.block = q.nv ? 256 : 1024;
   const long long want = (rows + q.block / q.tpr - 1) / (q.block / q.tpr), cap = (long long)sm_count() * (q.nv ? 2 : 1);
@@ -637,9 +639,13 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
       kernel<<<parts, RING_THREADS, bytes, st>>>(p, r);
       return check_launch("rms_norm_bwd");
     };
+    if constexpr (V == 4) {
+      if (nv == 4) return launch(rms_norm_bwd_ring_kernel<T, S, 4>);
+    }
     return nv == 1 ? launch(rms_norm_bwd_ring_kernel<T, S, 1>) : launch(rms_norm_bwd_ring_kernel<T, S, 2>);
   }
-  const NormBwdPlan q = norm_bwd_plan(p.rows, p.n, sizeof(T), aligned);
+  const int by = aligned && p.n % V == 0 ? V : p.n % 2 == 0 && aligned_to(8, {p.s, p.dy, p.ds, p.w, p.dx, p.dr}) ? 2 : 1;
+  const NormBwdPlan q = norm_bwd_plan(p.rows, p.n, sizeof(T), by);
   p.tpr = q.tpr;
   parts = q.grid;
   const size_t bytes = p.part ? (size_t)(q.block / q.tpr) * p.n * sizeof(float) : 0;
@@ -651,12 +657,14 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
     if (rc) return rc;                                                                                                                      \
     kernel<<<q.grid, q.block, bytes, st>>>(p);                                                                                              \
   } while (0)
-  if (q.vec) {
+  if (q.by == V) {
     switch (q.nv) {
       case 1: FLAB_NORM(V, 1); break;
       case 2: FLAB_NORM(V, 2); break;
       default: FLAB_NORM(V, 4); break;
     }
+  } else if (q.by == 2) {
+    FLAB_NORM(2, 8);
   } else if (q.nv == 16) {
     FLAB_NORM(1, 16);
   } else if (q.nv) {
@@ -709,9 +717,13 @@ int flab_rms_norm_fwd(const void *x, const void *residual, const void *weight, v
 int flab_rms_norm_partials(long long rows, int n, int dtype) {
   if (rows <= 0 || n <= 0) return 1;
   const int e = dtype == FLAB_FP32 ? 4 : 2;
-  const int a = flab::norm_bwd_plan(rows, n, e, true).grid, b = flab::norm_bwd_plan(rows, n, e, false).grid;
-  const int sms = flab::sm_count();  // the ring's grid
-  return a > b ? (a > sms ? a : sms) : b > sms ? b : sms;
+  int most = flab::sm_count();  // the ring's grid
+  for (int by : {16 / e, 2, 1}) {
+    if (n % by) continue;
+    const int grid = flab::norm_bwd_plan(rows, n, e, by).grid;
+    most = grid > most ? grid : most;
+  }
+  return most;
 }
 
 int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const void *weight, const float *rstd, void *dx, void *dresidual, void *dweight,

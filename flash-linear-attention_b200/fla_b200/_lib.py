@@ -119,16 +119,18 @@ def load() -> ctypes.CDLL:
     sz = ctypes.c_size_t
     lib.flab_linear_workspace.restype = sz
     lib.flab_linear_workspace.argtypes = [vp, vp, ci, ci, ci]
-    lib.flab_linear_bwd_workspace.restype = sz
-    lib.flab_linear_bwd_workspace.argtypes = [vp, ci, ci, ci]
+    lib.flab_linear_scratch.restype = sz
+    lib.flab_linear_scratch.argtypes = [ci, ci, ci, ci]
+    lib.flab_linear_bwd_scratch.restype = sz
+    lib.flab_linear_bwd_scratch.argtypes = [vp, ci, ci, ci, ci]
     lib.flab_linear_fwd.restype = ci
-    lib.flab_linear_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp]
+    lib.flab_linear_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp, sz, vp]
     lib.flab_linear_bwd_partials.restype = ci
     lib.flab_linear_bwd_partials.argtypes = [ci]
     lib.flab_linear_bwd.restype = ci
     lib.flab_linear_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp, sz, vp]
     lib.flab_linear_e4m3.restype = ci
-    lib.flab_linear_e4m3.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp]
+    lib.flab_linear_e4m3.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp]
     lib.flab_hgrn_workspace.restype = sz
     lib.flab_hgrn_workspace.argtypes = [ci, ll, ci]
     lib.flab_hgrn_fwd.restype = ci

@@ -45,9 +45,11 @@ def _forward(x2, w, b, r2, act, want_z):
         n = 0 if _as_is(x2, K) and _as_is(w, K) else lib.flab_linear_workspace(x2.data_ptr(), w.data_ptr(), M, N, K)
         if n:
             copies = torch.empty(n, dtype=torch.uint8, device=x2.device)
-        with _lib.device_of(x2):
+        with _lib.device_of(x2):  # (the scratch's size goes by the device's)
+            m = lib.flab_linear_scratch(M, N, K, _DTYPES[x2.dtype])
+            scratch = torch.empty(m, dtype=torch.uint8, device=x2.device) if m else None
             rc = lib.flab_linear_fwd(x2.data_ptr(), w.data_ptr(), _p(b), _p(r2), y.data_ptr(), _p(z), M, N, K, act, _DTYPES[x2.dtype], _p(copies), n,
-                                     _lib.stream_of(x2))
+                                     _p(scratch), m, _lib.stream_of(x2))
         _lib.finish("flab_linear_fwd", rc)
     return y, z, copies
 
@@ -66,14 +68,14 @@ def _backward(ctx, dy):
                 t.zero_()
     elif need_x or need_w or need_b:
         lib = _lib.load()
-        n = lib.flab_linear_bwd_workspace(d2.data_ptr(), M, N, ctx.act) if need_x or need_w else 0
-        dz = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         part = torch.empty(lib.flab_linear_bwd_partials(M), N, dtype=torch.float32, device=dev) if need_b else None
         # (an operand that was copied, or whose product is not wanted, is not kept: its address only says how the copies lie)
         x_at, w_at = ctx.places
         with _lib.device_of(d2):
+            n = lib.flab_linear_bwd_scratch(d2.data_ptr(), M, N, K, ctx.act) if need_x or need_w else 0
+            scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
             rc = lib.flab_linear_bwd(x_at, w_at, _p(z), d2.data_ptr(), _p(dx), _p(dw), _p(db), _p(part), M, N, K, ctx.act, _DTYPES[dy.dtype],
-                                     _p(copies), 0 if copies is None else copies.numel(), _p(dz), n, _lib.stream_of(d2))
+                                     _p(copies), 0 if copies is None else copies.numel(), _p(scratch), n, _lib.stream_of(d2))
         _lib.finish("flab_linear_bwd", rc)
     return (None if dx is None else _like(dx, ctx.x_shape)), dw, db, (dy if need_r else None), None
 
@@ -158,7 +160,9 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     if M:
         lib = _lib.load()
         with _lib.device_of(x2):
+            n = lib.flab_linear_scratch(M, N, K, 3)
+            scratch = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
             rc = lib.flab_linear_e4m3(x2.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), _p(b), _p(r2), y.data_ptr(), M, N, K,
-                                      ACTIVATIONS[activation], _DTYPES[out_dtype], _lib.stream_of(x2))
+                                      ACTIVATIONS[activation], _DTYPES[out_dtype], _p(scratch), n, _lib.stream_of(x2))
         _lib.finish("flab_linear_e4m3", rc)
     return _like(y, x.shape[:-1] + (N,))

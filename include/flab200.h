@@ -151,19 +151,21 @@ int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const v
  * needs with an activation. Each of dx, dweight, dbias may be NULL; db_partial: fp32 [flab_linear_bwd_partials(M), N], summed in a
  * fixed order. ws: 256-byte aligned scratch of flab_linear_workspace() bytes, for copies of operands whose rows do not begin on
  * 16-byte boundaries: forward fills it, and backward is given what forward filled, with the same x and weight (whose own bytes it
- * reads only where they were not copied, x for dweight and weight for dx). bwd_ws: 256-byte aligned, flab_linear_bwd_workspace() bytes, for dz.
- * 0 bytes: NULL. M == 0 is a no-op in forward.
+ * reads only where they were not copied, x for dweight and weight for dx). scratch: 256-byte aligned, of flab_linear_scratch() or
+ * flab_linear_bwd_scratch() bytes (dtype FLAB_E4M3 for the e4m3 product), for dz and for partial sums where few tiles have a long
+ * sum; its contents mean nothing between calls. 0 bytes: NULL. M == 0 is a no-op in forward.
  * flab_linear_e4m3: operands of e4m3 bytes that stand for x * x_scale[row] and weight * w_scale[row] (fp32 [M], [N]); bias, residual
  * and y of type out_dtype (bf16 or fp16); K a multiple of 16, operands 16-byte aligned. */
 size_t flab_linear_workspace(const void *x, const void *weight, int M, int N, int K);
-size_t flab_linear_bwd_workspace(const void *d_y, int M, int N, int act);
+size_t flab_linear_scratch(int M, int N, int K, int dtype);
+size_t flab_linear_bwd_scratch(const void *d_y, int M, int N, int K, int act);
 int flab_linear_fwd(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *z, int M, int N, int K, int act, int dtype,
-                    void *ws, size_t ws_bytes, void *stream);
+                    void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream);
 int flab_linear_bwd_partials(int M);
 int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *d_y, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
-                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *bwd_ws, size_t bwd_ws_bytes, void *stream);
+                    int K, int act, int dtype, void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream);
 int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, const float *w_scale, const void *bias, const void *residual, void *y, int M,
-                     int N, int K, int act, int out_dtype, void *stream);
+                     int N, int K, int act, int out_dtype, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ---- causal depthwise short convolution (q, k, v of the reference's layers pass through it first) ----
  * Replaces the convolution of ShortConvolution.forward / .step (fla/modules/convolution.py:142-216):

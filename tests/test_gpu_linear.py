@@ -53,7 +53,8 @@ def expected(x, w, b, r, act):
 
 
 SIZES = [(1, 8, 8), (1, 1, 1), (7, 64, 64), (3, 33, 5), (64, 200, 130), (128, 128, 256), (129, 72, 257), (256, 64, 512), (300, 515, 257), (513, 1000, 96),
-         (40, 2048, 640), (2000, 72, 16), (1100, 136, 1032)]
+         (40, 2048, 640), (2000, 72, 16), (1100, 136, 1032),
+         (33, 4096, 40), (5000, 40, 72), (6, 48, 5000), (6, 50, 5001)]  # the last: sums cut into runs, in y, dw and dx
 
 
 @pytest.mark.gpu
@@ -94,7 +95,7 @@ def test_forward_and_gradients(M, K, N, act, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("out", [BF, FH])
 @pytest.mark.parametrize("act", [None, "silu", "gelu"])
-@pytest.mark.parametrize("M,K,N", [(1, 16, 8), (5, 128, 64), (130, 144, 257), (256, 1024, 512), (600, 272, 96), (1300, 64, 2000)])
+@pytest.mark.parametrize("M,K,N", [(1, 16, 8), (5, 128, 64), (130, 144, 257), (256, 1024, 512), (600, 272, 96), (1300, 64, 2000), (50, 16384, 40), (17, 8192, 129)])
 def test_eight_bits(M, K, N, act, out):
     x, w, b, r, _ = make(M, K, N, out, M * N + K)
     with torch.no_grad():
@@ -308,21 +309,27 @@ def test_refusals_on_the_device():
 
 def test_abi_refusals():
     lib = _lib.load()
-    assert lib.flab_linear_fwd(None, None, None, None, None, None, 0, 8, 8, 0, 0, None, 0, None) == 0
-    assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 5, 0, None, 0, None) == -1
+    none = (None, 0, None, 0, None)
+    assert lib.flab_linear_fwd(None, None, None, None, None, None, 0, 8, 8, 0, 0, *none) == 0
+    assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 5, 0, *none) == -1
     assert b"activation" in lib.flab_last_error()
-    assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 0, 2, None, 0, None) == -2
+    assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 0, 2, *none) == -2
     assert lib.flab_linear_workspace(16, 16, 8, 8, 8) == 0
     assert lib.flab_linear_workspace(16, 18, 8, 8, 8) == 256 and lib.flab_linear_workspace(16, 16, 8, 8, 7) == 512
-    assert lib.flab_linear_bwd_workspace(16, 8, 8, 0) == 0 and lib.flab_linear_bwd_workspace(16, 8, 8, 1) == 256
-    assert lib.flab_linear_bwd_workspace(18, 8, 8, 0) == 256
-    assert lib.flab_linear_fwd(16, 18, None, None, 16, None, 8, 8, 8, 0, 0, None, 0, None) == -1
+    assert lib.flab_linear_bwd_scratch(16, 8, 8, 8, 0) == 0 and lib.flab_linear_bwd_scratch(16, 8, 8, 8, 1) == 256
+    assert lib.flab_linear_bwd_scratch(18, 8, 8, 8, 0) == 256
+    # a long sum of few tiles is cut into runs, the ordinary sizes are not
+    assert lib.flab_linear_scratch(64, 64, 1 << 16, 0) > 0 and lib.flab_linear_scratch(32768, 2048, 2048, 0) == 0
+    assert lib.flab_linear_bwd_scratch(16, 1 << 16, 64, 64, 0) > 0
+    assert lib.flab_linear_fwd(16, 18, None, None, 16, None, 8, 8, 8, 0, 0, *none) == -1
     assert b"workspace" in lib.flab_last_error()
-    assert lib.flab_linear_bwd(16, 16, None, 16, 16, None, None, None, 8, 8, 8, 1, 0, None, 0, None, 0, None) == -1
-    assert lib.flab_linear_bwd(None, 16, None, 16, 16, None, None, None, 8, 8, 8, 0, 0, None, 0, None, 0, None) == -1
-    assert lib.flab_linear_bwd(16, 18, None, 16, 16, None, None, None, 8, 8, 8, 0, 0, None, 0, None, 0, None) == -1
+    assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 64, 64, 1 << 16, 0, 0, *none) == -1
+    assert b"scratch" in lib.flab_last_error()
+    assert lib.flab_linear_bwd(16, 16, None, 16, 16, None, None, None, 8, 8, 8, 1, 0, *none) == -1
+    assert lib.flab_linear_bwd(None, 16, None, 16, 16, None, None, None, 8, 8, 8, 0, 0, *none) == -1
+    assert lib.flab_linear_bwd(16, 18, None, 16, 16, None, None, None, 8, 8, 8, 0, 0, *none) == -1
     assert b"flab_linear_workspace" in lib.flab_last_error()
-    assert lib.flab_linear_bwd(16, 16, 16, 16, 16, None, None, None, 8, 8, 8, 1, 0, None, 0, None, 0, None) == -1
-    assert b"workspace" in lib.flab_last_error()
-    assert lib.flab_linear_e4m3(16, 16, 16, 16, None, None, 16, 8, 8, 24, 0, 0, None) == -2
+    assert lib.flab_linear_bwd(16, 16, 16, 16, 16, None, None, None, 8, 8, 8, 1, 0, *none) == -1
+    assert b"scratch" in lib.flab_last_error()
+    assert lib.flab_linear_e4m3(16, 16, 16, 16, None, None, 16, 8, 8, 24, 0, 0, None, 0, None) == -2
     assert b"multiple of 16" in lib.flab_last_error()

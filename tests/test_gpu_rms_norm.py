@@ -55,7 +55,7 @@ TYPES = [(BF, None, BF, False), (BF, BF, BF, False), (FH, FH, FH, False), (F32, 
          (BF, BF, F32, True), (FH, F32, FH, True), (BF, None, BF, True), (BF, BF, None, False)]
 SIZES = [(1, 1), (3, 8), (5, 33), (130, 64), (2, 1111), (67, 2048), (1, 4096), (300, 520), (2, 8192), (3, 9001), (2, 20000), (1, 33000), (700, 96),
          (9500, 40), (9473, 512), (5000, 264), (1300, 2048), (700, 8192), (2400, 1032),
-         (9500, 192), (3, 12288)]  # several rows a group of the ring; the last two ask for 48 KB of shared memory to the byte
+         (9500, 192), (3, 12288), (600, 6000), (90, 1378), (4, 4100), (2, 66)]  # several rows a group of the ring; the last two ask for 48 KB of shared memory to the byte
 
 
 @pytest.mark.gpu
