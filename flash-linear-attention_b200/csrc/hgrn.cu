@@ -51,8 +51,10 @@ template <typename T, int V> struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) 
   T v[V];
 };
 
+// (held inside the tensor, whatever the caller's table says: it is never read on the host)
 __device__ __forceinline__ long long cu_at(const HgrnParams &p, int n) {
-  return p.cu64 ? reinterpret_cast<const long long *>(p.cu)[n] : (long long)reinterpret_cast<const int *>(p.cu)[n];
+  const long long v = p.cu64 ? reinterpret_cast<const long long *>(p.cu)[n] : (long long)reinterpret_cast<const int *>(p.cu)[n];
+  return v < 0 ? 0 : v < p.T ? v : p.T;
 }
 
 // Row t of a packed batch: which sequence's first / last row it is, if any.  The sequence is the last one that begins at or
@@ -342,7 +344,7 @@ template <typename T> __device__ __forceinline__ void pack2(T *s, float a, float
 // The codes of the L rows from t0 on, by a warp: `n` is the last sequence that begins at or before t0 (-1: none).  Only the sequences
 // that lie in the tile are looked at; a row between two edges has code 0.
 template <int L> __device__ __forceinline__ void tile_codes(const HgrnParams &p, long long t0, int n, int *code, int lane) {
-  const long long begin = cu_at(p, 0), end = cu_at(p, p.N) < p.T ? cu_at(p, p.N) : p.T;
+  const long long begin = cu_at(p, 0), end = cu_at(p, p.N);
   for (int r = lane; r < L; r += 32) code[r] = t0 + r < begin || t0 + r >= end ? ROW_OUT : 0;
   __syncwarp();
   for (int j0 = n < 0 ? 0 : n;; j0 += 32) {

@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T *__restrict__ dy, 
     T v[V];
   };
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (blockIdx.x * 32 + lane) * V;
-  const int end = min(M, (int)(blockIdx.y + 1) * run);
+  const int end = (int)min((long long)M, (blockIdx.y + 1ll) * run);
   float sum[V] = {};
   if (c < N) {
 #pragma unroll 4
@@ -511,18 +511,19 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T *__restrict__ dy, 
     }
 }
 
-constexpr int RUN = 128;  // rows of a partial column sum
+// Rows of a partial column sum: 128, more where that would be more runs than a grid's second dimension holds.
+int run_of(int M) { return 128 * (int)((M + 128ll * 65535 - 1) / (128ll * 65535)); }
 
 template <typename T>
 int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, int N, int pitch, int act, cudaStream_t st) {
   const T *d = reinterpret_cast<const T *>(dy), *u = act ? reinterpret_cast<const T *>(z) : nullptr;
   T *o = reinterpret_cast<T *>(dz);
-  const unsigned runs = (M + RUN - 1) / RUN;
-  FLAB_REQUIRE(runs < 65536, FLAB_E_UNSUPPORTED, "linear_bwd: too many rows (%d)", M);
+  const int run = run_of(M);
+  const unsigned runs = (M + run - 1) / run;
   bool wide = N % 8 == 0;
   for (const void *q : {(const void *)d, (const void *)u, (const void *)o}) wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
-  if (wide) act_bwd_kernel<T, 8><<<dim3((N + 255) / 256, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, RUN, act);
-  else act_bwd_kernel<T, 1><<<dim3((N + 31) / 32, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, RUN, act);
+  if (wide) act_bwd_kernel<T, 8><<<dim3((N + 255) / 256, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, run, act);
+  else act_bwd_kernel<T, 1><<<dim3((N + 31) / 32, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, run, act);
   return check_launch("linear_bwd");
 }
 
@@ -780,7 +781,7 @@ int flab_linear_fwd(const void *x, const void *weight, const void *bias, const v
                             : launch_gemm<__half, false, 0, false, false, true>(p, o.x, kp, o.w, kp, dtype, scratch, scratch_bytes, st);
 }
 
-int flab_linear_bwd_partials(int M) { return M <= 0 ? 1 : (M + flab::RUN - 1) / flab::RUN; }
+int flab_linear_bwd_partials(int M) { return M <= 0 ? 1 : (int)((M + (long long)flab::run_of(M) - 1) / flab::run_of(M)); }
 
 int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *dy, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
                     int K, int act, int dtype, void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream) {

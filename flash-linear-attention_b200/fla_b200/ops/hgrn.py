@@ -126,8 +126,8 @@ def chunk_hgrn(
     """h_t = exp(g_t) h_{t-1} + x_t along dim 1, element by element.
 
     x, g: `[B, T, D]` of one type (bf16, fp16 or fp32), g the log of the forget gate; initial_state `[N, D]` or None (zeros).
-    offsets (or `cu_seqlens`): int32 / int64 `[N + 1]` cumulative lengths of N sequences packed into B = 1, beginning at 0 and
-    non-decreasing. They are read on the device only (no synchronisation, so a call can be captured into a CUDA graph); a
+    offsets (or `cu_seqlens`): int32 / int64 `[N + 1]` cumulative lengths of N sequences packed into B = 1, non-decreasing
+    and within [0, T]. They are read on the device only (no synchronisation, so a call can be captured into a CUDA graph); a
     sequence may be empty, and tokens outside every sequence get zeros in o and in the gradients.
     Returns (o `[B, T, D]`, final_state `[N, D]` fp32 or None)."""
     return _hgrn(x, g, initial_state, output_final_state, resolve_offsets(offsets, cu_seqlens))

@@ -303,7 +303,8 @@ int flab_recurrent_delta_bwd(const flab_args *a, void *stream);
  * x, g, o, d_o, dx, dg: [B, T, D] contiguous of element type dtype. h0 (h before a sequence) and dht (gradient of its last h)
  * fp32 [N, D] or NULL (zeros); ht (its last h) and dh0 (c at its first token) fp32 [N, D] or NULL (not wanted).
  * cu_seqlens NULL: N = B sequences of T tokens. Otherwise B = 1 and cu_seqlens holds the N + 1 cumulative lengths on the device
- * (int32, or int64 with cu_is_int64); empty sequences pass h0 to ht (dht to dh0), and rows of no sequence get zeros.
+ * (int32, or int64 with cu_is_int64), non-decreasing and within [0, T] (a value outside is taken as the nearer end, and no table makes
+ * a kernel leave its buffers); empty sequences pass h0 to ht (dht to dh0), and rows of no sequence get zeros.
  * Scratch: ws, 16-byte aligned, of flab_hgrn_workspace(B, T, D) bytes (0: ws may be NULL); its contents need no preparation.
  * Blocks wait for earlier blocks of the same launch, with a bound: flab_tc_check() reports a wait that ran out. */
 size_t flab_hgrn_workspace(int B, long long T, int D);

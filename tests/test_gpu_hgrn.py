@@ -230,6 +230,32 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 31])
+def test_tables_that_leave_the_tensor(D):
+    """Offsets beyond the tensor are taken as its ends, and leading tokens of no sequence get zeros; nothing outside is touched."""
+    T = 400
+    x, g, do, h0, dht = inputs(T, D, 3, torch.float32, 3, True)
+    bad = torch.tensor([-5, 150, 10 ** 6, 10 ** 6 + 3], dtype=torch.int32, device=DEV)
+    good = torch.tensor([0, 150, T, T], dtype=torch.int64, device=DEV)
+    late = torch.tensor([20, 150, 390, 390], dtype=torch.int32, device=DEV)
+
+    def run(off):
+        leaves = [v.to(DEV).requires_grad_(True) for v in (x.view(1, T, D), g.view(1, T, D), h0)]
+        o, ht = chunk_hgrn(*leaves[:2], initial_state=leaves[2], output_final_state=True, offsets=off)
+        return [o, ht, *torch.autograd.grad([o, ht], leaves, [do.to(DEV).view_as(o), dht.to(DEV)])]
+
+    for a, b in zip(run(bad), run(good)):
+        assert torch.equal(a, b)
+    o, ht, dx, dg, dh0 = run(late)
+    for v in (o, dx, dg):
+        assert (v[0, :20] == 0).all() and (v[0, 390:] == 0).all() and (v[0, 20:390] != 0).any()
+    want, last = loop(x[20:390].double(), g[20:390].double(), h0.double(), [130, 240, 0])
+    near("o", o[0, 20:390], want, torch.float32)
+    near("ht", ht, last, torch.float32)
+    assert torch.equal(ht[2], h0[2].to(DEV)) and torch.equal(dh0[2], dht[2].to(DEV))
+
+
+@pytest.mark.gpu
 def test_strided_inputs_other_stream_and_graph():
     B, T, D = 2, 333, 48
     gen = torch.Generator().manual_seed(0)
