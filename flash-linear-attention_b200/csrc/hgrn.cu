@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       const int group = z.step / G, first = group * G, before = z.step - first;
       const bool leader = before == G - 1 && z.step + 1 < p.nT;  // hands the group's end on
       auto words = [&](unsigned long long *base, int step) { return base + ((size_t)step * chains + z.chain) * C + lane * 2; };
-      if (before < G - 1) {
+      if (before < G - 1 && z.step + 1 < p.nT) {
         put(words(p.maps, z.step), map_word(jP.x, jQ.x));
         put(words(p.maps, z.step) + 1, map_word(jP.y, jQ.y));
       }
@@ -717,7 +717,7 @@ template <typename T, int V, bool BWD> __global__ void __launch_bounds__(256) hg
   const size_t state = (size_t)b * p.D + ch;
   if (edge) c = *reinterpret_cast<const PF *>(edge + state);
   if (BWD && p.h0) h = *reinterpret_cast<const PF *>(p.h0 + state);
-  constexpr int U = BWD ? 4 : 8;  // tokens whose loads are in flight together
+  constexpr int U = BWD && V * sizeof(T) == 16 ? 4 : 8;  // tokens whose loads are in flight together
   const int last = (int)p.T - 1;
   for (int k0 = 0; k0 <= last; k0 += U) {
     PV g[U], x[U], o[BWD ? U : 1];
@@ -772,7 +772,7 @@ HgrnPlan hgrn_plan(int B, long long T, int D, int V, int L) {
   q.nT = (int)((T + L - 1) / L);
   q.nCG = (D + q.C - 1) / q.C;
   q.tiles = (long long)q.nT * B * q.nCG;
-  q.map_bytes = (size_t)q.tiles * q.C * 8;
+  q.map_bytes = q.nT > 1 ? (size_t)q.tiles * q.C * 8 : 0;
   q.end_bytes = (size_t)(q.nT / G) * B * q.nCG * q.C * 8;
   q.bytes = 256 + q.end_bytes + q.map_bytes;
   return q;
@@ -832,11 +832,11 @@ template <typename T, bool BWD, bool VAR> int launch_stream(HgrnParams p, void *
   return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
 }
 
-// Fixed-length sequences that are walked by one thread a channel group instead of being put into tiles: up to 32 tokens, of which a
-// tile would be mostly empty rows (62 x 15 x 1821 fp32: tiles 33 us forward, the walk 9), and up to a tile's 128 where the
-// channels alone fill the card (128 x 44 x 1284 bf16: 32 and 12 us).
-bool walks(const HgrnParams &p, int V) {
-  return !p.cu && (p.T <= 32 || (p.T <= 128 && (long long)p.B * p.D / V >= 512ll * sm_count()));
+// Fixed-length sequences of up to WALK tokens are walked by one thread a channel group instead of being put into tiles, which they
+// would leave mostly empty.  Rows that TMA cannot address are walked up to a tile's 128 tokens where the channels alone fill the card.
+constexpr int WALK = 32;
+bool walks(const HgrnParams &p, int V, bool tma) {
+  return !p.cu && (p.T <= WALK || (!tma && p.T <= 128 && (long long)p.B * p.D / V >= 512ll * sm_count()));
 }
 
 template <typename T, bool BWD, int V> int launch_step(const HgrnParams &p, cudaStream_t st) {
@@ -860,9 +860,9 @@ template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws,
     wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
     pair = pair && reinterpret_cast<uintptr_t>(q) % 8 == 0;
   }
-  if (walks(p, wide ? WIDE : pair ? 2 : 1))
+  if (walks(p, wide ? WIDE : pair ? 2 : 1, tma))
     return wide ? launch_step<T, BWD, WIDE>(p, st) : pair ? launch_step<T, BWD, 2>(p, st) : launch_step<T, BWD, 1>(p, st);
-  if (tma && p.T > HgrnTile<T>::L)
+  if (tma)
     return p.cu ? launch_stream<T, BWD, true>(p, ws, ws_bytes, st) : launch_stream<T, BWD, false>(p, ws, ws_bytes, st);
   if (p.cu) return pair ? launch_hgrn<T, BWD, true, 2>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, true, 1>(p, ws, ws_bytes, st);
   return pair ? launch_hgrn<T, BWD, false, 2>(p, ws, ws_bytes, st) : launch_hgrn<T, BWD, false, 1>(p, ws, ws_bytes, st);
@@ -886,12 +886,12 @@ extern "C" {
 
 size_t flab_hgrn_workspace(int B, long long T, int D) {
   using namespace flab;
-  if (B <= 0 || T <= 0 || D <= 0) return 0;
+  if (B <= 0 || T <= 0 || D <= 0 || (B > 1 && T <= WALK)) return 0;
   size_t most = 0;  // of the layouts that a call of this size may take
   for (int V : {1, 2})
     for (int L : {64, HgrnTile<float>::L}) {
       const HgrnPlan q = hgrn_plan(B, T, D, V, L);
-      const size_t n = T > HgrnTile<float>::L ? q.bytes : 0;
+      const size_t n = q.bytes;
       most = n > most ? n : most;
     }
   return most;

@@ -63,7 +63,7 @@ struct GemmParams {
 };
 
 template <int BN> struct GemmShape {
-  static constexpr int S = BN == 256 ? 5 : 6;
+  static constexpr int S = BN == 256 ? 5 : BN == 128 ? 6 : 8;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
   static constexpr int TURN = 8192;  // a warp's staging: four blocks of 32 rows of 64 bytes, or one of 32 x 32 floats to turn
@@ -643,10 +643,11 @@ int launch_gemm_bn(const GemmParams &p, const void *a, int a_pitch, const void *
   return launch_gemm_ts<TO, F8, T16, AMN, BMN, BN, EPI, false>(p, a, a_pitch, b, b_pitch, dtype, st);
 }
 
-// A product's tile width and the number of runs its sum is cut into, by an estimate of its time in us: rounds of tiles over the pairs
-// of SMs times the blocks of a run at 0.30, 0.22 and 0.20 us (256, 128 and 64 columns; measured on products of one round to forty),
-// and for a sum in runs the partial matrices' way through memory and the launch that joins them.  Cutting pays where few tiles have
-// a long sum: dW of 13943 x 192 x 64 was 73 us in one run a tile.
+// A product's tile width and the number of runs its sum is cut into, by an estimate of its time in us: 4.5 and the rounds of tiles over
+// the pairs of SMs times the blocks of a run at 0.38, 0.36 and 0.34 us (256, 128 and 64 columns; 4096 x 4096 x 4096: 102, 162 and 303
+// us; a block's way through the stages bounds a single round, whatever its width).  A sum in runs adds the launch that joins them (5
+// us, and 4 for what a second launch costs its caller) and the partial matrices' way through L2.  Cutting pays where few tiles have a
+// long sum: 64 x 16384 x 256 87 us in one run, 16 in sixteen; 256 x 2048 x 2048 would gain 3 of 16 us on the device.
 struct GemmPlan {
   int bn, splits, kper;
   size_t bytes;  // of partial sums
@@ -662,8 +663,8 @@ GemmPlan gemm_plan(int M, int N, int K, bool f8, bool bmn) {
     for (int want = 1; want <= 64; want *= 2) {
       if (want > 1 && (tiles * want > clusters || kb < 4 * want)) break;
       const int kper = (kb + want - 1) / want, splits = (kb + kper - 1) / kper;
-      double us = (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.30 : bn == 128 ? 0.22 : 0.20);
-      if (splits > 1) us += 6.0 + 8.0 * splits * M * N / 3.0e6;
+      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.38 : bn == 128 ? 0.36 : 0.34);
+      if (splits > 1) us += 9.0 + 8.0 * splits * M * N / 8.0e6;
       if (us < least) least = us, best = {bn, splits, kper, splits > 1 ? (size_t)splits * M * N * 4 : 0};
     }
   }

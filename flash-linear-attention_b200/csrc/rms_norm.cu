@@ -531,10 +531,10 @@ bool aligned_to(int bytes, std::initializer_list<const void *> ptrs) {
 }
 bool aligned16(std::initializer_list<const void *> ptrs) { return aligned_to(16, ptrs); }
 
-// The ring's shape for rows of n elements (V a vector) of which a stage holds row_bytes; nv = 0: not for this row.  It pays where
-// every group has several rows to walk (measured at 2048 columns of bf16: ring 95 against 110 us at 32768 rows, the direct kernel
-// ahead below four rows a group, where filling the ring is all there is).
-bool ring_shape(long long rows, int n, int V, int row_bytes, RingShape &q, int &nv, int &grid) {
+// The ring's shape for rows of n elements (V a vector) of which a stage holds row_bytes; false: not for these rows.  It pays from so
+// many rows a group on (`enough`): forward at 2048 columns of bf16, 2368 rows 9.0 us against 8.8 without it, 4096 rows 13.4 against
+// 15.0, 32768 rows 78 against 98; backward 1184 rows 10.5 against 15.1, 32768 rows 102 against 213.
+bool ring_shape(long long rows, int n, int V, int row_bytes, int enough, RingShape &q, int &nv, int &grid) {
   const int vecs = n / V;
   q.tpr = 32;
   while (2 * q.tpr < vecs && q.tpr < RING_THREADS) q.tpr *= 2;
@@ -545,7 +545,7 @@ bool ring_shape(long long rows, int n, int V, int row_bytes, RingShape &q, int &
   q.stages = (int)(200 * 1024 / ((size_t)q.groups * row_bytes));
   if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
   grid = sm_count();
-  return nv <= (V == 4 ? 4 : 2) && q.stages >= 2 && rows >= 4ll * q.groups * grid;
+  return nv <= (V == 4 ? 4 : 2) && q.stages >= 2 && rows >= (long long)enough * q.groups * grid;
 }
 
 template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_norm_fwd(NormParams p, cudaStream_t st) {
@@ -554,7 +554,7 @@ template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_nor
   const bool aligned = p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum});
   RingShape q;
   int grid_ring;
-  if (NORM && aligned && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0)), q, nv, grid_ring)) {
+  if (NORM && aligned && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0)), 6, q, nv, grid_ring)) {
     const size_t bytes = (size_t)q.groups * q.stages * q.row_bytes;
     auto launch = [&](auto kernel) {
       const int rc = set_smem(kernel, bytes);
@@ -629,7 +629,7 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
   const bool aligned = aligned16({p.s, p.dy, p.ds, p.w, p.dx, p.dr});
   RingShape r;
   int nv;
-  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + 2 * sizeof(S)), r, nv, parts)) {
+  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + 2 * sizeof(S)), 2, r, nv, parts)) {
     size_t bytes = (size_t)r.groups * r.stages * r.row_bytes;
     const size_t sums = (size_t)r.groups * p.n * sizeof(float);
     if (bytes < sums) bytes = sums;

@@ -16,9 +16,8 @@ def _p(t):
 
 
 def _workspace(lib, ref):
-    """(scratch from the current stream's allocator, its bytes); none for what one tile holds."""
-    B, T, D = ref.shape
-    n = lib.flab_hgrn_workspace(B, T, D) if T > 64 else 0
+    """(scratch from the current stream's allocator, its bytes); none where every sequence is walked by itself."""
+    n = lib.flab_hgrn_workspace(*ref.shape)
     return (torch.empty(n, dtype=torch.uint8, device=ref.device) if n else None), n
 
 

@@ -355,7 +355,7 @@ def test_abi_refusals():
     assert lib.flab_hgrn_fwd(16, 16, None, 16, None, 16, 0, 2, 8, 8, 2, 0, None, 0, None) == -1
     assert b"B = 1" in lib.flab_last_error()
     # more than one tile along time needs the workspace
-    assert lib.flab_hgrn_workspace(1, 1, 8) == 0 and lib.flab_hgrn_workspace(1, 1 << 14, 8) > 0
+    assert lib.flab_hgrn_workspace(2, 32, 8) == 0 and lib.flab_hgrn_workspace(1, 1 << 14, 8) > 0
     assert lib.flab_hgrn_bwd(16, 16, None, 16, None, 16, 16, None, None, 0, 1, 1 << 14, 8, 1, 0, None, 0, None) == -1
     assert b"workspace" in lib.flab_last_error()
     assert lib.flab_hgrn_fwd(16, 16, None, 16, None, None, 0, 1, 8, 8, 1, 7, None, 0, None) == -1
