@@ -97,7 +97,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
   __syncthreads();
   tc::cluster_sync();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
   const int kblocks = (p.K + BK - 1) / BK, units = p.tiles * p.splits;
   auto run = [&](int unit, int &from, int &to) {  // a unit's blocks of the sum
     from = unit / p.tiles * p.kper;
@@ -110,11 +110,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
     tm = group * 8 + in - tn * high;
   };
 
+  // The two loops below are a warp's each: an iteration of theirs is the least that a block of the sum takes, so stages and phases are
+  // counted up, and addresses and descriptors added to.
   if (warp == 0) {  // ---- loads
     if (lane == 0) {
       tc::tma_prefetch_desc(&ma);
       tc::tma_prefetch_desc(&mb);
-      uint32_t it = 0;
+      const uint32_t bars = tc::peer_addr(&full[0], 0);
+      int s = 0;
+      uint32_t phase = 1;  // of `empty`: the first round finds every stage free
       bool ok = true;
       for (int unit = cluster; unit < units && ok; unit += clusters) {
         int tm, tn;
@@ -122,61 +126,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
         int k0, k1;
         run(unit, k0, k1);
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % S;
-          if (it >= S && !tc::mbar_wait(&empty[s], (it / S - 1) & 1)) {
+        for (int k = k0 * BK; k < k1 * BK; k += BK) {
+          if (!tc::mbar_wait(&empty[s], phase)) {
             tu_tc_error = 730;
             ok = false;
             break;
           }
-          const uint32_t bar = tc::peer_addr(&full[s], 0);
+          const uint32_t bar = bars + s * 8;
           if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * Z::STAGE);
           uint8_t *const a = buf + s * Z::STAGE, *const b = a + Z::A_BYTES;
           if constexpr (AMN) {
-            for (int i = 0; i < 2; ++i) tc::tma_load_2d_pair(a + i * 8192, &ma, bar, m0 + i * 64, kb * BK);
+            tc::tma_load_2d_pair(a, &ma, bar, m0, k);
+            tc::tma_load_2d_pair(a + 8192, &ma, bar, m0 + 64, k);
           } else {
-            tc::tma_load_2d_pair(a, &ma, bar, kb * BK, m0);
+            tc::tma_load_2d_pair(a, &ma, bar, k, m0);
           }
           if constexpr (BMN) {
-            for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(b + i * 8192, &mb, bar, n0 + i * 64, kb * BK);
+#pragma unroll
+            for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(b + i * 8192, &mb, bar, n0 + i * 64, k);
           } else {
-            tc::tma_load_2d_pair(b, &mb, bar, kb * BK, n0);
+            tc::tma_load_2d_pair(b, &mb, bar, k, n0);
           }
+          if (++s == S) s = 0, phase ^= 1;
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {  // ---- products
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = F8 ? tc::instr_desc(256, BN, 0, 0, 0) : tc::instr_desc(256, BN, T16, AMN, BMN);
-      uint32_t it = 0;
+      // addresses in a descriptor are in 16 bytes; shared memory's stay within its 14 bits
+      constexpr uint64_t A_STEP = AMN ? 128 : 2, B_STEP = BMN ? 128 : 2, STAGE_STEP = Z::STAGE / 16;
+      const uint32_t at = tc::smem_u32(buf), full0 = tc::smem_u32(&full[0]), empty0 = tc::smem_u32(&empty[0]);
+      const uint64_t a0 = AMN ? tc::desc_mnmajor(at, 0, 8192) : tc::desc_kmajor(at, 0, 0);
+      const uint64_t b0 = BMN ? tc::desc_mnmajor(at + Z::A_BYTES, 0, 8192) : tc::desc_kmajor(at + Z::A_BYTES, 0, 0);
+      const bool one = lane == 0;
+      uint64_t ad = a0, bd = b0;
+      int s = 0;
+      uint32_t phase = 0;
       int n = 0;
       bool ok = true;
       for (int unit = cluster; unit < units && ok; unit += clusters, ++n) {
         const int half = n & 1;
-        if (n >= 2 && !tc::mbar_wait(&acc_empty[half], (n / 2 - 1) & 1)) {
+        if (n >= 2 && !__all_sync(0xffffffffu, tc::mbar_wait(&acc_empty[half], (n / 2 - 1) & 1))) {
           tu_tc_error = 731;
           break;
         }
         tc::fence_after_sync();
+        const uint32_t d = tmem + half * BN;
+        uint32_t add = 0;
         int k0, k1;
         run(unit, k0, k1);
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % S;
-          if (!tc::mbar_wait(&full[s], (it / S) & 1)) {
+        for (int kb = k1 - k0; kb > 0; --kb) {
+          if (!__all_sync(0xffffffffu, tc::mbar_wait(full0 + s * 8, phase))) {
             tu_tc_error = 732;
             ok = false;
             break;
           }
-          tc::fence_after_sync();
-          const uint32_t a = tc::smem_u32(buf + s * Z::STAGE), b = a + Z::A_BYTES;
+          tc::umma_pair<F8>(one, d, ad, bd, idesc, add);
+          add = 1;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc::umma_pair<F8>(tmem + half * BN, AMN ? tc::desc_mnmajor(a, k, 8192) : tc::desc_kmajor(a, k, 0),
-                              BMN ? tc::desc_mnmajor(b, k, 8192) : tc::desc_kmajor(b, k, 0), idesc, kb > k0 || k > 0);
-          tc::umma_commit_pair(&empty[s]);
+          for (int k = 1; k < 4; ++k) tc::umma_pair<F8>(one, d, ad + k * A_STEP, bd + k * B_STEP, idesc, 1);
+          tc::umma_commit_pair(one, empty0 + s * 8);
+          ad += STAGE_STEP, bd += STAGE_STEP;
+          if (++s == S) s = 0, phase ^= 1, ad = a0, bd = b0;
         }
-        if (ok) tc::umma_commit_pair(&acc_full[half]);
+        if (ok) tc::umma_commit_pair(one, tc::smem_u32(&acc_full[half]));
       }
     }
     __syncwarp();

@@ -55,6 +55,24 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
   }
 }
 
+// the same on a shared-memory address
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  auto look = [&]() {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+  };
+  if (look()) return true;
+  const long long t0 = clock64();
+  while (true) {
+    if (look()) return true;
+    if (clock64() - t0 > (1ll << 31)) return false;
+  }
+}
+
 // The same wait with a caller-chosen limit in clock ticks (the wait self-test uses a short one).
 __device__ __forceinline__ bool mbar_wait_limit(uint64_t *bar, uint32_t parity, long long limit_ticks) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -264,23 +282,28 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst, uint32_t ncols) {
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
-template <bool F8> __device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Issued by the thread of a converged warp for which `one` holds: a warp that runs its loop as a whole keeps descriptors in uniform
+// registers, where a single thread's branch moves them there anew for every product (62 clocks each).
+template <bool F8>
+__device__ __forceinline__ void umma_pair(bool one, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   if constexpr (F8)
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n.reg .pred p, q;\nsetp.ne.b32 q, %5, 0;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"((uint32_t)one)
         : "memory");
   else
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n.reg .pred p, q;\nsetp.ne.b32 q, %5, 0;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"((uint32_t)one)
         : "memory");
 }
 // `bar` of both CTAs completes once all MMAs issued so far by this thread have finished
-__device__ __forceinline__ void umma_commit_pair(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-               "h"((uint16_t)3)
-               : "memory");
+__device__ __forceinline__ void umma_commit_pair(bool one, uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n"
+      ::"r"(bar), "h"((uint16_t)3), "r"((uint32_t)one)
+      : "memory");
 }
 
 // ---- swizzled shared-memory addressing for ordinary threads ---------------------------------------
