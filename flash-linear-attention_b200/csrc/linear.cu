@@ -113,42 +113,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
   // The two loops below are a warp's each: an iteration of theirs is the least that a block of the sum takes, so stages and phases are
   // counted up, and addresses and descriptors added to.
   if (warp == 0) {  // ---- loads
-    if (lane == 0) {
-      tc::tma_prefetch_desc(&ma);
-      tc::tma_prefetch_desc(&mb);
-      const uint32_t bars = tc::peer_addr(&full[0], 0);
-      int s = 0;
-      uint32_t phase = 1;  // of `empty`: the first round finds every stage free
-      bool ok = true;
-      for (int unit = cluster; unit < units && ok; unit += clusters) {
-        int tm, tn;
-        place(unit, tm, tn);
-        const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
-        int k0, k1;
-        run(unit, k0, k1);
-        for (int k = k0 * BK; k < k1 * BK; k += BK) {
-          if (!tc::mbar_wait(&empty[s], phase)) {
-            tu_tc_error = 730;
-            ok = false;
-            break;
-          }
-          const uint32_t bar = bars + s * 8;
-          if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * Z::STAGE);
-          uint8_t *const a = buf + s * Z::STAGE, *const b = a + Z::A_BYTES;
-          if constexpr (AMN) {
-            tc::tma_load_2d_pair(a, &ma, bar, m0, k);
-            tc::tma_load_2d_pair(a + 8192, &ma, bar, m0 + 64, k);
-          } else {
-            tc::tma_load_2d_pair(a, &ma, bar, k, m0);
-          }
-          if constexpr (BMN) {
-#pragma unroll
-            for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(b + i * 8192, &mb, bar, n0 + i * 64, k);
-          } else {
-            tc::tma_load_2d_pair(b, &mb, bar, k, n0);
-          }
-          if (++s == S) s = 0, phase ^= 1;
+    const bool one = lane == 0;
+    if (one) tc::tma_prefetch_desc(&ma), tc::tma_prefetch_desc(&mb);
+    const uint32_t bars = tc::peer_addr(&full[0], 0), full0 = tc::smem_u32(&full[0]), empty0 = tc::smem_u32(&empty[0]), stage0 = tc::smem_u32(buf);
+    int s = 0;
+    uint32_t phase = 1;  // of `empty`: the first round finds every stage free
+    bool ok = true;
+    for (int unit = cluster; unit < units && ok; unit += clusters) {
+      int tm, tn;
+      place(unit, tm, tn);
+      const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
+      int k0, k1;
+      run(unit, k0, k1);
+      for (int k = k0 * BK; k < k1 * BK; k += BK) {
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(empty0 + s * 8, phase))) {
+          tu_tc_error = 730;
+          ok = false;
+          break;
         }
+        const uint32_t bar = bars + s * 8, a = stage0 + s * Z::STAGE, b = a + Z::A_BYTES;
+        tc::mbar_expect_tx(one && rank == 0, full0 + s * 8, 2 * Z::STAGE);
+        if constexpr (AMN) {
+          tc::tma_load_2d_pair(one, a, &ma, bar, m0, k);
+          tc::tma_load_2d_pair(one, a + 8192, &ma, bar, m0 + 64, k);
+        } else {
+          tc::tma_load_2d_pair(one, a, &ma, bar, k, m0);
+        }
+        if constexpr (BMN) {
+#pragma unroll
+          for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(one, b + i * 8192, &mb, bar, n0 + i * 64, k);
+        } else {
+          tc::tma_load_2d_pair(one, b, &mb, bar, k, n0);
+        }
+        if (++s == S) s = 0, phase ^= 1;
       }
     }
     __syncwarp();
@@ -659,10 +656,10 @@ int launch_gemm_bn(const GemmParams &p, const void *a, int a_pitch, const void *
 }
 
 // A product's tile width and the number of runs its sum is cut into, by an estimate of its time in us: 4.5 and the rounds of tiles over
-// the pairs of SMs times the blocks of a run at 0.38, 0.36 and 0.34 us (256, 128 and 64 columns; 4096 x 4096 x 4096: 102, 162 and 303
-// us; a block's way through the stages bounds a single round, whatever its width).  A sum in runs adds the launch that joins them (5
+// the pairs of SMs times the blocks of a run at 0.37, 0.32 and 0.30 us (256, 128 and 64 columns; 4096 x 8192 x 4096: 195, 294 and 537
+// us; the loop over a block bounds the narrow ones).  A sum in runs adds the launch that joins them (5
 // us, and 4 for what a second launch costs its caller) and the partial matrices' way through L2.  Cutting pays where few tiles have a
-// long sum: 64 x 16384 x 256 87 us in one run, 16 in sixteen; 256 x 2048 x 2048 would gain 3 of 16 us on the device.
+// long sum: 64 x 16384 x 256 87 us in one run, 16 in sixteen; 256 x 2048 x 2048 would gain 3 of 15 us on the device.
 struct GemmPlan {
   int bn, splits, kper;
   size_t bytes;  // of partial sums
@@ -678,7 +675,7 @@ GemmPlan gemm_plan(int M, int N, int K, bool f8, bool bmn) {
     for (int want = 1; want <= 64; want *= 2) {
       if (want > 1 && (tiles * want > clusters || kb < 4 * want)) break;
       const int kper = (kb + want - 1) / want, splits = (kb + kper - 1) / kper;
-      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.38 : bn == 128 ? 0.36 : 0.34);
+      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.37 : bn == 128 ? 0.32 : 0.30);
       if (splits > 1) us += 9.0 + 8.0 * splits * M * N / 8.0e6;
       if (us < least) least = us, best = {bn, splits, kper, splits > 1 ? (size_t)splits * M * N * 4 : 0};
     }
