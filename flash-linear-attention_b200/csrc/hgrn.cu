@@ -10,10 +10,17 @@
 // it in registers: each warp composes R consecutive rows (lanes side by side over the channels), the warps' maps are joined
 // through shared memory, and the tile's start value comes from the tiles before it: every tile publishes its map, the last tile
 // of each group of G publishes the group's end value, and a tile takes the end of the group before its own through the maps of
-// its group's earlier tiles.  The sums are formed in the same order whatever block runs when, so results repeat bit for bit (a
-// look-back that takes whatever is there first would be no faster and would not).  Serial along time is one hop a group: a word
+// its group's earlier tiles.  The sums are formed in the same order whatever block runs when, so results repeat bit for bit (taking
+// whichever of a predecessor's map and end value is there first does not repeat).  Groups of 4 and of 16 were slower (forward at
+// [1, 262144, 1024] 480 and 575 us against 344: more hops, and more maps to fetch).  Serial along time is one hop a group: a word
 // of 64 bits that holds value and mark.  Tiles are handed out by a ticket in the order of time, so that a tile waits only for
 // tiles whose blocks already run; one launch then reads everything once, where a two-pass scan would read the inputs twice.
+// Three forms: rows that TMA can address stream through a persistent block (hgrn_stream_kernel), others go tile by tile through
+// registers (hgrn_tile_kernel), and a few tokens a sequence are walked by one thread a channel group (hgrn_step_kernel).
+// Measured against the bytes above at the copy rate of 6.55 TB/s, bf16: [8, 4096, 2048] forward 68 us (91 %), backward 107 us (96 %);
+// [1, 262144, 2048] forward 601 us (82 %), backward 944 us (87 %): 32 channel groups side by side, where a tile's wait for the loads
+// of all tiles before it is what the six (four) stages no longer cover; 64 packed sequences of 290000 tokens 723 and 1069 us; one
+// token of 256 x 2048 2.5 us.
 // All arithmetic and every state is fp32; o, dx, dg are rounded once, when stored.  Backward takes h_{t-1} from the stored o:
 // dg is a plain product with it, so the 16-bit rounding of o enters dg once, with the size of dg's own rounding, and backward
 // needs neither x nor a second forward scan.
@@ -329,7 +336,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
 //   chain warps  publish the tile's map, fetch what came before it and leave the start value of every R rows
 //   row warps    run the recurrence from there, outputs in place of inputs
 //   store warp   sends the tile off and hands the stage back
-// A tile's start value costs two or three trips to L2; the map warps being stages ahead of the row warps hides them, and keeps
+// A tile's start value costs a trip or two to L2; the map warps being stages ahead of the row warps hides them, and keeps
 // several groups of a long chain in flight.  Gates are evaluated twice (map, rows): two more instructions an element, against
 // 64 registers a thread that would have to live through the wait.
 template <typename T> __device__ __forceinline__ float2 unpack2(const T *s) {
