@@ -56,7 +56,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 struct GemmParams {
   int M, N, K;          // C [M, N]; K: the summed extent
   int tiles_m, tiles_n, tiles;
-  int splits, kper;     // the sum in `splits` runs of kper blocks of 128 bytes; each writes a matrix of its own behind the last one's
+  int splits, kper;     // the sum in `splits` runs of kper stages; each writes a matrix of its own behind the last one's
   void *c;              // [M, N]
   void *z;              // z before the activation, same type, or null
   const void *bias;     // [N] or null
@@ -67,8 +67,9 @@ struct GemmParams {
 };
 
 template <int BN> struct GemmShape {
-  static constexpr int S = BN == 256 ? 5 : BN == 128 ? 6 : 8;
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int KS = BN == 256 ? 1 : 2;  // blocks of the sum (128 bytes of each row) a stage: narrow tiles are bound by its hand-over
+  static constexpr int S = BN == 256 ? 5 : BN == 128 ? 3 : 4;
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = KS * (A_BYTES + B_BYTES);
   static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
   static constexpr int TURN = 8192;  // a warp's staging: four blocks of 32 rows of 64 bytes, or one of 32 x 32 floats to turn
   static constexpr int BYTES = S * STAGE + EPI_WARPS * TURN + 1024;
@@ -80,7 +81,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
     gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc,
                 const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap mr) {
   typedef GemmShape<BN> Z;
-  constexpr int S = Z::S, BK = F8 ? 128 : 64;  // 128 bytes of each row
+  constexpr int S = Z::S, KS = Z::KS, BK = F8 ? 128 : 64;  // 128 bytes of each row
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2], res_full[Z::EPI_WARPS][2];
   __shared__ uint32_t tmem_base;
@@ -102,7 +103,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
   tc::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-  const int kblocks = (p.K + BK - 1) / BK, units = p.tiles * p.splits;
+  const int kblocks = (p.K + BK * KS - 1) / (BK * KS), units = p.tiles * p.splits;
   auto run = [&](int unit, int &from, int &to) {  // a unit's blocks of the sum
     from = unit / p.tiles * p.kper;
     to = min(kblocks, from + p.kper);
@@ -129,25 +130,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
       int k0, k1;
       run(unit, k0, k1);
-      for (int k = k0 * BK; k < k1 * BK; k += BK) {
+      for (int k = k0 * BK * KS; k < k1 * BK * KS; k += BK * KS) {
         if (!__all_sync(0xffffffffu, tc::mbar_wait(empty0 + s * 8, phase))) {
           tu_tc_error = 730;
           ok = false;
           break;
         }
-        const uint32_t bar = bars + s * 8, a = stage0 + s * Z::STAGE, b = a + Z::A_BYTES;
+        const uint32_t bar = bars + s * 8, a = stage0 + s * Z::STAGE, b = a + KS * Z::A_BYTES;
         tc::mbar_expect_tx(one && rank == 0, full0 + s * 8, 2 * Z::STAGE);
-        if constexpr (AMN) {
-          tc::tma_load_2d_pair(one, a, &ma, bar, m0, k);
-          tc::tma_load_2d_pair(one, a + 8192, &ma, bar, m0 + 64, k);
-        } else {
-          tc::tma_load_2d_pair(one, a, &ma, bar, k, m0);
-        }
-        if constexpr (BMN) {
 #pragma unroll
-          for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(one, b + i * 8192, &mb, bar, n0 + i * 64, k);
-        } else {
-          tc::tma_load_2d_pair(one, b, &mb, bar, k, n0);
+        for (int h = 0; h < KS; ++h) {  // (a block behind the sum's end arrives as zeros)
+          const uint32_t ah = a + h * Z::A_BYTES, bh = b + h * Z::B_BYTES;
+          if constexpr (AMN) {
+            tc::tma_load_2d_pair(one, ah, &ma, bar, m0, k + h * BK);
+            tc::tma_load_2d_pair(one, ah + 8192, &ma, bar, m0 + 64, k + h * BK);
+          } else {
+            tc::tma_load_2d_pair(one, ah, &ma, bar, k + h * BK, m0);
+          }
+          if constexpr (BMN) {
+#pragma unroll
+            for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d_pair(one, bh + i * 8192, &mb, bar, n0 + i * 64, k + h * BK);
+          } else {
+            tc::tma_load_2d_pair(one, bh, &mb, bar, k + h * BK, n0);
+          }
         }
         if (++s == S) s = 0, phase ^= 1;
       }
@@ -160,7 +165,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       constexpr uint64_t A_STEP = AMN ? 128 : 2, B_STEP = BMN ? 128 : 2, STAGE_STEP = Z::STAGE / 16;
       const uint32_t at = tc::smem_u32(buf), full0 = tc::smem_u32(&full[0]), empty0 = tc::smem_u32(&empty[0]);
       const uint64_t a0 = AMN ? tc::desc_mnmajor(at, 0, 8192) : tc::desc_kmajor(at, 0, 0);
-      const uint64_t b0 = BMN ? tc::desc_mnmajor(at + Z::A_BYTES, 0, 8192) : tc::desc_kmajor(at + Z::A_BYTES, 0, 0);
+      const uint64_t b0 = BMN ? tc::desc_mnmajor(at + KS * Z::A_BYTES, 0, 8192) : tc::desc_kmajor(at + KS * Z::A_BYTES, 0, 0);
       const bool one = lane == 0;
       uint64_t ad = a0, bd = b0;
       int s = 0;
@@ -187,7 +192,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
           tc::umma_pair<F8>(one, d, ad, bd, idesc, add);
           add = 1;
 #pragma unroll
-          for (int k = 1; k < 4; ++k) tc::umma_pair<F8>(one, d, ad + k * A_STEP, bd + k * B_STEP, idesc, 1);
+          for (int k = 1; k < 4 * KS; ++k)
+            tc::umma_pair<F8>(one, d, ad + k % 4 * A_STEP + k / 4 * (Z::A_BYTES / 16), bd + k % 4 * B_STEP + k / 4 * (Z::B_BYTES / 16), idesc, 1);
           tc::umma_commit_pair(one, empty0 + s * 8);
           ad += STAGE_STEP, bd += STAGE_STEP;
           if (++s == S) s = 0, phase ^= 1, ad = a0, bd = b0;
@@ -660,26 +666,26 @@ int launch_gemm_bn(const GemmParams &p, const void *a, int a_pitch, const void *
 }
 
 // A product's tile width and the number of runs its sum is cut into, by an estimate of its time in us: 4.5 and the rounds of tiles over
-// the pairs of SMs times the blocks of a run at 0.37, 0.32 and 0.30 us (256, 128 and 64 columns; 4096 x 8192 x 4096: 195, 294 and 537
-// us; the loop over a block bounds the narrow ones).  A sum in runs adds the launch that joins them (5
-// us, and 4 for what a second launch costs its caller) and the partial matrices' way through L2.  Cutting pays where few tiles have a
-// long sum: 64 x 16384 x 256 87 us in one run, 16 in sixteen; 256 x 2048 x 2048 would gain 3 of 15 us on the device.
+// the pairs of SMs times the stages of a run at 0.37 us (256 columns, 128 bytes a stage), 0.52 and 0.455 us (128 and 64 columns, 256
+// bytes; 4096 x 4096 x 4096: 98, 121 and 210 us, 256 x 2048 x 2048: 16.2, 12.7 and 12.2).  A sum in runs adds the launch that joins
+// them (5 us, and 4 for what a second launch costs its caller) and the partial matrices' way through L2.  Cutting pays where few tiles
+// have a long sum: 64 x 16384 x 256 60 us in one run, 14.5 in sixteen; 256 x 2048 x 2048 would gain 0.7 of 12.2 us on the device.
 struct GemmPlan {
   int bn, splits, kper;
   size_t bytes;  // of partial sums
 };
 GemmPlan gemm_plan(int M, int N, int K, bool f8, bool bmn) {
   const long long rows = (M + 255) / 256, clusters = sm_count() / 2;
-  const int kb = (K + (f8 ? 127 : 63)) / (f8 ? 128 : 64);
-  GemmPlan best = {256, 1, kb, 0};
+  GemmPlan best = {};
   double least = 1e30;
   for (int bn : {256, 128, 64}) {
     if (bmn && bn == 64) continue;
+    const int per = (f8 ? 128 : 64) * (bn == 256 ? 1 : 2), kb = (K + per - 1) / per;  // stages of a sum
     const long long tiles = rows * ((N + bn - 1) / bn);
     for (int want = 1; want <= 64; want *= 2) {
-      if (want > 1 && (tiles * want > clusters || kb < 4 * want)) break;
+      if (want > 1 && (tiles * want > clusters || kb < 2 * want)) break;
       const int kper = (kb + want - 1) / want, splits = (kb + kper - 1) / kper;
-      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.37 : bn == 128 ? 0.32 : 0.30);
+      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.37 : bn == 128 ? 0.52 : 0.455);
       if (splits > 1) us += 9.0 + 8.0 * splits * M * N / 8.0e6;
       if (us < least) least = us, best = {bn, splits, kper, splits > 1 ? (size_t)splits * M * N * 4 : 0};
     }
