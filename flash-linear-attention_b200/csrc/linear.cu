@@ -67,11 +67,11 @@ struct GemmParams {
 };
 
 template <int BN> struct GemmShape {
-  static constexpr int KS = BN == 256 ? 1 : 2;  // blocks of the sum (128 bytes of each row) a stage: narrow tiles are bound by its hand-over
-  static constexpr int S = BN == 256 ? 5 : BN == 128 ? 3 : 4;
+  static constexpr int KS = 2;  // blocks of the sum (128 bytes of each row) a stage: one was bound by the stages' hand-over
+  static constexpr int S = BN == 64 ? 4 : 3;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, STAGE = KS * (A_BYTES + B_BYTES);
   static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
-  static constexpr int TURN = 8192;  // a warp's staging: four blocks of 32 rows of 64 bytes, or one of 32 x 32 floats to turn
+  static constexpr int TURN = BN == 256 ? 4096 : 8192;  // a warp's staging: blocks of 32 rows of 64 bytes, or one of 32 x 32 floats to turn
   static constexpr int BYTES = S * STAGE + EPI_WARPS * TURN + 1024;
 };
 
@@ -204,7 +204,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
     __syncwarp();
   } else if (TS && warp >= 4) {  // ---- epilogue: two warps a quarter of the rows, on blocks of 32 columns in turn
     const int w = warp - 4, quarter = w & 3, side = w >> 2;
-    uint8_t *const stage = buf + S * Z::STAGE + w * Z::TURN;  // y, y, z, z
+    // y and z in turn (y, y, z, z), or where there is room for two blocks only y in turn, or y and z
+    uint8_t *const stage = buf + S * Z::STAGE + w * Z::TURN;
+    constexpr bool ROOM = Z::TURN == 8192;
+    const bool two = ROOM || !EPI || !p.z;
     constexpr int BLOCKS = BN / 64;  // of this warp
     uint32_t seen = 0;  // parity of the residual blocks taken, a bit a buffer
     int n = 0;
@@ -214,8 +217,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       place(unit, tm, tn);
       const int m0 = tm * 256 + rank * 128 + quarter * 32, n0 = tn * BN + side * 32;
       auto ask = [&](int b) {  // lane 0: the residual of block b, into the buffer that its result will leave from
-        tc::mbar_expect_tx(&res_full[w][b & 1], 2048);
-        tc::tma_load_2d(stage + (b & 1) * 2048, &mr, &res_full[w][b & 1], n0 + b * 64, m0);
+        const int q = two ? b & 1 : 0;
+        tc::mbar_expect_tx(&res_full[w][q], 2048);
+        tc::tma_load_2d(stage + q * 2048, &mr, &res_full[w][q], n0 + b * 64, m0);
       };
       if (lane == 0) {
         tc::tma_store_wait_read();
@@ -233,10 +237,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
       bool ok = true;
 #pragma unroll 1
       for (int b = 0; b < BLOCKS; ++b) {
-        const int q = b & 1, c = n0 + b * 64;
+        const int q = two ? b & 1 : 0, c = n0 + b * 64;
         float v[32];
         tc::tmem_ld_32x32b_x32(from + b * 64, v);
-        if (EPI && p.res) {
+        if (!two) {
+          if (b > 0 && lane == 0) {
+            tc::tma_store_wait_read();  // of block b - 1
+            if (EPI && p.res) ask(b);
+          }
+        } else if (EPI && p.res) {
           if (b + 1 < BLOCKS && lane == 0) {
             tc::tma_store_wait_read();  // of block b - 1, a block's work ago
             ask(b + 1);
@@ -276,6 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += Num<TO>::f(bias[j >> 3].v[j & 7]);
         }
+        const int zq = ROOM ? 2 + q : 1;
         // rows of 64 bytes, 64-byte swizzle: 16-byte piece j of row r lies at j ^ (r / 2 % 4)
         auto piece = [&](int buffer, int j) { return reinterpret_cast<Eight *>(stage + buffer * 2048 + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)); };
         if (EPI && p.z) {
@@ -284,7 +294,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
             Eight o;
 #pragma unroll
             for (int i = 0; i < 8; ++i) o.v[i] = Num<TO>::t(v[8 * j + i]);
-            *piece(2 + q, j) = o;
+            *piece(zq, j) = o;
           }
         }
         if (EPI && p.act) {
@@ -331,7 +341,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         __syncwarp();
         if (lane == 0) {
           tc::tma_store_2d(&mc, stage + q * 2048, c, m0);
-          if (EPI && p.z) tc::tma_store_2d(&mz, stage + (2 + q) * 2048, c, m0);
+          if (EPI && p.z) tc::tma_store_2d(&mz, stage + zq * 2048, c, m0);
           tc::tma_store_commit();
         }
       }
@@ -666,8 +676,7 @@ int launch_gemm_bn(const GemmParams &p, const void *a, int a_pitch, const void *
 }
 
 // A product's tile width and the number of runs its sum is cut into, by an estimate of its time in us: 4.5 and the rounds of tiles over
-// the pairs of SMs times the stages of a run at 0.37 us (256 columns, 128 bytes a stage), 0.52 and 0.455 us (128 and 64 columns, 256
-// bytes; 4096 x 4096 x 4096: 98, 121 and 210 us, 256 x 2048 x 2048: 16.2, 12.7 and 12.2).  A sum in runs adds the launch that joins
+// the pairs of SMs times the stages of a run at 0.72, 0.52 and 0.455 us (256, 128 and 64 columns; 4096 x 4096 x 4096: 98, 121 and 210 us, 256 x 2048 x 2048: 16.2, 12.7 and 12.2).  A sum in runs adds the launch that joins
 // them (5 us, and 4 for what a second launch costs its caller) and the partial matrices' way through L2.  Cutting pays where few tiles
 // have a long sum: 64 x 16384 x 256 60 us in one run, 14.5 in sixteen; 256 x 2048 x 2048 would gain 0.7 of 12.2 us on the device.
 struct GemmPlan {
@@ -680,12 +689,12 @@ GemmPlan gemm_plan(int M, int N, int K, bool f8, bool bmn) {
   double least = 1e30;
   for (int bn : {256, 128, 64}) {
     if (bmn && bn == 64) continue;
-    const int per = (f8 ? 128 : 64) * (bn == 256 ? 1 : 2), kb = (K + per - 1) / per;  // stages of a sum
+    const int per = f8 ? 256 : 128, kb = (K + per - 1) / per;  // stages of a sum
     const long long tiles = rows * ((N + bn - 1) / bn);
     for (int want = 1; want <= 64; want *= 2) {
       if (want > 1 && (tiles * want > clusters || kb < 2 * want)) break;
       const int kper = (kb + want - 1) / want, splits = (kb + kper - 1) / kper;
-      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.37 : bn == 128 ? 0.52 : 0.455);
+      double us = 4.5 + (double)((tiles * splits + clusters - 1) / clusters) * kper * (bn == 256 ? 0.72 : bn == 128 ? 0.52 : 0.455);
       if (splits > 1) us += 9.0 + 8.0 * splits * M * N / 8.0e6;
       if (us < least) least = us, best = {bn, splits, kper, splits > 1 ? (size_t)splits * M * N * 4 : 0};
     }
