@@ -28,10 +28,17 @@ namespace {
 
 enum { ACT_NONE = 0, ACT_SILU = 1, ACT_SIGMOID = 2, ACT_LOGSIGMOID = 3, ACT_GELU = 4 };
 
+// 1 / (1 + e^-z) from the hardware's base-2 exponential and reciprocal (about 2^-22 of the value; e^-z beyond fp32 gives 0 as it should)
+__device__ __forceinline__ float sigmoid(float z) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return s;
+}
 __device__ __forceinline__ float act_fwd(float z, int act) {
   switch (act) {
-    case ACT_SILU: return __fdividef(z, 1.f + __expf(-z));
-    case ACT_SIGMOID: return __fdividef(1.f, 1.f + __expf(-z));
+    case ACT_SILU: return z * sigmoid(z);
+    case ACT_SIGMOID: return sigmoid(z);
     case ACT_LOGSIGMOID: return fminf(z, 0.f) - log1pf(__expf(-fabsf(z)));
     case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
     default: return z;
@@ -40,14 +47,14 @@ __device__ __forceinline__ float act_fwd(float z, int act) {
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case ACT_SILU: {
-      const float s = __fdividef(1.f, 1.f + __expf(-z));
-      return s * (1.f + z * (1.f - s));
+      const float s = sigmoid(z);
+      return fmaf(z, fmaf(-s, s, s), s);
     }
     case ACT_SIGMOID: {
-      const float s = __fdividef(1.f, 1.f + __expf(-z));
-      return s * (1.f - s);
+      const float s = sigmoid(z);
+      return fmaf(-s, s, s);
     }
-    case ACT_LOGSIGMOID: return __fdividef(1.f, 1.f + __expf(z));
+    case ACT_LOGSIGMOID: return sigmoid(-z);
     case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
     default: return 1.f;
   }
@@ -503,27 +510,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
 
 // ---- dz = dy act'(z), and the column sums of dz ---------------------------------------------------------------------------
 // A block takes 32 V columns x a run of rows; dz may have a row pitch of its own.  Partial column sums, one row a run.
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) act_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ z, T *__restrict__ dz, float *__restrict__ part, int M,
-                                                      int N, int pitch, int run, int act) {
+                                                      int N, int pitch, int run) {
   __shared__ float s[8][32 * V];
   struct alignas(V * sizeof(T)) Pack {
     T v[V];
   };
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (blockIdx.x * 32 + lane) * V;
   const int end = (int)min((long long)M, (blockIdx.y + 1ll) * run);
+  auto once = [](const T *at) {  // dy and z are not read again: evict-first loads (79 us without them at 32768 x 2048, 69 with)
+    Pack q;
+    if constexpr (V == 8) {
+      const int4 raw = __ldcs(reinterpret_cast<const int4 *>(at));
+      q = *reinterpret_cast<const Pack *>(&raw);
+    } else {
+      q = *reinterpret_cast<const Pack *>(at);
+    }
+    return q;
+  };
   float sum[V] = {};
   if (c < N) {
 #pragma unroll 4
     for (int r = blockIdx.y * run + w; r < end; r += 8) {
       const size_t at = (size_t)r * N + c;
-      const Pack d = *reinterpret_cast<const Pack *>(dy + at);
+      const Pack d = once(dy + at);
       Pack u, o;
-      if (z) u = *reinterpret_cast<const Pack *>(z + at);
+      if (ACT) u = once(z + at);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float f = Num<T>::f(d.v[j]);
-        if (z) f *= act_slope(Num<T>::f(u.v[j]), act);
+        if (ACT) f *= act_slope(Num<T>::f(u.v[j]), ACT);
         sum[j] += f;
         o.v[j] = Num<T>::t(f);
       }
@@ -543,20 +560,36 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T *__restrict__ dy, 
     }
 }
 
-// Rows of a partial column sum: 128, more where that would be more runs than a grid's second dimension holds.
-int run_of(int M) { return 128 * (int)((M + 128ll * 65535 - 1) / (128ll * 65535)); }
+// Rows of a block, and of a partial column sum: one wave of four blocks an SM over the column groups of `cols` (32768 x 2048: 592
+// blocks of 448 rows).
+int run_of(int M, int N, int cols) {
+  const long long groups = (N + cols - 1) / cols, most = groups < 4ll * sm_count() ? 4ll * sm_count() / groups : 1;
+  const long long run = ((M + most - 1) / most + 31) / 32 * 32;
+  return (int)run;
+}
 
 template <typename T>
-int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, int N, int pitch, int act, cudaStream_t st) {
-  const T *d = reinterpret_cast<const T *>(dy), *u = act ? reinterpret_cast<const T *>(z) : nullptr;
+int launch_act_bwd(const void *dy, const void *z, void *dz, float *part, int M, int N, int pitch, int act, int &parts, cudaStream_t st) {
+  const T *d = reinterpret_cast<const T *>(dy), *u = reinterpret_cast<const T *>(z);
   T *o = reinterpret_cast<T *>(dz);
-  const int run = run_of(M);
-  const unsigned runs = (M + run - 1) / run;
   bool wide = N % 8 == 0;
   for (const void *q : {(const void *)d, (const void *)u, (const void *)o}) wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
-  if (wide) act_bwd_kernel<T, 8><<<dim3((N + 255) / 256, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, run, act);
-  else act_bwd_kernel<T, 1><<<dim3((N + 31) / 32, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, run, act);
-  return check_launch("linear_bwd");
+  const int run = run_of(M, N, wide ? 256 : 32);
+  const unsigned runs = (unsigned)((M + (long long)run - 1) / run);
+  parts = (int)runs;
+  auto launch = [&](auto which) {
+    constexpr int ACT = decltype(which)::value;
+    if (wide) act_bwd_kernel<T, 8, ACT><<<dim3((N + 255) / 256, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, run);
+    else act_bwd_kernel<T, 1, ACT><<<dim3((N + 31) / 32, runs), 256, 0, st>>>(d, u, o, part, M, N, pitch, run);
+    return check_launch("linear_bwd");
+  };
+  switch (act) {
+    case ACT_SILU: return launch(std::integral_constant<int, ACT_SILU>());
+    case ACT_SIGMOID: return launch(std::integral_constant<int, ACT_SIGMOID>());
+    case ACT_LOGSIGMOID: return launch(std::integral_constant<int, ACT_LOGSIGMOID>());
+    case ACT_GELU: return launch(std::integral_constant<int, ACT_GELU>());
+    default: return launch(std::integral_constant<int, ACT_NONE>());
+  }
 }
 
 // Rows of n elements to rows of `pitch`, V elements at a time, for one or two matrices in a launch.
@@ -813,7 +846,16 @@ int flab_linear_fwd(const void *x, const void *weight, const void *bias, const v
                             : launch_gemm<__half, false, 0, false, false, true>(p, o.x, kp, o.w, kp, dtype, scratch, scratch_bytes, st);
 }
 
-int flab_linear_bwd_partials(int M) { return M <= 0 ? 1 : (int)((M + (long long)flab::run_of(M) - 1) / flab::run_of(M)); }
+int flab_linear_bwd_partials(int M, int N) {
+  if (M <= 0 || N <= 0) return 1;
+  long long most = 1;
+  for (int cols : {256, 32}) {
+    const int run = flab::run_of(M, N, cols);
+    const long long runs = (M + (long long)run - 1) / run;
+    most = runs > most ? runs : most;
+  }
+  return (int)most;
+}
 
 int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *dy, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
                     int K, int act, int dtype, void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream) {
@@ -841,10 +883,11 @@ int flab_linear_bwd(const void *x, const void *weight, const void *z, const void
       dz = out = scratch;
       part += dz_bytes, part_bytes -= dz_bytes;
     }
-    rc = dtype == FLAB_BF16 ? launch_act_bwd<bf16>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st)
-                            : launch_act_bwd<__half>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, st);
+    int parts = 0;
+    rc = dtype == FLAB_BF16 ? launch_act_bwd<bf16>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, parts, st)
+                            : launch_act_bwd<__half>(dy, z, out, dbias ? db_partial : nullptr, M, N, zp, act, parts, st);
     if (rc) return rc;
-    if (dbias && (rc = sum_partials(db_partial, dbias, flab_linear_bwd_partials(M), N, dtype, st))) return rc;
+    if (dbias && (rc = sum_partials(db_partial, dbias, parts, N, dtype, st))) return rc;
   }
   GemmParams p = {};
   if (dx) {

@@ -126,7 +126,7 @@ def load() -> ctypes.CDLL:
     lib.flab_linear_fwd.restype = ci
     lib.flab_linear_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp, sz, vp]
     lib.flab_linear_bwd_partials.restype = ci
-    lib.flab_linear_bwd_partials.argtypes = [ci]
+    lib.flab_linear_bwd_partials.argtypes = [ci, ci]
     lib.flab_linear_bwd.restype = ci
     lib.flab_linear_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, sz, vp, sz, vp]
     lib.flab_linear_e4m3.restype = ci

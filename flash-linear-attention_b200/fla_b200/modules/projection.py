@@ -68,7 +68,7 @@ def _backward(ctx, dy):
                 t.zero_()
     elif need_x or need_w or need_b:
         lib = _lib.load()
-        part = torch.empty(lib.flab_linear_bwd_partials(M), N, dtype=torch.float32, device=dev) if need_b else None
+        part = torch.empty(lib.flab_linear_bwd_partials(M, N), N, dtype=torch.float32, device=dev) if need_b else None
         # (an operand that was copied, or whose product is not wanted, is not kept: its address only says how the copies lie)
         x_at, w_at = ctx.places
         with _lib.device_of(d2):

@@ -148,7 +148,7 @@ int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const v
  *   z = x weight^T + bias;  y = act(z) + residual;   dz = d_y act'(z);  dx = dz weight;  dweight = dz^T x;  dbias = sum of dz over rows
  * x, dx: [M, K]; weight, dweight: [N, K]; bias, dbias: [N]; y, z, residual, d_y: [M, N]; contiguous, of type dtype (bf16 or fp16).
  * act: 0 none, 1 silu, 2 sigmoid, 3 log sigmoid, 4 gelu (erf). bias, residual may be NULL; z (NULL: not wanted) is what backward
- * needs with an activation. Each of dx, dweight, dbias may be NULL; db_partial: fp32 [flab_linear_bwd_partials(M), N], summed in a
+ * needs with an activation. Each of dx, dweight, dbias may be NULL; db_partial: fp32 [flab_linear_bwd_partials(M, N), N], summed in a
  * fixed order. ws: 256-byte aligned scratch of flab_linear_workspace() bytes, for copies of operands whose rows do not begin on
  * 16-byte boundaries: forward fills it, and backward is given what forward filled, with the same x and weight (whose own bytes it
  * reads only where they were not copied, x for dweight and weight for dx). scratch: 256-byte aligned, of flab_linear_scratch() or
@@ -161,7 +161,7 @@ size_t flab_linear_scratch(int M, int N, int K, int dtype);
 size_t flab_linear_bwd_scratch(const void *d_y, int M, int N, int K, int act);
 int flab_linear_fwd(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *z, int M, int N, int K, int act, int dtype,
                     void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream);
-int flab_linear_bwd_partials(int M);
+int flab_linear_bwd_partials(int M, int N);
 int flab_linear_bwd(const void *x, const void *weight, const void *z, const void *d_y, void *dx, void *dweight, void *dbias, float *db_partial, int M, int N,
                     int K, int act, int dtype, void *ws, size_t ws_bytes, void *scratch, size_t scratch_bytes, void *stream);
 int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, const float *w_scale, const void *bias, const void *residual, void *y, int M,
