@@ -61,9 +61,9 @@ def _backward(ctx, dy, dsum=None):
     if rows and n:
         lib = _lib.load()
         part = None
-        if dw is not None:
-            part = torch.empty(lib.flab_rms_norm_partials(rows, n, _DTYPES[ctx.x_dtype]), n, dtype=torch.float32, device=dev)
         with _lib.device_of(total):
+            if dw is not None:
+                part = torch.empty(lib.flab_rms_norm_partials(rows, n, _DTYPES[ctx.x_dtype]), n, dtype=torch.float32, device=dev)
             rc = lib.flab_rms_norm_bwd(total.data_ptr(), dy.data_ptr(), _p(dsum), _p(w), rstd.data_ptr(), _p(dx), _p(dr), _p(dw), _p(part),
                                        rows, n, _DTYPES[ctx.x_dtype], _DTYPES[total.dtype],
                                        _DTYPES[torch.float32 if w is None else w.dtype], _lib.stream_of(total))

@@ -68,12 +68,12 @@ def _backward(ctx, dy):
                 t.zero_()
     elif need_x or need_w or need_b:
         lib = _lib.load()
-        part = torch.empty(lib.flab_linear_bwd_partials(M, N), N, dtype=torch.float32, device=dev) if need_b else None
         # (an operand that was copied, or whose product is not wanted, is not kept: its address only says how the copies lie)
         x_at, w_at = ctx.places
         with _lib.device_of(d2):
             n = lib.flab_linear_bwd_scratch(d2.data_ptr(), M, N, K, ctx.act) if need_x or need_w else 0
             scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+            part = torch.empty(lib.flab_linear_bwd_partials(M, N), N, dtype=torch.float32, device=dev) if need_b else None
             rc = lib.flab_linear_bwd(x_at, w_at, _p(z), d2.data_ptr(), _p(dx), _p(dw), _p(db), _p(part), M, N, K, ctx.act, _DTYPES[dy.dtype],
                                      _p(copies), 0 if copies is None else copies.numel(), _p(scratch), n, _lib.stream_of(d2))
         _lib.finish("flab_linear_bwd", rc)

@@ -269,6 +269,16 @@ def test_only_some_gradients_and_no_rows():
         assert linear_fp8(q, torch.zeros(0, device=DEV), torch.zeros(24, 48, device=DEV).to(q.dtype), torch.ones(24, device=DEV)).shape == (0, 24)
 
 
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x, w = (torch.randn(n, 32, device=DEV, dtype=BF, requires_grad=True) for n in (6, 8))
+    v, one = torch.randn(2, 9, 32, device=DEV, requires_grad=True), torch.ones(32, device=DEV, requires_grad=True)
+    for out, leaf in ((linear(x, w, activation="silu"), x), (rms_norm(v, one), v), (chunk_hgrn(v, v)[0], v)):
+        (g,) = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.autograd.grad(g.sum(), leaf)
+
+
 def test_refusals():
     x, w = torch.zeros(4, 16, dtype=BF), torch.zeros(8, 16, dtype=BF)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
