@@ -274,8 +274,11 @@ def test_second_derivatives_are_refused():
     x, w = (torch.randn(n, 32, device=DEV, dtype=BF, requires_grad=True) for n in (6, 8))
     v, one = torch.randn(2, 9, 32, device=DEV, requires_grad=True), torch.ones(32, device=DEV, requires_grad=True)
     for out, leaf in ((linear(x, w, activation="silu"), x), (rms_norm(v, one), v), (chunk_hgrn(v, v)[0], v)):
-        (g,) = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)
+        dy = torch.ones_like(out).requires_grad_(True)
+        (g,) = torch.autograd.grad(out, leaf, dy, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.autograd.grad(g.sum(), dy, retain_graph=True)
+        with pytest.raises(RuntimeError):  # never a silent zero
             torch.autograd.grad(g.sum(), leaf)
 
 
