@@ -334,6 +334,29 @@ def test_no_tokens():
         assert dx.shape == shape and dh0.shape == h0.shape
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [2048, 2047])
+def test_offsets_beyond_32_bits(D):
+    """More than 2^31 elements (aligned rows, and rows that TMA cannot address): the ends against calls on the ends alone."""
+    T, tail = 2 ** 31 // D + 5000, 3000
+    x = torch.empty(1, T, D, dtype=torch.bfloat16, device=DEV).normal_()
+    g = torch.empty_like(x).uniform_(-2, -0.1)
+    off = torch.tensor([0, T - tail - 10, T], device=DEV)
+    xs, gs = x.requires_grad_(True), g.requires_grad_(True)
+    o, ht = chunk_hgrn(xs, gs, output_final_state=True, offsets=off)
+    dx, dg = torch.autograd.grad(o, [xs, gs], x.detach())
+    part = [v.detach()[:, -tail - 10:].clone().requires_grad_(True) for v in (x, g)]
+    o2, h2 = chunk_hgrn(*part, output_final_state=True)
+    dx2, dg2 = torch.autograd.grad(o2, part, part[0].detach())
+    # the same rows in tiles that begin elsewhere: fp32 sums in another order, one rounding each
+    near("o", o[0, -tail - 10:], o2[0].cpu(), torch.bfloat16, halves=2.1)
+    near("ht", ht[1], h2[0].cpu(), torch.float32)
+    near("dx", dx[0, -tail - 10:], dx2[0].cpu(), torch.bfloat16, halves=2.1)
+    near("dg", dg[0, -tail - 10:], dg2[0].cpu(), torch.bfloat16, halves=4.2)
+    head, _ = chunk_hgrn(x.detach()[:, :500], g.detach()[:, :500])
+    near("head", o[0, :500], head[0].cpu(), torch.bfloat16, halves=2.1)
+
+
 def test_refusals():
     x = torch.zeros(2, 4, 8)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):

@@ -129,6 +129,23 @@ def test_tiles_in_turn_and_large_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [2048, 2047])
+def test_offsets_beyond_32_bits(N):
+    M, K = 2 ** 31 // N + 900, 16
+    x, w, b, _, _ = make(1000, K, N, BF, 4, residual=False)
+    x, w, b = x.to(DEV).repeat(M // 1000 + 1, 1)[:M].contiguous(), w.to(DEV), b.to(DEV)
+    xs = x.requires_grad_(True)
+    y = linear(xs, w, bias=b, activation="silu")
+    for rows in (slice(0, 300), slice(M - 300, M)):
+        assert torch.equal(y.detach()[rows], linear(x.detach()[rows], w, bias=b, activation="silu"))
+    (dx,) = torch.autograd.grad(y, xs, y.detach())
+    small = x.detach()[-300:].clone().requires_grad_(True)
+    (dx2,) = torch.autograd.grad(linear(small, w, bias=b, activation="silu"), small, y.detach()[-300:])
+    # the small call may cut its sums into runs: fp32 in another order, one rounding each
+    assert ((dx[-300:].double() - dx2.double()).abs() <= 2 * half(dx2.double(), BF) + 2.0 ** -12).all()
+
+
+@pytest.mark.gpu
 def test_shapes_views_streams_and_graph():
     gen = torch.Generator().manual_seed(2)
     x = torch.randn(3, 5, 80, generator=gen).to(DEV).to(BF)

@@ -228,6 +228,30 @@ def test_only_some_gradients_and_no_rows():
         assert q.shape == shape and scale.shape == shape[:-1]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2048, 2047])
+def test_offsets_beyond_32_bits(n):
+    rows = 2 ** 31 // n + 700
+    x = torch.empty(rows, n, dtype=BF, device=DEV).normal_()
+    w = torch.ones(n, device=DEV, dtype=BF)
+    xs = x.requires_grad_(True)
+    y = rms_norm(xs, w)
+    (dx,) = torch.autograd.grad(y, xs, x.detach())
+    small = x.detach()[-300:].clone().requires_grad_(True)
+    y2 = rms_norm(small, w)
+    (dx2,) = torch.autograd.grad(y2, small, small.detach())
+    y64, rstd = forward64(small.detach().cpu(), w.cpu(), 1e-6)
+    within("y", y[-300:], y64, 96 * U * y64.abs() + half_step(y64, BF))
+    D, xhat = small.detach().double().cpu(), small.detach().double().cpu() * rstd
+    inner = (xhat * D).mean(1, keepdim=True)
+    d64 = rstd * (D - xhat * inner)
+    size = rstd * (D.abs() + xhat.abs() * (xhat * D).abs().mean(1, keepdim=True))
+    for d in (dx[-300:], dx2):
+        within("dx", d, d64, 96 * U * size + half_step(d64, BF))
+    q, scale = quantize_rows(x.detach())
+    held(q[-300:], scale[-300:], small.detach().double().cpu())
+
+
 def test_refusals():
     x, w = torch.zeros(2, 8), torch.ones(8)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
