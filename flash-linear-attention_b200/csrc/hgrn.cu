@@ -369,6 +369,18 @@ template <int L> __device__ __forceinline__ void tile_codes(const HgrnParams &p,
   }
 }
 
+// maps of two channels, one after the other (`a` first)
+struct Map2 {
+  float2 P, Q;
+};
+__device__ __forceinline__ float2 through(const Map2 &m, float2 c) { return make_float2(through(m.P.x, m.Q.x, c.x), through(m.P.y, m.Q.y, c.y)); }
+__device__ __forceinline__ Map2 join(const Map2 &a, const Map2 &b) {
+  Map2 m;
+  m.Q = through(b, a.Q);
+  m.P = make_float2(is_cut(b.P.x) ? CUT : a.P.x * b.P.x, is_cut(b.P.y) ? CUT : a.P.y * b.P.y);
+  return m;
+}
+
 template <typename T, int R, int S, bool BWD> struct Stream {
   static constexpr int V = 2, C = 32 * V, W = 8, L = W * R;
   static constexpr int TILE = L * C, TENSORS = BWD ? 3 : 2;
@@ -378,7 +390,8 @@ template <typename T, int R, int S, bool BWD> struct Stream {
   static constexpr int THREADS = 32 * (2 * W + CHAINS + 2);
   struct Stage {
     T buf[TENSORS][TILE];   // x (do), g, o of a token earlier
-    float2 P[W][32], Q[W][32];  // the warps' maps; the start values take the place of P
+    float2 P[W][32], Q[W][32];  // the warps' maps, then the maps of all rows before theirs
+    float2 start[32];           // the tile's start value
     int code[L];
   };
   struct Shared {
@@ -489,7 +502,8 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       const bool on = ch < p.D;
       T *const xs = st.buf[0] + lane * 2, *const gs = st.buf[1] + lane * 2;
       const T *const os = st.buf[BWD ? 2 : 0] + lane * 2;
-      float2 c = st.P[w][lane];
+      float2 c = st.start[lane];
+      if (w > 0) c = make_float2(through(st.P[w][lane].x, st.Q[w][lane].x, c.x), through(st.P[w][lane].y, st.Q[w][lane].y, c.y));
       auto take = [&](int at, float2 g, float2 x, float2 h) {
         const float2 a = make_float2(gate(g.x), gate(g.y));
         if (!BWD) {
@@ -563,53 +577,79 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       typename Z::Stage &st = sh.st[s];
       const typename Z::Shared::Place z = sh.at[s];
       const int ch = z.cg * C + lane * 2;
-      float2 jP = make_float2(1.f, 1.f), jQ = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float2 P = st.P[i][lane], Q = st.Q[i][lane];
-        jQ.x = through(P.x, Q.x, jQ.x), jQ.y = through(P.y, Q.y, jQ.y);
-        jP.x = is_cut(P.x) ? CUT : jP.x * P.x, jP.y = is_cut(P.y) ? CUT : jP.y * P.y;
-      }
       const int group = z.step / G, first = group * G, before = z.step - first;
       const bool leader = before == G - 1 && z.step + 1 < p.nT;  // hands the group's end on
       auto words = [&](unsigned long long *base, int step) { return base + ((size_t)step * chains + z.chain) * C + lane * 2; };
+      auto rows_map = [&](int i) {
+        Map2 m;
+        m.P = st.P[i][lane], m.Q = st.Q[i][lane];
+        return m;
+      };
+      // the tile's map, by halves: what other tiles wait for goes out first
+      const Map2 tile = join(join(join(rows_map(0), rows_map(1)), join(rows_map(2), rows_map(3))),
+                             join(join(rows_map(4), rows_map(5)), join(rows_map(6), rows_map(7))));
       if (before < G - 1 && z.step + 1 < p.nT) {
-        put(words(p.maps, z.step), map_word(jP.x, jQ.x));
-        put(words(p.maps, z.step) + 1, map_word(jP.y, jQ.y));
+        put(words(p.maps, z.step), map_word(tile.P.x, tile.Q.x));
+        put(words(p.maps, z.step) + 1, map_word(tile.P.y, tile.Q.y));
       }
-      // everything that comes before is asked for at once
-      unsigned long long m[G - 1][2], e[2];
+      // everything that comes before is asked for at once, again and again until all of it is there
+      unsigned long long g[G - 1][2], e[2] = {0, 0};
+      const unsigned long long *const maps = words(p.maps, first), *const ends = words(p.ends, group > 0 ? group - 1 : 0);
+      const size_t by = (size_t)chains * C;
 #pragma unroll
       for (int i = 0; i < G - 1; ++i)
-        if (i < before) m[i][0] = look(words(p.maps, first + i)), m[i][1] = look(words(p.maps, first + i) + 1);
-      float2 c = make_float2(0.f, 0.f);
-      if (group > 0) e[0] = look(words(p.ends, group - 1)), e[1] = look(words(p.ends, group - 1) + 1);
-      else if (!VAR && edge && ch < p.D) c = *reinterpret_cast<const float2 *>(edge + (size_t)z.b * p.D + ch);
-      // the group's earlier tiles as one map, so that little is left to do once the end of the group before is there: that end to
-      // the next one is what is serial along time
-      float2 gP = make_float2(1.f, 1.f), gQ = make_float2(0.f, 0.f);
+        if (i < before) g[i][0] = look(maps + i * by), g[i][1] = look(maps + i * by + 1);
+      if (group > 0) e[0] = look(ends), e[1] = look(ends + 1);
+      {  // meanwhile, the way from the tile's start to each warp's rows takes the place of the rows' own map
+        Map2 to = rows_map(0);
 #pragma unroll
-      for (int i = 0; i < G - 1; ++i)
-        if (i < before) {
-          const float2 mx = map_of(await(words(p.maps, first + i), m[i][0])), my = map_of(await(words(p.maps, first + i) + 1, m[i][1]));
-          gQ.x = through(mx.x, mx.y, gQ.x), gQ.y = through(my.x, my.y, gQ.y);
-          gP.x = is_cut(mx.x) ? CUT : gP.x * mx.x, gP.y = is_cut(my.x) ? CUT : gP.y * my.x;
+        for (int i = 1; i < W; ++i) {
+          const Map2 own = rows_map(i);
+          st.P[i][lane] = to.P, st.Q[i][lane] = to.Q;
+          if (i + 1 < W) to = join(to, own);
         }
-      if (group > 0) {
-        c.x = end_of(await(words(p.ends, group - 1), e[0]));
-        c.y = end_of(await(words(p.ends, group - 1) + 1, e[1]));
       }
-      c.x = through(gP.x, gQ.x, c.x), c.y = through(gP.y, gQ.y, c.y);
-      if (leader) {
-        put(words(p.ends, group), end_word(through(jP.x, jQ.x, c.x)));
-        put(words(p.ends, group) + 1, end_word(through(jP.y, jQ.y, c.y)));
-      }
+      const long long asked = clock64();
+      for (int spins = 1;; ++spins) {
+        bool missing = group > 0 && !((e[0] >> 32) && (e[1] >> 32));
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float2 P = st.P[i][lane], Q = st.Q[i][lane];
-        st.P[i][lane] = c;
-        c.x = through(P.x, Q.x, c.x), c.y = through(P.y, Q.y, c.y);
+        for (int i = 0; i < G - 1; ++i) missing = missing || (i < before && !((g[i][0] >> 32) && (g[i][1] >> 32)));
+        if (!__any_sync(0xffffffffu, missing)) break;
+        // the wait has a bound like every other: about a second, and none once any has run out
+        if ((spins & 255) == 0 && __any_sync(0xffffffffu, clock64() - asked > (1ll << 31) || *reinterpret_cast<volatile int *>(&tu_tc_error))) {
+          tu_tc_error = 700;
+          break;
+        }
+#pragma unroll
+        for (int i = 0; i < G - 1; ++i)
+          if (i < before) {
+            if (!(g[i][0] >> 32)) g[i][0] = look(maps + i * by);
+            if (!(g[i][1] >> 32)) g[i][1] = look(maps + i * by + 1);
+          }
+        if (group > 0) {
+          if (!(e[0] >> 32)) e[0] = look(ends);
+          if (!(e[1] >> 32)) e[1] = look(ends + 1);
+        }
       }
+      // the group's earlier tiles as one map, then its start
+      auto tile_map = [&](int i) {
+        const float2 x = map_of(g[i][0]), y = map_of(g[i][1]);
+        Map2 m;
+        m.P = i < before ? make_float2(x.x, y.x) : make_float2(1.f, 1.f);
+        m.Q = i < before ? make_float2(x.y, y.y) : make_float2(0.f, 0.f);
+        return m;
+      };
+      const Map2 group_map = join(join(join(tile_map(0), tile_map(1)), join(tile_map(2), tile_map(3))), join(join(tile_map(4), tile_map(5)), tile_map(6)));
+      float2 c = make_float2(0.f, 0.f);
+      if (group > 0) c = make_float2(end_of(e[0]), end_of(e[1]));
+      else if (!VAR && edge && ch < p.D) c = *reinterpret_cast<const float2 *>(edge + (size_t)z.b * p.D + ch);
+      c = through(group_map, c);
+      if (leader) {
+        const float2 end = through(tile, c);
+        put(words(p.ends, group), end_word(end.x));
+        put(words(p.ends, group) + 1, end_word(end.y));
+      }
+      st.start[lane] = c;
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sh.ready[s]);
     }
