@@ -592,7 +592,8 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         put(words(p.maps, z.step), map_word(tile.P.x, tile.Q.x));
         put(words(p.maps, z.step) + 1, map_word(tile.P.y, tile.Q.y));
       }
-      // everything that comes before is asked for at once, again and again until all of it is there
+      // everything that comes before is asked for at once; the earlier tiles of the group again and again until all of them are there,
+      // and then the end of the group before, which is last to come where tiles wait at all
       unsigned long long g[G - 1][2], e[2] = {0, 0};
       const unsigned long long *const maps = words(p.maps, first), *const ends = words(p.ends, group > 0 ? group - 1 : 0);
       const size_t by = (size_t)chains * C;
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       }
       const long long asked = clock64();
       for (int spins = 1;; ++spins) {
-        bool missing = group > 0 && !((e[0] >> 32) && (e[1] >> 32));
+        bool missing = false;
 #pragma unroll
         for (int i = 0; i < G - 1; ++i) missing = missing || (i < before && !((g[i][0] >> 32) && (g[i][1] >> 32)));
         if (!__any_sync(0xffffffffu, missing)) break;
@@ -641,7 +642,9 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       };
       const Map2 group_map = join(join(join(tile_map(0), tile_map(1)), join(tile_map(2), tile_map(3))), join(join(tile_map(4), tile_map(5)), tile_map(6)));
       float2 c = make_float2(0.f, 0.f);
-      if (group > 0) c = make_float2(end_of(e[0]), end_of(e[1]));
+      if (group > 0) {
+        c = make_float2(end_of(await(ends, e[0])), end_of(await(ends + 1, e[1])));
+      }
       else if (!VAR && edge && ch < p.D) c = *reinterpret_cast<const float2 *>(edge + (size_t)z.b * p.D + ch);
       c = through(group_map, c);
       if (leader) {
