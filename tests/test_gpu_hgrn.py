@@ -82,7 +82,7 @@ def check(x, g, do, h0, dht, lengths, dtype, shape, offsets, fn=chunk_hgrn, fina
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("B,T,D,state", [(1, 1, 1, True), (2, 1, 64, True), (3, 2, 33, False), (1, 7, 2, True), (2, 127, 66, True), (1, 128, 64, False),
                                          (2, 129, 31, True), (1, 700, 130, True), (1, 1500, 8, False), (5, 260, 96, True), (2, 9, 24, True),
-                                         (2, 1300, 72, True), (3, 1024, 136, False), (1, 129, 8, True),
+                                         (2, 1300, 72, True), (3, 1024, 136, False), (1, 129, 8, True), (1, 8300, 72, True), (2, 8192, 8, False),
                                          (2, 15, 77, True), (3, 32, 34, True), (2, 33, 64, True), (1, 32, 16, False), (160, 40, 512, True)])
 def test_fixed_length(B, T, D, state, dtype):
     x, g, do, h0, dht = inputs(B * T, D, B, dtype, B * T + D, state)
