@@ -31,11 +31,10 @@ def _like(t: torch.Tensor, shape) -> torch.Tensor:
 def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=True):
     """x2, r2 `[rows, n]` contiguous. Returns (y, scale, sum, rstd), None for what was not asked for."""
     rows, n = x2.shape
-    dev = x2.device
-    y = torch.empty(rows, n, dtype=torch.float8_e4m3fn if quant else x2.dtype, device=dev)
-    total = torch.empty(rows, n, dtype=sum_dtype, device=dev) if want_sum else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if want_rstd else None
-    scale = torch.empty(rows, dtype=torch.float32, device=dev) if quant else None
+    y = torch.empty_like(x2, dtype=torch.float8_e4m3fn) if quant else torch.empty_like(x2)  # (empty() from sizes takes 1 us longer)
+    total = torch.empty_like(x2, dtype=sum_dtype) if want_sum else None
+    rstd = x2.new_empty(rows, dtype=torch.float32) if want_rstd else None
+    scale = x2.new_empty(rows, dtype=torch.float32) if quant else None
     if rows and n:
         lib = _lib.load()
         with _lib.device_of(x2):
@@ -50,20 +49,19 @@ def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=T
 def _backward(ctx, dy, dsum=None):
     total, rstd, w = ctx.saved_tensors
     rows, n = total.shape
-    dev = total.device
     need_x, need_w, need_r = ctx.needs_input_grad[:3]
-    dy = torch.zeros(rows, n, dtype=ctx.x_dtype, device=dev) if dy is None else _rows(dy.to(ctx.x_dtype))
-    dsum = None if dsum is None else _rows(dsum.to(total.dtype))
+    dy = torch.zeros_like(total, dtype=ctx.x_dtype) if dy is None else _rows(dy if dy.dtype == ctx.x_dtype else dy.to(ctx.x_dtype))
+    dsum = None if dsum is None else _rows(dsum if dsum.dtype == total.dtype else dsum.to(total.dtype))
     wide = need_r and ctx.r_dtype != ctx.x_dtype  # the residual's gradient has a type of its own (the sum's)
-    dx = torch.empty(rows, n, dtype=ctx.x_dtype, device=dev) if need_x or (need_r and not wide) else None
-    dr = torch.empty(rows, n, dtype=total.dtype, device=dev) if wide else None
+    dx = torch.empty_like(dy) if need_x or (need_r and not wide) else None
+    dr = torch.empty_like(total) if wide else None
     dw = torch.empty_like(w) if w is not None and need_w else None
     if rows and n:
         lib = _lib.load()
         part = None
         with _lib.device_of(total):
             if dw is not None:
-                part = torch.empty(lib.flab_rms_norm_partials(rows, n, _DTYPES[ctx.x_dtype]), n, dtype=torch.float32, device=dev)
+                part = rstd.new_empty((lib.flab_rms_norm_partials(rows, n, _DTYPES[ctx.x_dtype]), n))
             rc = lib.flab_rms_norm_bwd(total.data_ptr(), dy.data_ptr(), _p(dsum), _p(w), rstd.data_ptr(), _p(dx), _p(dr), _p(dw), _p(part),
                                        rows, n, _DTYPES[ctx.x_dtype], _DTYPES[total.dtype],
                                        _DTYPES[torch.float32 if w is None else w.dtype], _lib.stream_of(total))
