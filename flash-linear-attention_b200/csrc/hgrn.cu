@@ -12,15 +12,15 @@
 // of each group of G publishes the group's end value, and a tile takes the end of the group before its own through the maps of
 // its group's earlier tiles.  The sums are formed in the same order whatever block runs when, so results repeat bit for bit (taking
 // whichever of a predecessor's map and end value is there first does not repeat).  Groups of 4 and of 16 were slower (forward at
-// [1, 262144, 1024] 480 and 575 us against 344: more hops, and more maps to fetch).  Serial along time is one hop a group: a word
+// [1, 262144, 1024] 480 and 575 us where groups of 8 took 344: more hops, and more maps to fetch).  Serial along time is one hop a group: a word
 // of 64 bits that holds value and mark.  Tiles are handed out by a ticket in the order of time, so that a tile waits only for
 // tiles whose blocks already run; one launch then reads everything once, where a two-pass scan would read the inputs twice.
 // Three forms: rows that TMA can address stream through a persistent block (hgrn_stream_kernel), others go tile by tile through
 // registers (hgrn_tile_kernel), and a few tokens a sequence are walked by one thread a channel group (hgrn_step_kernel).
 // Measured against the bytes above at the copy rate of 6.55 TB/s, bf16: [8, 4096, 2048] forward 68 us (91 %), backward 107 us (96 %);
-// [1, 262144, 2048] forward 601 us (82 %), backward 944 us (87 %): 32 channel groups side by side, where a tile's wait for the loads
-// of all tiles before it is what the six (four) stages no longer cover; 64 packed sequences of 290000 tokens 723 and 1069 us; one
-// token of 256 x 2048 2.5 us.
+// [1, 262144, 2048] forward 548 us (90 %), backward 872 us (94 %): 32 channel groups side by side, where a tile's wait for the maps
+// of the tiles before it is what the stages no longer cover whole ([1, 262144, 1024] 310 and 480 us, 79 and 85 %); 64 packed
+// sequences of 290000 tokens 660 and 987 us (82 and 92 %); one token of 256 x 2048 2.5 us.
 // All arithmetic and every state is fp32; o, dx, dg are rounded once, when stored.  Backward takes h_{t-1} from the stored o:
 // dg is a plain product with it, so the 16-bit rounding of o enters dg once, with the size of dg's own rounding, and backward
 // needs neither x nor a second forward scan.

@@ -13,10 +13,10 @@
 // residual comes in the same way, a block ahead.  Outputs whose rows do not begin on 16-byte boundaries go through a transposition in
 // shared memory instead, so that a warp reads and writes runs of 64 bytes.  Tiles go in groups of 8 rows of tiles, so that what the
 // pairs work on at one time shares operands in L2.
-// Measured, bf16, 32768 x 2048 x 2048: product alone 192 us (1430 TFLOP/s; the library's 183), with silu, bias and residual 215 us, dx
-// 188, dW 195 us; 8192 x 8192 x 8192 721 us (1525 TFLOP/s; the library's 670).  e4m3, 32768 x 2048 x 2048 with scales 113 us (2430
-// TFLOP/s), with silu 126 us.  Bound by the tensor pipe under the power cap (77 to 82 % active without an epilogue, 68 % with
-// one); 256 x 2048 x 2048 takes 15 us, the loop over 32 blocks.
+// Measured, bf16, 32768 x 2048 x 2048: product alone 184 us (1490 TFLOP/s; the library's 180), with silu, bias and residual 194 us, dx
+// 183, dW 186 us; 8192 x 8192 x 8192 706 us (1558 TFLOP/s; the library's 663).  e4m3, 32768 x 2048 x 2048 with scales 105 us (2620
+// TFLOP/s), with silu 121 us.  Bound by the tensor pipe under the power cap (77 to 82 % active without an epilogue, 68 % with
+// one); 256 x 2048 x 2048 takes 12.2 us, the loop over 32 blocks.
 #include <type_traits>
 
 #include "tc.cuh"
