@@ -68,8 +68,9 @@ def _backward(ctx, dy):
                 t.zero_()
     elif need_x or need_w or need_b:
         lib = _lib.load()
-        # (an operand that was copied, or whose product is not wanted, is not kept: its address only says how the copies lie)
-        x_at, w_at = ctx.places
+        # Kept operands are read where they are now (a checkpoint or a hook may have brought them back elsewhere). One that was copied, or
+        # whose product is not wanted, is not kept: its address in forward only says how the copies lie.
+        x_at, w_at = (at if t is None else t.data_ptr() for t, at in zip((x2, w), ctx.places))
         with _lib.device_of(d2):
             n = lib.flab_linear_bwd_scratch(d2.data_ptr(), M, N, K, ctx.act) if need_x or need_w else 0
             scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None

@@ -7,6 +7,7 @@ through the next product with the sizes of its other operand."""
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 from fla_b200 import _lib
 from fla_b200.modules import linear, linear_fp8, quantize_rows, rms_norm, rms_norm_quant
@@ -297,6 +298,34 @@ def test_second_derivatives_are_refused():
             torch.autograd.grad(g.sum(), leaf, retain_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(300, 128, 96), (130, 77, 51)])
+@pytest.mark.parametrize("bias", [True, False])
+def test_operands_that_come_back_elsewhere(M, K, N, bias):
+    """A checkpoint works its inputs out again and a hook may keep them on the host: backward reads them where they are then."""
+    x, w, b, r, dy = (v if v is None else v.to(DEV) for v in make(M, K, N, BF, 21, bias=bias))
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r) if t is not None]
+
+    def step(x, w, b, r):
+        return linear(torch.tanh(linear(x * 2, w * 1.5, bias=b, activation="silu")), torch.eye(N, device=DEV, dtype=BF), residual=r)
+
+    want = torch.autograd.grad(step(x, w, b, r), leaves, dy)
+
+    def elsewhere(y):  # what forward freed is given to others before backward
+        junk = [torch.full((n,), float("nan"), device=DEV, dtype=BF) for n in (M * K, M * K, N * K, N * K, M * N, N * N)]
+        grads = torch.autograd.grad(y, leaves, dy)
+        del junk
+        return grads
+
+    with torch.autograd.graph.save_on_cpu():
+        y = step(x, w, b, r)
+    for got, ref in zip(elsewhere(y), want):
+        assert torch.equal(got, ref)
+    y = torch.utils.checkpoint.checkpoint(step, x, w, b, r, use_reentrant=False)
+    for got, ref in zip(elsewhere(y), want):
+        assert torch.equal(got, ref)
 
 
 def test_refusals():
