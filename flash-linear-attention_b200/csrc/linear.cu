@@ -717,12 +717,12 @@ struct GemmPlan {
   size_t bytes;  // of partial sums
 };
 GemmPlan gemm_plan(int M, int N, int K, bool f8, bool bmn) {
-  const long long rows = (M + 255) / 256, clusters = sm_count() / 2;
+  const long long rows = (M + 255ll) / 256, clusters = sm_count() / 2;
   GemmPlan best = {};
   double least = 1e30;
   for (int bn : {256, 128, 64}) {
     if (bmn && bn == 64) continue;
-    const int per = f8 ? 256 : 128, kb = (K + per - 1) / per;  // stages of a sum
+    const int per = f8 ? 256 : 128, kb = (int)((K + (long long)per - 1) / per);  // stages of a sum
     const long long tiles = rows * ((N + bn - 1) / bn);
     for (int want = 1; want <= 64; want *= 2) {
       if (want > 1 && (tiles * want > clusters || kb < 2 * want)) break;
@@ -763,6 +763,8 @@ int launch_gemm(GemmParams p, const void *a, int a_pitch, const void *b, int b_p
   else join_kernel<TO, 1><<<blocks, 256, 0, st>>>((const float *)scratch, q.splits, p);
   return check_launch("linear join");
 }
+
+bool indexed(int M, int N, int K) { return M <= 1 << 30 && N <= 1 << 30 && K <= 1 << 30; }  // by ints, with room for a tile's overhang
 
 template <typename... Ptr> bool four(int n, Ptr... ptr) {
   bool ok = n % 2 == 0;
@@ -831,6 +833,7 @@ int flab_linear_fwd(const void *x, const void *weight, const void *bias, const v
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M >= 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_fwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
+  FLAB_REQUIRE(indexed(M, N, K), FLAB_E_UNSUPPORTED, "linear_fwd: sides beyond 2^30");
   FLAB_REQUIRE(dtype == FLAB_BF16 || dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_fwd: element type %d is not supported", dtype);
   if (M == 0) return FLAB_OK;
   FLAB_REQUIRE(x && weight && y, FLAB_E_BADARG, "linear_fwd needs x, weight, y");
@@ -862,6 +865,7 @@ int flab_linear_bwd(const void *x, const void *weight, const void *z, const void
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M > 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_bwd: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
+  FLAB_REQUIRE(indexed(M, N, K), FLAB_E_UNSUPPORTED, "linear_bwd: sides beyond 2^30");
   FLAB_REQUIRE(dtype == FLAB_BF16 || dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_bwd: element type %d is not supported", dtype);
   FLAB_REQUIRE(dy && ((!dx && !dweight) || (x && weight)) && (act == ACT_NONE || z) && (!dbias || db_partial), FLAB_E_BADARG,
                "linear_bwd needs dy, x and weight for dx or dweight, z for an activation, db_partial for dbias");
@@ -910,6 +914,7 @@ int flab_linear_e4m3(const void *x, const float *x_scale, const void *weight, co
   using namespace flab;
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(M >= 0 && N > 0 && K > 0 && act >= 0 && act <= ACT_GELU, FLAB_E_BADARG, "linear_e4m3: M = %d, N = %d, K = %d or activation %d", M, N, K, act);
+  FLAB_REQUIRE(indexed(M, N, K), FLAB_E_UNSUPPORTED, "linear_e4m3: sides beyond 2^30");
   FLAB_REQUIRE(out_dtype == FLAB_BF16 || out_dtype == FLAB_FP16, FLAB_E_UNSUPPORTED, "linear_e4m3: output type %d is not supported", out_dtype);
   if (M == 0) return FLAB_OK;
   FLAB_REQUIRE(x && x_scale && weight && w_scale && y, FLAB_E_BADARG, "linear_e4m3 needs x, weight, their scales and y");

@@ -718,7 +718,7 @@ int flab_rms_norm_fwd(const void *x, const void *residual, const void *weight, v
                "rms_norm_fwd: a residual of type %d with a sum of type %d is not supported", residual_dtype, sum_dtype);
   FLAB_REQUIRE(norm || (quant && !residual && !weight && !sum && sum_dtype == dtype), FLAB_E_BADARG, "quantisation alone takes x only");
   FLAB_REQUIRE(!quant || scale, FLAB_E_BADARG, "an e4m3 output needs scale");
-  FLAB_REQUIRE(rows < (1ll << 31) - 1, FLAB_E_UNSUPPORTED, "rms_norm_fwd: too many rows (%lld)", rows);
+  FLAB_REQUIRE(rows < (1ll << 31) - 1 && n <= 1 << 30, FLAB_E_UNSUPPORTED, "rms_norm_fwd: too many rows (%lld) or columns (%d)", rows, n);
   NormParams p = {x, residual, weight, y, sum, rstd, scale, rows, n, 0, residual && residual_dtype == FLAB_FP32 && dtype != FLAB_FP32, weight_dtype, eps};
   const bool wide = sum_dtype == FLAB_FP32;
   switch (dtype) {
@@ -746,6 +746,7 @@ int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const v
   cudaStream_t st = (cudaStream_t)stream;
   FLAB_REQUIRE(rows >= 0 && n > 0 && dtype >= 0 && dtype <= 2 && (sum_dtype == dtype || sum_dtype == FLAB_FP32) && weight_dtype >= 0 && weight_dtype <= 2,
                FLAB_E_BADARG, "rms_norm_bwd: unknown element types %d, %d, %d or sizes", dtype, sum_dtype, weight_dtype);
+  FLAB_REQUIRE(n <= 1 << 30, FLAB_E_UNSUPPORTED, "rms_norm_bwd: too many columns (%d)", n);
   FLAB_REQUIRE(!dweight || dw_partial, FLAB_E_BADARG, "rms_norm_bwd: dweight needs dw_partial");
   int parts = 0;
   if (rows > 0) {

@@ -98,6 +98,8 @@ def _check(x, weight, residual, residual_in_fp32):
     """The arguments' checks; returns the type of the residual stream."""
     if x.dim() < 1 or x.dtype not in _DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32 with at least one dimension, got {x.dtype} {tuple(x.shape)}")
+    if x.shape[-1] > 2 ** 30:  # (the C ABI takes it as an int)
+        raise ValueError(f"rows of {x.shape[-1]} elements are beyond 2^30, which the kernels do not index")
     if weight is not None and (tuple(weight.shape) != (x.shape[-1],) or weight.dtype not in _DTYPES):
         raise ValueError(f"weight must be [{x.shape[-1]}] in bfloat16, float16 or float32, got {weight.dtype} {tuple(weight.shape)}")
     if residual is not None:

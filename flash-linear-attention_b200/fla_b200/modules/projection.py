@@ -13,6 +13,7 @@ from .._lib import _DTYPES
 
 ACTIVATIONS = {None: 0, "silu": 1, "swish": 1, "sigmoid": 2, "logsigmoid": 3, "gelu": 4}
 _HALF = (torch.bfloat16, torch.float16)
+_LARGEST = 2 ** 30  # rows or columns (the C ABI takes them as ints)
 
 
 def _p(t):
@@ -106,6 +107,8 @@ def _check(x, weight, bias, residual, activation, dtype):
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"x must be [..., K] and weight [N, K] with N, K > 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
     N = weight.shape[0]
+    if max(math.prod(x.shape[:-1]), N, x.shape[-1]) > _LARGEST:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} have sides beyond 2^30, which the kernels do not index")
     if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != dtype):
         raise ValueError(f"bias must be [{N}] in {dtype}, got {bias.dtype} {tuple(bias.shape)}")
     if residual is not None and (residual.shape != x.shape[:-1] + (N,) or residual.dtype != dtype):

@@ -90,6 +90,8 @@ def _hgrn(x, g, initial_state, output_final_state, offsets):
         raise ValueError(f"x and g must both be [B, T, D], got {tuple(x.shape)} and {tuple(g.shape)}")
     if x.dtype not in _DTYPES or g.dtype != x.dtype:
         raise ValueError(f"x and g must share one of the types bfloat16, float16 and float32, got {x.dtype} and {g.dtype}")
+    if max(x.shape[0], x.shape[2]) > 2 ** 30:  # (the C ABI takes them as ints)
+        raise ValueError(f"x {tuple(x.shape)} has more than 2^30 sequences or channels, which the kernels do not index")
     if not x.is_cuda:
         raise RuntimeError("flab200 kernels run on CUDA tensors only (no CPU fallback)")
     N = x.shape[0]

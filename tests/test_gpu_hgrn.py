@@ -367,6 +367,9 @@ def test_refusals():
         chunk_hgrn(x, x.bfloat16())
     with pytest.raises(ValueError, match="share one of the types"):
         fused_recurrent_hgrn(x.double(), x.double())
+    for big in (x[:1].expand(2 ** 32 + 1, 4, 8), x[:, :, :1].expand(2, 4, 2 ** 32 + 8)):
+        with pytest.raises(ValueError, match="more than 2"):
+            chunk_hgrn(big, big)
     with pytest.raises(ValueError, match="either"):
         chunk_hgrn(x, x, offsets=torch.tensor([0, 4]), cu_seqlens=torch.tensor([0, 4]))
 

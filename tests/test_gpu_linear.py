@@ -267,6 +267,31 @@ def test_a_block_of_them():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FH])
+def test_a_block_under_a_checkpoint(dtype):
+    """The block's gradients are the same bits whether its intermediates are kept, worked out again or brought back from the host."""
+    gen = torch.Generator().manual_seed(31)
+    B, T, D = 2, 70, 96
+    x, dy = (torch.randn(B, T, D, generator=gen).to(DEV).to(dtype) for _ in range(2))
+    ws = [(torch.randn(D, D, generator=gen) * D ** -0.5).to(DEV).to(dtype) for _ in range(3)]
+    leaves = [t.requires_grad_(True) for t in (x, (1 + torch.randn(D, generator=gen)).to(DEV).to(dtype), *ws)]
+
+    def block(x, n, wi, wf, wo):
+        y = rms_norm(x, n)
+        o, _ = chunk_hgrn(linear(y, wi, activation="silu"), linear(y, wf, activation="logsigmoid"))
+        y, s = rms_norm(o, n, residual=x, prenorm=True)
+        return linear(y, wo, residual=s)
+
+    want = torch.autograd.grad(block(*leaves), leaves, dy)
+    for got, ref in zip(torch.autograd.grad(torch.utils.checkpoint.checkpoint(block, *leaves, use_reentrant=False), leaves, dy), want):
+        assert torch.equal(got, ref)
+    with torch.autograd.graph.save_on_cpu():
+        y = block(*leaves)
+    for got, ref in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(got, ref)
+
+
+@pytest.mark.gpu
 def test_only_some_gradients_and_no_rows():
     x, w, b, r, dy = (t.to(DEV) for t in make(70, 40, 24, BF, 0))
     for which in range(4):
@@ -344,6 +369,11 @@ def test_refusals():
         linear(x, w, bias=torch.zeros(7, dtype=BF))
     with pytest.raises(ValueError, match="residual must be"):
         linear(x, w, residual=torch.zeros(1, 8, dtype=BF))
+    for big in (x[:1].expand(2 ** 31 + 4, 16), x[:1].expand(2 ** 17, 2 ** 15, 16)):
+        with pytest.raises(ValueError, match="sides beyond 2"):
+            linear(big, w)
+    with pytest.raises(ValueError, match="sides beyond 2"):
+        linear(x, w[:1].expand(2 ** 32 + 8, 16))
     q, v = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
     with pytest.raises(ValueError, match="float8_e4m3fn"):
         linear_fp8(x, torch.ones(4), w, torch.ones(8))
@@ -373,6 +403,8 @@ def test_abi_refusals():
     assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 5, 0, *none) == -1
     assert b"activation" in lib.flab_last_error()
     assert lib.flab_linear_fwd(16, 16, None, None, 16, None, 8, 8, 8, 0, 2, *none) == -2
+    assert lib.flab_linear_fwd(16, 16, None, None, 16, None, (1 << 31) - 1, 8, 8, 0, 0, *none) == -2
+    assert b"beyond 2^30" in lib.flab_last_error()
     assert lib.flab_linear_workspace(16, 16, 8, 8, 8) == 0
     assert lib.flab_linear_workspace(16, 18, 8, 8, 8) == 256 and lib.flab_linear_workspace(16, 16, 8, 8, 7) == 512
     assert lib.flab_linear_bwd_scratch(16, 8, 8, 8, 0) == 0 and lib.flab_linear_bwd_scratch(16, 8, 8, 8, 1) == 256

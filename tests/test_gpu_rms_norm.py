@@ -270,6 +270,8 @@ def test_refusals():
         rms_norm_quant(x.double(), w)
     with pytest.raises(ValueError, match="bfloat16, float16 or float32"):
         quantize_rows(x.int())
+    with pytest.raises(ValueError, match="beyond 2"):
+        rms_norm(x[:, :1].expand(2, 2 ** 32 + 8), None)
 
 
 @pytest.mark.gpu
