@@ -197,12 +197,12 @@ def call(entry: str, ref: torch.Tensor, **kw):
         check_device_waits(entry)
 
 
-_HERE = nullcontext()
+_STAY = nullcontext()
 
 
 def device_of(t: torch.Tensor):
     """Context in which `t`'s device is the current one; nothing to enter where it already is."""
-    return _HERE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+    return _STAY if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def once(backward):
