@@ -124,6 +124,21 @@ template <int V, typename T> __device__ __forceinline__ void store_e4m3(void *ba
   *reinterpret_cast<Vec<unsigned char, V> *>(reinterpret_cast<unsigned char *>(base) + at) = q;
 }
 
+// The largest magnitude of 16-bit values, as fp32 bits, two to an instruction: magnitudes go as their bits here as well.
+template <typename T, int V> __device__ __forceinline__ unsigned top_of(unsigned most, const Vec<T, V> &v) {
+  if constexpr (V == 1) {
+    return max(most, (unsigned)(*reinterpret_cast<const unsigned short *>(&v) & 0x7fff));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) most = __vmaxu2(most, reinterpret_cast<const unsigned *>(&v)[j] & 0x7fff7fffu);
+    return most;
+  }
+}
+template <typename T> __device__ __forceinline__ unsigned wide_top(unsigned most) {
+  const unsigned short one = (unsigned short)max(most & 0xffffu, most >> 16);
+  return magnitude(Num<T>::f(*reinterpret_cast<const T *>(&one)));
+}
+
 // T: x and y;  S: the stored sum;  RES: residual, 0 none, 1 of type T, 2 fp32;  V elements a vector, NV vectors a thread (0: read
 // again);  QUANT: e4m3 output;  NORM: without it the rows are quantised as they are.
 // All of a row's loads are issued before its first store: with loads and stores of one loop in turn a row was eight trips to
@@ -194,6 +209,11 @@ __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const Nor
   }
   auto result = [&](int k, float (&y)[V]) {
     const Vec<S, V> v = NV ? s[NV ? k : 0] : fetch(at(k));
+    if (!NORM) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[j] = Num<S>::f(v.v[j]);
+      return;
+    }
     float w[V];
     load_w<V>(p.w, p.w_type, at(k), w);
 #pragma unroll
@@ -205,11 +225,16 @@ __global__ void __launch_bounds__(NV ? 512 : 1024) rms_norm_fwd_kernel(const Nor
 #pragma unroll
     for (int k = 0; k < (NV ? NV : loops); ++k)
       if (on && at(k) < p.n) {
-        float y[V];
-        result(k, y);
+        if constexpr (!NORM && sizeof(S) == 2) {
+          bits = top_of<S, V>(bits, NV ? s[NV ? k : 0] : fetch(at(k)));
+        } else {
+          float y[V];
+          result(k, y);
 #pragma unroll
-        for (int j = 0; j < V; ++j) bits = max(bits, magnitude(y[j]));
+          for (int j = 0; j < V; ++j) bits = max(bits, magnitude(y[j]));
+        }
       }
+    if constexpr (!NORM && sizeof(S) == 2) bits = wide_top<S>(bits);
     top = row_top(bits, p.tpr, slots[1], BlockSync());
     if (on && li == 0) p.scale[row] = top * (1.f / E4M3_MAX);
   }
