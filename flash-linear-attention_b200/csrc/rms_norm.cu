@@ -11,7 +11,7 @@
 // that are read again from L2 (NV = 0).  dw: every thread sums its columns over the rows of its block in registers, one partial row a
 // block, and a second small kernel adds the partial rows in order: no atomics, results repeat bit for bit.
 // Measured at 32768 x 2048 bf16 with a residual, of the copy rate: forward 78 us (105 % with the inputs of the run before still partly
-// in L2, 97 us cold), e4m3 93 us, backward 102 us; 256 rows 2.5 us, e4m3 2.9 us, backward 7.4 us (the latency of a row).
+// in L2, 97 us cold), e4m3 87 us, backward 102 us, quantised as they are 40 us (77 %); 256 rows 2.5 us, e4m3 2.9 us, backward 7.4 us (the latency of a row).
 #include <cuda_fp8.h>
 
 #include <initializer_list>
@@ -98,7 +98,7 @@ struct BlockSync {
 
 // How a row's values become e4m3: divided by the scale where x has 32 bits, so that a value next to the border of two bytes falls as the
 // formula has it; multiplied by the scale's reciprocal where x has 16 (an ulp of fp32 is 2^-16 of its step, and the division would
-// make the kernel wait for its arithmetic: 93 us a product against 72 for the bytes at 32768 x 2048).
+// make the kernel wait for its arithmetic: 87 us with the product against 72 for the bytes at 32768 x 2048).
 template <typename T> struct Quantiser {
   static constexpr bool DIVIDE = sizeof(T) == 4;
   float by;
@@ -424,14 +424,24 @@ __global__ void __launch_bounds__(RING_THREADS, 1) rms_norm_fwd_ring_kernel(cons
       for (int k = 0; k < NV; ++k)
         if (at(k) < p.n) *reinterpret_cast<Vec<S, V> *>(reinterpret_cast<S *>(p.sum) + base + at(k)) = s[k];
     }
-    float top = 0.f;
+    // The products that an e4m3 row needs twice are kept where the sum has 16 bits (32768 x 2048 bf16, cold: 91 -> 87 us) and formed again
+    // where it has 32 (with an fp32 residual 123 us, and 131 kept).
+    constexpr bool ONCE = QUANT && sizeof(S) == 2;
+    float top = 0.f, kept[ONCE ? NV : 1][V];
+    auto result = [&](int k, int j) { return Num<S>::f(s[k].v[j]) * rstd * w[k][j]; };
+    if (ONCE) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) kept[ONCE ? k : 0][j] = result(k, j);
+    }
     if (QUANT) {
       unsigned bits = 0;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
         if (at(k) < p.n) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) bits = max(bits, magnitude(Num<S>::f(s[k].v[j]) * rstd * w[k][j]));
+          for (int j = 0; j < V; ++j) bits = max(bits, magnitude(ONCE ? kept[ONCE ? k : 0][j] : result(k, j)));
         }
       top = row_top(bits, q.tpr, slots[2 + par], GroupSync{q.tpr, group});
       if (li == 0) p.scale[row] = top * (1.f / E4M3_MAX);
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) rms_norm_fwd_ring_kernel(cons
       if (at(k) < p.n) {
         float y[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] = Num<S>::f(s[k].v[j]) * rstd * w[k][j];
+        for (int j = 0; j < V; ++j) y[j] = ONCE ? kept[ONCE ? k : 0][j] : result(k, j);
         if constexpr (QUANT) store_e4m3<V>(p.y, base + at(k), y, to);
         else store_f<T, V>(p.y, base + at(k), y);
       }
