@@ -10,8 +10,9 @@
 // vectors of 16 bytes each; rows whose length or address does not allow vectors go element by element, and rows too long for
 // that are read again from L2 (NV = 0).  dw: every thread sums its columns over the rows of its block in registers, one partial row a
 // block, and a second small kernel adds the partial rows in order: no atomics, results repeat bit for bit.
-// Measured at 32768 x 2048 bf16 with a residual, of the copy rate: forward 78 us (105 % with the inputs of the run before still partly
-// in L2, 97 us cold), e4m3 87 us, backward 102 us, quantised as they are 40 us (77 %); 256 rows 2.5 us, e4m3 2.9 us, backward 7.4 us (the latency of a row).
+// Measured at 32768 x 2048 bf16 with a residual, of the copy rate: forward 90 us (91 %) in a training step, e4m3 83
+// us (87 %), quantised as they are 40 us (77 %), backward 109 us with its partial sums (the kernel alone 102, 80 %); with an fp32 stream
+// forward 141 us (87 %), backward 170 (96 %); 256 rows 2.5 us, e4m3 2.9 us, backward 7.4 us (the latency of a row).
 #include <cuda_fp8.h>
 
 #include <initializer_list>
@@ -580,13 +581,18 @@ bool aligned_to(int bytes, std::initializer_list<const void *> ptrs) {
 }
 bool aligned16(std::initializer_list<const void *> ptrs) { return aligned_to(16, ptrs); }
 
-// The ring's shape for rows of n elements (V a vector) of which a stage holds row_bytes; false: not for these rows.  It pays from so
-// many rows a group on (`enough`): forward at 2048 columns of bf16, 2368 rows 9.0 us against 8.8 without it, 4096 rows 13.4 against
-// 15.0, 32768 rows 78 against 98; backward 1184 rows 10.5 against 15.1, 32768 rows 102 against 213.
-bool ring_shape(long long rows, int n, int V, int row_bytes, int enough, RingShape &q, int &nv, int &grid) {
+// The ring's shape for rows of n elements (V a vector) of which a stage holds row_bytes; false: not for these rows.  `per` is how many
+// vectors a thread is to have, `most` how many it can.  Few are quick over a row, many let more groups have rows in hand, which is what
+// counts where a row has a second reduction (e4m3) or a longer way (backward).  Us with 8 / 16 / 32 elements a thread: e4m3 32768 x 2048
+// bf16 121 / 87 / 83, 16384 x 8192 bf16 - / 177 / 150, with an fp32 residual 141 / 124 / 144; backward 32768 x 2048 bf16 140 / 109 /
+// 224 (spilled), 16384 x 2048 fp32 128, 89 and 71 with 4, 8 and 16.
+// The ring pays from so many rows a group on (`enough`, at two vectors a thread): forward at 2048 columns of bf16, 2368 rows 9.0 us
+// against 8.8 without it, 4096 rows 13.4 against 15.0, 32768 rows 78 against 98; backward 1184 rows 10.5 against 15.1, 32768 rows 102
+// against 213.
+bool ring_shape(long long rows, int n, int V, int row_bytes, int enough, int per, int most, RingShape &q, int &nv, int &grid) {
   const int vecs = n / V;
   q.tpr = 32;
-  while (2 * q.tpr < vecs && q.tpr < RING_THREADS) q.tpr *= 2;
+  while (per * q.tpr < vecs && q.tpr < RING_THREADS) q.tpr *= 2;
   nv = (vecs + q.tpr - 1) / q.tpr;
   if (nv == 3) nv = 4;
   q.groups = RING_THREADS / q.tpr;
@@ -594,7 +600,8 @@ bool ring_shape(long long rows, int n, int V, int row_bytes, int enough, RingSha
   q.stages = (int)(200 * 1024 / ((size_t)q.groups * row_bytes));
   if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
   grid = sm_count();
-  return nv <= (V == 4 ? 4 : 2) && q.stages >= 2 && rows >= (long long)enough * q.groups * grid;
+  const int have = per > 2 && nv < per ? 2 : per;
+  return nv <= most && q.stages >= 2 && rows * have >= 2ll * enough * q.groups * grid;
 }
 
 template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_norm_fwd(NormParams p, cudaStream_t st) {
@@ -603,7 +610,11 @@ template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_nor
   const bool aligned = p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum});
   RingShape q;
   int grid_ring;
-  if (NORM && aligned && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0)), 6, q, nv, grid_ring)) {
+  const int row_bytes = p.n * (int)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0));
+  // Forward has one reduction: 16 elements a thread for 16 bits (32768 x 2048 90 us against 99 with 8, in a training step), and for 32 bits
+  // 8 where the inputs may still lie in L2 (below its 126 MB: 2368 x 2048 11.0 us against 13.6) and 4 from HBM (16384 x 2048 98 and 85).
+  const int per = QUANT ? (sizeof(S) == 2 ? 32 : 16) / V : sizeof(T) == 4 && p.rows * row_bytes >= 1ll << 27 ? 1 : 2;
+  if (NORM && aligned && ring_shape(p.rows, p.n, V, row_bytes, 6, per, QUANT || V == 4 ? 4 : 2, q, nv, grid_ring)) {
     const size_t bytes = (size_t)q.groups * q.stages * q.row_bytes;
     auto launch = [&](auto kernel) {
       const int rc = set_smem(kernel, bytes);
@@ -611,7 +622,7 @@ template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_nor
       kernel<<<grid_ring, RING_THREADS, bytes, st>>>(p, q);
       return check_launch("rms_norm_fwd");
     };
-    if constexpr (V == 4) {
+    if constexpr (QUANT || V == 4) {
       if (nv == 4) return launch(rms_norm_fwd_ring_kernel<T, S, RES, 4, QUANT>);
     }
     return nv == 1 ? launch(rms_norm_fwd_ring_kernel<T, S, RES, 1, QUANT>) : launch(rms_norm_fwd_ring_kernel<T, S, RES, 2, QUANT>);
@@ -678,7 +689,7 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
   const bool aligned = aligned16({p.s, p.dy, p.ds, p.w, p.dx, p.dr});
   RingShape r;
   int nv;
-  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + 2 * sizeof(S)), 2, r, nv, parts)) {
+  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + 2 * sizeof(S)), 2, 16 / V, 16 / V, r, nv, parts)) {
     size_t bytes = (size_t)r.groups * r.stages * r.row_bytes;
     const size_t sums = (size_t)r.groups * p.n * sizeof(float);
     if (bytes < sums) bytes = sums;
