@@ -15,7 +15,7 @@
 // pairs work on at one time shares operands in L2.
 // Measured, bf16, 32768 x 2048 x 2048: product alone 184 us (1490 TFLOP/s; the library's 180), with silu, bias and residual 194 us, dx
 // 183, dW 186 us; 8192 x 8192 x 8192 706 us (1558 TFLOP/s; the library's 663).  e4m3, 32768 x 2048 x 2048 with scales 105 us (2620
-// TFLOP/s), with silu 121 us.  Bound by the tensor pipe under the power cap (77 to 82 % active without an epilogue, 68 % with
+// TFLOP/s), with silu 121 us.  Bound by the tensor pipe under the power cap (88 to 93 % active without an epilogue, 83 % with
 // one); 256 x 2048 x 2048 takes 12.2 us, the loop over 32 blocks.
 #include <type_traits>
 
