@@ -125,6 +125,15 @@ def held(q, scale, y64):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,res,wdtype,wide", [TYPES[1], TYPES[2], TYPES[4], TYPES[5]])
+@pytest.mark.parametrize("rows,n", [(1000, 8192), (3700, 2048), (3700, 1032), (14300, 264), (8200, 2048)])
+def test_many_rows(rows, n, dtype, res, wdtype, wide):
+    """Enough rows for the ring in both directions and in 8 bits, with one to four vectors a thread; the last are 128 MB in 32 bits."""
+    test_forward_and_gradients(rows, n, dtype, res, wdtype, wide)
+    test_eight_bits(rows, n, dtype, res, wdtype, wide)
+
+
+@pytest.mark.gpu
 def test_rows_without_a_scale():
     x = torch.zeros(4, 512, device=DEV)
     x[1, 3] = float("nan")
