@@ -1,0 +1,87 @@
+"""The ends of the ranges that the operators of the gated-recurrence block are documented for: values that a type cannot hold, rows of
+nothing, derivatives and uses of the results that a program may ask for, waits that ran out. Each test says which value the
+definition gives; the tolerances count roundings as in the operators' own test files."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+import torch.nn.functional as F
+
+from fla_b200 import _lib
+from fla_b200.modules import RMSNorm, linear, linear_fp8, quantize_rows, rms_norm, rms_norm_quant
+from fla_b200.ops import chunk_hgrn, fused_recurrent_hgrn
+
+DEV = "cuda"
+BF, FH, F32 = torch.bfloat16, torch.float16, torch.float32
+U = 2.0 ** -24
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def half_step(value, dtype):
+    tiny = {BF: 2.0 ** -134, FH: 2.0 ** -25, F32: 2.0 ** -150}[dtype]
+    return value.abs() * torch.finfo(dtype).eps / 2 + tiny
+
+
+def within(name, got, want, bound):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape and torch.isfinite(got).all(), name
+    over = ((got - want).abs() - bound).max().item()
+    assert over <= 0, f"{name}: {over:.3e} over its bound"
+
+
+ACTIVATIONS = {"silu": F.silu, "sigmoid": torch.sigmoid, "logsigmoid": F.logsigmoid, "gelu": F.gelu}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("M,K,N", [(40, 64, 48), (40, 64, 33), (33, 4096, 40)])  # tile stores, other outputs, a sum in runs
+def test_gradients_where_fp16_cannot_hold_the_argument(M, K, N, act):
+    """z = -131072 and 131072 overflow fp16, in which z is kept for backward; the slopes there are 0 and 1, and so are the gradients'
+    parts. The bounds are those of the operator's own tests; beyond |z| = 100 every slope is 0 or 1 to within 2^-20."""
+    gen = torch.Generator().manual_seed(M + N)
+    x = torch.randn(M, K, generator=gen).to(FH)
+    w = (torch.randn(N, K, generator=gen) * K ** -0.5).to(FH)
+    w[0] = -64
+    x[0], x[1] = 2048.0 / K, -2048.0 / K
+    b = torch.randn(N, generator=gen).to(FH)
+    dy = torch.randn(M, N, generator=gen).to(FH)
+    X, W, D = x.double(), w.double(), dy.double()
+    z = (X @ W.T + b.double()).requires_grad_(True)
+    assert z[0, 0] < -131000 and z[1, 0] > 131000
+    dz = torch.autograd.grad(ACTIVATIONS[act](z), z, D)[0]
+    z = z.detach()
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    y = linear(leaves[0], leaves[1], bias=leaves[2], activation=act)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.to(DEV))
+    size = (X.abs() @ W.abs().T) * K * 2.0 ** -23
+    near = 0.8 * (half_step(z, FH) + size + 2.0 ** -23 * z.abs()) + 2.0 ** -18 * (1 + z.abs())
+    slope = D.abs() * torch.where(z.abs() > 100, 2.0 ** -20, near)
+    edz = slope + half_step(dz, FH)
+    want = dz @ W
+    within("dx", dx, want, edz @ W.abs() + (dz.abs() @ W.abs()) * N * 2.0 ** -23 + half_step(want, FH))
+    want = dz.T @ X
+    within("dw", dw, want, edz.T @ X.abs() + (dz.abs().T @ X.abs()) * M * 2.0 ** -23 + half_step(want, FH))
+    want = dz.sum(0)
+    within("db", db, want, slope.sum(0) + dz.abs().sum(0) * M * U + half_step(want, FH))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [48, 33])
+def test_an_argument_that_is_not_finite_stays_so(N):
+    """What is held in fp16's range are values that fp32 holds: a NaN or an infinity among the inputs still reaches the gradients of its
+    row, and no other row's."""
+    gen = torch.Generator().manual_seed(7)
+    x, w = torch.randn(6, 64, generator=gen).to(FH), (torch.randn(N, 64, generator=gen) / 8).to(FH)
+    clean = x.clone()
+    x[2, 5], x[4, 5] = float("nan"), float("inf")
+    dys = torch.ones(6, N, dtype=FH, device=DEV)
+    out = []
+    for v in (x, clean):
+        v = v.to(DEV).requires_grad_(True)
+        out.append(torch.autograd.grad(linear(v, w.to(DEV), activation="silu"), v, dys)[0])
+    assert torch.isnan(out[0][2]).all() and not torch.isfinite(out[0][4]).all()
+    keep = [0, 1, 3, 5]
+    assert torch.equal(out[0][keep], out[1][keep]) and torch.isfinite(out[1]).all()
