@@ -43,6 +43,8 @@ def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=T
                                        _DTYPES[torch.float32 if w is None else w.dtype], NORM_E4M3 * quant + NORM_NONE * (not norm), eps,
                                        _lib.stream_of(x2))
         _lib.finish("flab_rms_norm_fwd", rc)
+    elif quant:
+        scale.zero_()  # rows of no elements
     return y, scale, total, rstd
 
 

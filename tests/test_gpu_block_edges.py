@@ -85,3 +85,16 @@ def test_an_argument_that_is_not_finite_stays_so(N):
     assert torch.isnan(out[0][2]).all() and not torch.isfinite(out[0][4]).all()
     keep = [0, 1, 3, 5]
     assert torch.equal(out[0][keep], out[1][keep]) and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 0), (2, 5, 0), (700, 0)])
+def test_rows_of_no_elements_have_scale_zero(shape):
+    rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
+    for _ in range(4):  # what the allocator hands out next held something else
+        junk = torch.full((rows,), float("nan"), device=DEV)
+        torch.cuda.synchronize()
+        del junk
+        x, w = torch.empty(shape, device=DEV, dtype=BF), torch.ones(0, device=DEV, dtype=BF)
+        for q, scale in (quantize_rows(x), rms_norm_quant(x, w), rms_norm_quant(x, w, residual=x, prenorm=True)[:2]):
+            assert q.shape == shape and scale.shape == shape[:-1] and (scale == 0).all()
