@@ -50,6 +50,7 @@ struct HgrnParams {
   int nT, nCG;       // tiles along time, channel groups
   long long T;
   int *ticket;
+  int *abort;                // set by a wait of this launch that ran out
   unsigned long long *maps;  // [tiles][C] words; null with one tile along time
   unsigned long long *ends;  // [groups][C] words
 };
@@ -124,16 +125,28 @@ __device__ __forceinline__ unsigned long long look(const unsigned long long *a) 
   asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(a) : "memory");
   return w;
 }
-// Bounded wait for a word's mark, about a second; once any wait has run out, no further one waits.
-__device__ __forceinline__ unsigned long long await(const unsigned long long *a, unsigned long long w) {
+// What a wait that ran out hands back, as an end and as a map: NaN, so that nothing which depends on it looks like a result.
+__device__ __forceinline__ unsigned long long lost() { return map_word(0.f, __uint_as_float(0x7fffffffu)); }
+// Bounded wait for a word's mark, about a second; once any wait of the launch has run out, no further one of it waits.  (The error word
+// is only written here: it stays set until the host clears it, and other launches are not to give up for it.  CALL: the record
+// by a call.  Inlined, it costs the tile kernel registers ([8, 4096, 2047] bf16 forward 273 us against 265); the call costs the
+// streaming kernel some ([1, 262144, 2048] forward 552 us against 547).)
+__device__ __forceinline__ void give_up(int *abort) {
+  *reinterpret_cast<volatile int *>(abort) = 1;
+  tu_tc_error = 700;
+}
+__device__ __noinline__ void give_up_by_call(int *abort) { give_up(abort); }
+template <bool CALL>
+__device__ __forceinline__ unsigned long long await(const unsigned long long *a, unsigned long long w, int *abort, long long limit = 1ll << 31) {
   if (w >> 32) return w;
   const long long t0 = clock64();
   for (int spins = 1;; ++spins) {
     w = look(a);
     if (w >> 32) return w;
-    if ((spins & 255) == 0 && (clock64() - t0 > (1ll << 31) || *reinterpret_cast<volatile int *>(&tu_tc_error))) {
-      tu_tc_error = 700;
-      return map_word(0.f, 0.f);
+    if ((spins & 255) == 0 && (clock64() - t0 > limit || *reinterpret_cast<volatile int *>(abort))) {
+      if (CALL) give_up_by_call(abort);
+      else give_up(abort);
+      return lost();
     }
   }
 }
@@ -239,7 +252,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const unsigned long long *a = p.maps + ((size_t)(first + w) * chains + chain) * C + lane * V + j;
-        const float2 m = map_of(await(a, look(a)));
+        const float2 m = map_of(await<true>(a, look(a), p.abort));
         lP[w][lane * V + j] = m.x;
         lQ[w][lane * V + j] = m.y;
       }
@@ -252,7 +265,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const unsigned long long *a = p.ends + ((size_t)(group - 1) * chains + chain) * C + lane * V + j;
-        c[j] = end_of(await(a, look(a)));
+        c[j] = end_of(await<true>(a, look(a), p.abort));
       }
     }
 #pragma unroll
@@ -616,9 +629,13 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < G - 1; ++i) missing = missing || (i < before && !((g[i][0] >> 32) && (g[i][1] >> 32)));
         if (!__any_sync(0xffffffffu, missing)) break;
-        // the wait has a bound like every other: about a second, and none once any has run out
-        if ((spins & 255) == 0 && __any_sync(0xffffffffu, clock64() - asked > (1ll << 31) || *reinterpret_cast<volatile int *>(&tu_tc_error))) {
-          tu_tc_error = 700;
+        // the wait has a bound like every other: about a second, and none once any of the launch has run out
+        if ((spins & 255) == 0 && __any_sync(0xffffffffu, clock64() - asked > (1ll << 31) || *reinterpret_cast<volatile int *>(p.abort))) {
+          give_up(p.abort);
+#pragma unroll
+          for (int i = 0; i < G - 1; ++i)
+            for (int k = 0; k < 2; ++k)
+              if (!(g[i][k] >> 32)) g[i][k] = lost();
           break;
         }
 #pragma unroll
@@ -643,7 +660,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       const Map2 group_map = join(join(join(tile_map(0), tile_map(1)), join(tile_map(2), tile_map(3))), join(join(tile_map(4), tile_map(5)), tile_map(6)));
       float2 c = make_float2(0.f, 0.f);
       if (group > 0) {
-        c = make_float2(end_of(await(ends, e[0])), end_of(await(ends + 1, e[1])));
+        c = make_float2(end_of(await<false>(ends, e[0], p.abort)), end_of(await<false>(ends + 1, e[1], p.abort)));
       }
       else if (!VAR && edge && ch < p.D) c = *reinterpret_cast<const float2 *>(edge + (size_t)z.b * p.D + ch);
       c = through(group_map, c);
@@ -806,6 +823,13 @@ template <typename T, int V, bool BWD> __global__ void __launch_bounds__(256) hg
   if (p.ht) *reinterpret_cast<PF *>(p.ht + state) = c;
 }
 
+// A wait that is meant to run out, on a word that nothing sets.  status[32] is its call's abort flag.
+__device__ unsigned long long never_set = 0;
+__global__ void __launch_bounds__(32) hgrn_wait_selftest_kernel(long long limit_ticks, int *status) {
+  const unsigned long long w = await<false>(&never_set, look(&never_set), status + 32, limit_ticks);
+  if (threadIdx.x == 0) *status = isnan(end_of(w)) && isnan(map_of(w).y) ? 700 : 0;
+}
+
 template <typename T> struct HgrnTile {
   static constexpr int W = 8, R = 16, L = W * R;
 };
@@ -813,7 +837,7 @@ template <typename T> struct HgrnTile {
 struct HgrnPlan {
   int V, C, nT, nCG;
   long long tiles;
-  size_t bytes, end_bytes, map_bytes;  // the ticket (256 bytes), the ends, the maps
+  size_t bytes, end_bytes, map_bytes;  // the ticket and the abort flag (256 bytes), the ends, the maps
 };
 
 HgrnPlan hgrn_plan(int B, long long T, int D, int V, int L) {
@@ -834,6 +858,7 @@ int hgrn_scratch(HgrnParams &p, const HgrnPlan &q, void *ws, size_t ws_bytes, cu
                "hgrn needs a 16-byte aligned workspace of flab_hgrn_workspace() bytes");
   char *w = reinterpret_cast<char *>(ws);
   p.ticket = reinterpret_cast<int *>(w);
+  p.abort = p.ticket + 32;
   p.ends = reinterpret_cast<unsigned long long *>(w + 256);
   p.maps = reinterpret_cast<unsigned long long *>(w + 256 + q.end_bytes);
   FLAB_REQUIRE(cudaMemsetAsync(w, 0, q.bytes, st) == cudaSuccess, FLAB_E_LAUNCH, "hgrn: clearing the workspace failed");
@@ -975,5 +1000,14 @@ int flab_hgrn_bwd(const void *g, const void *o, const float *h0, const void *d_o
   p.x = d_o, p.g = g, p.o_in = o, p.h0 = h0, p.dht = dht, p.o = dx, p.dg = dg, p.ht = dh0, p.cu = cu_seqlens, p.cu64 = cu_is_int64;
   p.B = B, p.T = T, p.D = D, p.N = N;
   return run_hgrn<true>(p, dtype, ws, ws_bytes, (cudaStream_t)stream);
+}
+
+int flab_hgrn_wait_selftest(long long limit_ticks, int *status, void *stream) {
+  using namespace flab;
+  FLAB_REQUIRE(status != nullptr, FLAB_E_BADARG, "hgrn_wait_selftest: NULL status");
+  FLAB_REQUIRE(limit_ticks > 0 && limit_ticks <= (1ll << 28), FLAB_E_BADARG,
+               "hgrn_wait_selftest: the limit must be between 1 and 2^28 clock ticks (a fraction of a second)");
+  hgrn_wait_selftest_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(limit_ticks, status);
+  return check_launch("hgrn_wait_selftest");
 }
 }

@@ -84,8 +84,9 @@ def load() -> ctypes.CDLL:
     for name in ("flab_tc_error_state", "flab_tc_check", "flab_tc_error_clear"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = []
-    lib.flab_tc_wait_selftest.restype = ctypes.c_int
-    lib.flab_tc_wait_selftest.argtypes = [ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]
+    for name in ("flab_tc_wait_selftest", "flab_hgrn_wait_selftest"):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]
     lib.flab_l2norm_fwd.restype = ctypes.c_int
     lib.flab_l2norm_fwd.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                     ctypes.c_float, ctypes.c_void_p]

@@ -306,7 +306,8 @@ int flab_recurrent_delta_bwd(const flab_args *a, void *stream);
  * (int32, or int64 with cu_is_int64), non-decreasing and within [0, T] (a value outside is taken as the nearer end, and no table makes
  * a kernel leave its buffers); empty sequences pass h0 to ht (dht to dh0), and rows of no sequence get zeros.
  * Scratch: ws, 16-byte aligned, of flab_hgrn_workspace(B, T, D) bytes (0: ws may be NULL); its contents need no preparation.
- * Blocks wait for earlier blocks of the same launch, with a bound: flab_tc_check() reports a wait that ran out. */
+ * Blocks wait for earlier blocks of the same launch, with a bound: flab_tc_check() reports a wait that ran out, and the values that
+ * would have come through it are NaN. Other launches are not touched by it. */
 size_t flab_hgrn_workspace(int B, long long T, int D);
 int flab_hgrn_fwd(const void *x, const void *g, const float *h0, void *o, float *ht, const void *cu_seqlens, int cu_is_int64, int B, long long T,
                   int D, int N, int dtype, void *ws, size_t ws_bytes, void *stream);
@@ -363,6 +364,10 @@ int flab_tc_selftest(const void *a, const void *b, const void *h, const void *v,
  * *status (device int) and to the error word, and returns. Afterwards flab_tc_check() reports
  * FLAB_E_TIMEOUT until flab_tc_error_clear(). */
 int flab_tc_wait_selftest(long long limit_ticks, int *status, void *stream);
+/* The same for the wait of the recurrence's blocks for one another (id 700), on a word that nothing sets. status: 64 device ints; [32]
+ * is what the workspace's abort flag is to a call (set here, and with it set before the call the wait gives up at once instead of at
+ * its limit), [0] becomes 700 where NaN came back, as it has to. */
+int flab_hgrn_wait_selftest(long long limit_ticks, int *status, void *stream);
 
 #ifdef __cplusplus
 }

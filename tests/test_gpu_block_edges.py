@@ -98,3 +98,47 @@ def test_rows_of_no_elements_have_scale_zero(shape):
         x, w = torch.empty(shape, device=DEV, dtype=BF), torch.ones(0, device=DEV, dtype=BF)
         for q, scale in (quantize_rows(x), rms_norm_quant(x, w), rms_norm_quant(x, w, residual=x, prenorm=True)[:2]):
             assert q.shape == shape and scale.shape == shape[:-1] and (scale == 0).all()
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_stays_with_its_call():
+    """A wait for an earlier tile's word, with a short limit, on a word that nothing sets: it hands back NaN, marks its own call's abort
+    flag and is recorded. Later calls, whose tiles wait for each other thousands of times, do not look at that record."""
+    lib = _lib.load()
+    T, D = 120000, 64
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(1, T, D, generator=gen).to(DEV).to(BF)
+    odd = torch.randn(1, T // 4, 63, generator=gen).to(DEV)
+    g, godd = -x.abs() / 16, -odd.abs() / 16
+    want = [chunk_hgrn(x, g, output_final_state=True), chunk_hgrn(odd, godd, output_final_state=True)]
+    torch.cuda.synchronize()
+    assert lib.flab_tc_check() == 0
+    status = torch.zeros(64, dtype=torch.int32, device=DEV)  # [0]: what came back, [32]: the call's abort flag
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.flab_hgrn_wait_selftest(1 << 20, status.data_ptr(), stream) == 0
+    torch.cuda.synchronize()
+    assert status[0].item() == 700 and status[32].item() == 1  # NaN, and no later wait of that call waits
+    assert lib.flab_tc_error_state() == 700
+    try:
+        for _ in range(5):
+            for (v, gate), (o, ht) in zip(((x, g), (odd, godd)), want):
+                again, last = chunk_hgrn(v, gate, output_final_state=True)
+                assert torch.equal(again, o) and torch.equal(last, ht)
+    finally:
+        torch.cuda.synchronize()
+        assert lib.flab_tc_error_clear() == 0
+    # with the flag set the same wait gives up instead of at its limit
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    assert lib.flab_hgrn_wait_selftest(1 << 28, status.data_ptr(), stream) == 0
+    end.record()
+    torch.cuda.synchronize()
+    assert status[0].item() == 700 and begin.elapsed_time(end) < 50  # 2^28 ticks are 130 ms and more
+    assert lib.flab_tc_error_clear() == 0 and lib.flab_tc_check() == 0
+
+
+def test_wait_selftest_refuses():
+    lib = _lib.load()
+    for limit in (0, -1, (1 << 28) + 1):
+        assert lib.flab_hgrn_wait_selftest(limit, 16, None) == -1
+    assert lib.flab_hgrn_wait_selftest(1 << 20, None, None) == -1
