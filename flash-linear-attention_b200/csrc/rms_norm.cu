@@ -589,15 +589,17 @@ bool aligned16(std::initializer_list<const void *> ptrs) { return aligned_to(16,
 // The ring pays from so many rows a group on (`enough`, at two vectors a thread): forward at 2048 columns of bf16, 2368 rows 9.0 us
 // against 8.8 without it, 4096 rows 13.4 against 15.0, 32768 rows 78 against 98; backward 1184 rows 10.5 against 15.1, 32768 rows 102
 // against 213.
-bool ring_shape(long long rows, int n, int V, int row_bytes, int enough, int per, int most, RingShape &q, int &nv, int &grid) {
+bool ring_shape(long long rows, int n, int V, long long row_bytes, int enough, int per, int most, RingShape &q, int &nv, int &grid) {
+  constexpr int RING = 200 * 1024;
+  if (2 * row_bytes > RING) return false;
   const int vecs = n / V;
   q.tpr = 32;
   while (per * q.tpr < vecs && q.tpr < RING_THREADS) q.tpr *= 2;
   nv = (vecs + q.tpr - 1) / q.tpr;
   if (nv == 3) nv = 4;
   q.groups = RING_THREADS / q.tpr;
-  q.row_bytes = row_bytes;
-  q.stages = (int)(200 * 1024 / ((size_t)q.groups * row_bytes));
+  q.row_bytes = (int)row_bytes;
+  q.stages = (int)(RING / (q.groups * row_bytes));
   if (q.stages > MAX_STAGES) q.stages = MAX_STAGES;
   grid = sm_count();
   const int have = per > 2 && nv < per ? 2 : per;
@@ -610,7 +612,7 @@ template <typename T, typename S, int RES, bool QUANT, bool NORM> int launch_nor
   const bool aligned = p.n % V == 0 && aligned16({p.x, p.res, p.w, p.y, p.sum});
   RingShape q;
   int grid_ring;
-  const int row_bytes = p.n * (int)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0));
+  const long long row_bytes = p.n * (long long)(sizeof(T) + (RES == 2 ? 4 : RES ? sizeof(T) : 0));
   // Forward has one reduction: 16 elements a thread for 16 bits (32768 x 2048 90 us against 99 with 8, in a training step), and for 32 bits
   // 8 where the inputs may still lie in L2 (below its 126 MB: 2368 x 2048 11.0 us against 13.6) and 4 from HBM (16384 x 2048 98 and 85).
   const int per = QUANT ? (sizeof(S) == 2 ? 32 : 16) / V : sizeof(T) == 4 && p.rows * row_bytes >= 1ll << 27 ? 1 : 2;
@@ -689,7 +691,7 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
   const bool aligned = aligned16({p.s, p.dy, p.ds, p.w, p.dx, p.dr});
   RingShape r;
   int nv;
-  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (int)(sizeof(T) + 2 * sizeof(S)), 2, 16 / V, 16 / V, r, nv, parts)) {
+  if (aligned && p.n % V == 0 && ring_shape(p.rows, p.n, V, p.n * (long long)(sizeof(T) + 2 * sizeof(S)), 2, 16 / V, 16 / V, r, nv, parts)) {
     size_t bytes = (size_t)r.groups * r.stages * r.row_bytes;
     const size_t sums = (size_t)r.groups * p.n * sizeof(float);
     if (bytes < sums) bytes = sums;

@@ -142,3 +142,27 @@ def test_wait_selftest_refuses():
     for limit in (0, -1, (1 << 28) + 1):
         assert lib.flab_hgrn_wait_selftest(limit, 16, None) == -1
     assert lib.flab_hgrn_wait_selftest(1 << 20, None, None) == -1
+
+
+LONG_ROWS = """
+import sys
+sys.path.insert(0, sys.argv[1])
+from fla_b200 import _lib
+lib = _lib.load()
+codes = []
+for n, dtype, res in ((1 << 30, 2, False), (1 << 29, 2, True), (1 << 30, 0, True), (1 << 30, 2, True), (357913944, 0, True), (1 << 20, 0, True)):
+    for flags in (0, 1):
+        codes.append(lib.flab_rms_norm_fwd(16, 16 if res else None, 16, 16, 16, 16, 16, 1, n, dtype, dtype, dtype, dtype, flags, 1e-6, None))
+    codes.append(lib.flab_rms_norm_bwd(16, 16, 16, 16, 16, 16, None, None, None, 1, n, dtype, dtype, dtype, None))
+    codes.append(lib.flab_rms_norm_bwd(16, 16, 16, 16, 16, 16, None, 16, 16, 1, n, dtype, dtype, dtype, None))
+print(codes)
+assert all(code < 0 for code in codes)  # there is no device to launch on
+"""
+
+
+def test_rows_whose_bytes_pass_32_bits():
+    """Rows of up to 2^30 elements are taken; their bytes pass an int. On a machine without a device (none is visible to the process) such a
+    call ends with an error's code and not with the process."""
+    run = subprocess.run([sys.executable, "-c", LONG_ROWS, os.path.join(ROOT, "flash-linear-attention_b200")], capture_output=True, text=True, timeout=600,
+                         env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
+    assert run.returncode == 0, (run.returncode, run.stdout, run.stderr)
