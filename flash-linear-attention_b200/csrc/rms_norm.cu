@@ -343,7 +343,9 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
 // ---- many rows: a persistent block, rows by bulk copies -----------------------------------------------------------------
 // A group of TPR threads walks rows through a ring of shared-memory stages that its first thread keeps filled, so that loads
 // stay in flight over the reductions and stores of the rows before; a thread holds its columns' weights (and, in backward, their
-// dw) in registers for all its rows.  The barrier of a row's reduction is also the point behind which its stage may be refilled.
+// dw) in registers for all its rows.  The reduction of a row is also the point behind which its stage may be refilled: forward's takes in
+// all that was read of the stage.  Backward's does not take in the stream's gradient, and a row of one warp reduces by shuffles alone,
+// so a barrier of the warp stands there as well.
 __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes),
                "r"(tc::smem_u32(bar))
@@ -512,6 +514,7 @@ template <typename T, typename S, int NV> __global__ void __launch_bounds__(RING
         }
       }
     dot = row_sum(dot, q.tpr, slots[par], GroupSync{q.tpr, group}) / p.n;
+    __syncwarp();  // (all lanes have read ds)
     if (li == 0 && !dead && row + q.stages * stride < p.rows) fill(st, row + q.stages * stride);
     if (++st == q.stages) st = 0, phase ^= 1;
 #pragma unroll

@@ -166,3 +166,23 @@ def test_rows_whose_bytes_pass_32_bits():
     run = subprocess.run([sys.executable, "-c", LONG_ROWS, os.path.join(ROOT, "flash-linear-attention_b200")], capture_output=True, text=True, timeout=600,
                          env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
     assert run.returncode == 0, (run.returncode, run.stdout, run.stderr)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dtype", [(64, BF), (512, BF), (256, F32)])
+def test_one_warp_rows_with_a_gradient_of_the_stream(n, dtype):
+    """Rows of one warp: the stage that holds the stream's gradient is refilled behind all lanes' reads of it. Bit for bit from run to run."""
+    rows = 60000
+    x, dy, ds = (torch.randn(rows, n, device=DEV, generator=torch.Generator(DEV).manual_seed(i)).to(dtype) for i in range(3))
+    r, w = x.flip(0).requires_grad_(True), torch.rand(n, device=DEV, generator=torch.Generator(DEV).manual_seed(4)).to(dtype)
+    first = None
+    for _ in range(4):
+        (dr,) = torch.autograd.grad(rms_norm(x, w, residual=r, prenorm=True), r, (dy, ds))
+        first = dr if first is None else first
+        assert torch.equal(dr, first)
+    s = (x.float() + r.detach().float()).to(dtype).double()
+    rstd = 1 / (s.square().mean(1, keepdim=True) + 1e-6).sqrt()
+    xhat, wd = s * rstd, w.double() * dy.double()
+    d64 = rstd * (wd - xhat * (xhat * wd).mean(1, keepdim=True)) + ds.double()
+    size = rstd * (wd.abs() + xhat.abs() * (xhat * wd).abs().mean(1, keepdim=True)) + ds.double().abs()
+    within("dr", first, d64.cpu(), (96 * U * size + half_step(d64, dtype)).cpu())
