@@ -11,6 +11,7 @@ from contextlib import nullcontext
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -210,6 +211,14 @@ def once(backward):
     """A Function's backward body that is not differentiable itself. The marking (which costs 3 us a call) is only needed where a
     second derivative could be asked for."""
     return once_differentiable(backward) if torch.is_grad_enabled() else backward
+
+
+def dual(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of them carries a forward-mode tangent (with gradients switched off as well). An autograd Function's apply refuses
+    it where it has no such derivative; a plain launch would drop it."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -121,6 +121,13 @@ def _differentiable(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _refuse_derivatives(name, *tensors):
+    if _differentiable(*tensors):
+        raise NotImplementedError(f"{name} has no backward: call it under torch.no_grad()")
+    if _lib.dual(*tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6, prenorm: bool = False, residual_in_fp32: bool = False):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x + residual.
@@ -132,7 +139,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[tor
         raise NotImplementedError("rms_norm: a bias is not built")
     sum_dtype = _check(x, weight, residual, residual_in_fp32)
     same = residual is None and sum_dtype == x.dtype  # the stream is x
-    if _differentiable(x, weight, residual):
+    if _differentiable(x, weight, residual) or _lib.dual(x, weight, residual):
         out = RMSNormFunction.apply(x, weight, residual, float(eps), sum_dtype, prenorm and not same)
         return (out, x) if prenorm and same else out
     y, _, total, _ = _forward(_rows(x), None if weight is None else weight.contiguous(), None if residual is None else _rows(residual), float(eps),
@@ -148,8 +155,7 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Op
     q `[..., n]` float8_e4m3fn and scale `[...]` fp32 stand for q * scale; scale is the row's largest |y| / 448, and 0 for a row of
     zeros. For inference: there is no backward, and a call that would need one is refused."""
     sum_dtype = _check(x, weight, residual, residual_in_fp32)
-    if _differentiable(x, weight, residual):
-        raise NotImplementedError("rms_norm_quant has no backward: call it under torch.no_grad()")
+    _refuse_derivatives("rms_norm_quant", x, weight, residual)
     same = residual is None and sum_dtype == x.dtype
     q, scale, total, _ = _forward(_rows(x), None if weight is None else weight.contiguous(), None if residual is None else _rows(residual), float(eps),
                                   sum_dtype, prenorm and not same, False, quant=True)
@@ -161,8 +167,7 @@ def quantize_rows(x: torch.Tensor):
     """(q float8_e4m3fn of x's shape, scale fp32 of x's leading dimensions): x row by row as q * scale, scale = max|x| / 448. What
     `linear_fp8` takes for weights (`[N, K]`, one scale an output) and for tokens that do not come out of `rms_norm_quant`."""
     _check(x, None, None, False)
-    if _differentiable(x):
-        raise NotImplementedError("quantize_rows has no backward: call it under torch.no_grad()")
+    _refuse_derivatives("quantize_rows", x)
     q, scale, _, _ = _forward(_rows(x), None, None, 0.0, x.dtype, False, False, quant=True, norm=False)
     return _like(q, x.shape), _like(scale, x.shape[:-1])
 

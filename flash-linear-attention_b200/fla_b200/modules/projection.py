@@ -130,7 +130,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         raise ValueError(f"x and weight must both be bfloat16 or both float16, got {x.dtype} and {weight.dtype}")
     _check(x, weight, bias, residual, activation, x.dtype)
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))) or _lib.dual(x, weight, bias, residual):
         return LinearFunction.apply(x, weight, bias, residual, act)
     y, _, _ = _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False)
     return _like(y, x.shape[:-1] + (weight.shape[0],))
@@ -150,6 +150,8 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     _check(x, weight, bias, residual, activation, out_dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, weight_scale, bias, residual)):
         raise NotImplementedError("linear_fp8 has no backward: call it under torch.no_grad()")
+    if _lib.dual(x, x_scale, weight, weight_scale, bias, residual):
+        raise NotImplementedError("linear_fp8 has no forward-mode derivative")
     if x.shape[-1] % 16:
         raise ValueError(f"linear_fp8: K = {x.shape[-1]} must be a multiple of 16")
     x2, w = _rows(x), weight.contiguous()

@@ -110,7 +110,8 @@ def _hgrn(x, g, initial_state, output_final_state, offsets):
     if initial_state is not None and tuple(initial_state.shape) != (N, x.shape[2]):
         raise ValueError(f"The number of initial states is expected to be equal to the number of input sequences, "
                          f"i.e., a shape of {(N, x.shape[2])} rather than {tuple(initial_state.shape)}.")
-    if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or (initial_state is not None and initial_state.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or (initial_state is not None and initial_state.requires_grad))) \
+            or _lib.dual(x, g, initial_state):
         return HGRNFunction.apply(x, g, initial_state, bool(output_final_state), offsets)
     h0 = None if initial_state is None else initial_state.float().contiguous()
     return hgrn_fwd(x.contiguous(), g.contiguous(), h0, bool(output_final_state), offsets)

@@ -186,3 +186,26 @@ def test_one_warp_rows_with_a_gradient_of_the_stream(n, dtype):
     d64 = rstd * (wd - xhat * (xhat * wd).mean(1, keepdim=True)) + ds.double()
     size = rstd * (wd.abs() + xhat.abs() * (xhat * wd).abs().mean(1, keepdim=True)) + ds.double().abs()
     within("dr", first, d64.cpu(), (96 * U * size + half_step(d64, dtype)).cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(10))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(which, grad):
+    """A dual tensor's tangent is never dropped without a word, with and without gradients switched on."""
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(4, 6, 32, generator=gen).to(DEV).to(BF)
+    w = torch.randn(32, 32, generator=gen).to(DEV).to(BF)
+    h0, v = torch.zeros(4, 32, device=DEV), torch.ones(32, device=DEV, dtype=BF)
+    with torch.no_grad():
+        (q, qs), (p, ps) = quantize_rows(x), quantize_rows(w)
+    calls = [lambda d: chunk_hgrn(d(x), -x.abs()), lambda d: chunk_hgrn(x, d(-x.abs())), lambda d: fused_recurrent_hgrn(x, -x.abs(), initial_state=d(h0)),
+             lambda d: rms_norm(d(x), v), lambda d: rms_norm(x, d(v), residual=x), lambda d: rms_norm_quant(x, v, residual=d(x)),
+             lambda d: quantize_rows(d(x)), lambda d: linear(x, d(w)), lambda d: linear(x, w, residual=d(x)),
+             lambda d: linear_fp8(q, d(qs), p, ps)]
+    with torch.set_grad_enabled(grad):
+        calls[which](lambda t: t)
+        with forward_ad.dual_level():
+            calls[which](lambda t: t)  # a level by itself changes nothing
+            with pytest.raises(RuntimeError, match="forward"):
+                calls[which](lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
