@@ -209,3 +209,55 @@ def test_forward_mode_derivatives_are_refused(which, grad):
             calls[which](lambda t: t)  # a level by itself changes nothing
             with pytest.raises(RuntimeError, match="forward"):
                 calls[which](lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+INSTALL = """
+import sys, types
+sys.path.insert(0, sys.argv[1])
+def module(name, **names):
+    m = sys.modules[name] = types.ModuleType(name)
+    m.__dict__.update(names)
+    if "." in name:
+        setattr(sys.modules[name.rpartition(".")[0]], name.rpartition(".")[2], m)
+    return m
+for name in ("fla", "fla.modules", "fla.ops"):
+    module(name).__path__ = []
+module("fla.modules.layernorm", LayerNorm="their LayerNorm", RMSNorm="their RMSNorm")
+module("fla.ops.hgrn", chunk_hgrn="their chunk", other="their other").__path__ = ["/nowhere"]
+module("fla.ops.hgrn.naive", naive_recurrent_hgrn="their loop")
+import fla_b200
+for _ in range(2):  # a second call changes nothing
+    fla_b200.install_as_fla_modules()
+    fla_b200.install_as_fla_ops()
+from fla.modules.layernorm import LayerNorm, RMSNorm, rms_norm
+assert LayerNorm == "their LayerNorm"
+from fla_b200.modules import RMSNorm as ours, rms_norm as own
+assert RMSNorm is ours and rms_norm is own
+import fla.modules.layernorm as by_path
+assert by_path.LayerNorm == LayerNorm and by_path.RMSNorm is ours
+from fla.ops.hgrn import chunk_hgrn, other
+from fla_b200.ops import chunk_hgrn as own
+assert other == "their other" and chunk_hgrn is own
+from fla.ops.hgrn.naive import naive_recurrent_hgrn
+assert naive_recurrent_hgrn == "their loop"
+for bad in ("fla.modules.layernorm", "fla.ops.hgrn"):
+    try:
+        exec(f"from {bad} import nobody_has_this")
+    except ImportError:
+        continue
+    raise SystemExit(bad)
+print("as it should be")
+"""
+
+
+@pytest.mark.parametrize("there", [True, False])
+def test_names_of_a_replaced_module_stay(there):
+    """Installing the package's modules over a `fla` that was imported before keeps the names that this package has no form of its own
+    for; without one, a name that nobody has is an ImportError as ever."""
+    code = INSTALL
+    if not there:
+        code = code[:code.index("def module")] + "import fla_b200\n" + "\n".join(
+            ["fla_b200.install_as_fla_modules()", "fla_b200.install_as_fla_ops()", "from fla.modules.layernorm import RMSNorm",
+             "from fla.ops.hgrn import chunk_hgrn", code[code.index("for bad in"):]])
+    run = subprocess.run([sys.executable, "-c", code, os.path.join(ROOT, "flash-linear-attention_b200")], capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0 and "as it should be" in run.stdout, run.stdout + run.stderr
