@@ -28,11 +28,15 @@ def _like(t: torch.Tensor, shape) -> torch.Tensor:
     return t if t.shape == shape else t.reshape(shape)
 
 
-def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=True):
-    """x2, r2 `[rows, n]` contiguous. Returns (y, scale, sum, rstd), None for what was not asked for."""
+def _forward(x, w, r, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=True):
+    """Returns (y, scale, sum, rstd), None for what was not asked for; y and sum have x's shape from the start, so that outputs of an
+    autograd Function are no views and may be changed in place."""
+    x2, r2 = _rows(x), None if r is None else _rows(r)
+    w = None if w is None else w.contiguous()
     rows, n = x2.shape
-    y = torch.empty_like(x2, dtype=torch.float8_e4m3fn) if quant else torch.empty_like(x2)  # (empty() from sizes takes 1 us longer)
-    total = torch.empty_like(x2, dtype=sum_dtype) if want_sum else None
+    flat = dict(memory_format=torch.contiguous_format)  # (empty() from sizes takes 1 us longer)
+    y = torch.empty_like(x, dtype=torch.float8_e4m3fn, **flat) if quant else torch.empty_like(x, **flat)
+    total = torch.empty_like(x, dtype=sum_dtype, **flat) if want_sum else None
     rstd = x2.new_empty(rows, dtype=torch.float32) if want_rstd else None
     scale = x2.new_empty(rows, dtype=torch.float32) if quant else None
     if rows and n:
@@ -50,6 +54,7 @@ def _forward(x2, w, r2, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=T
 
 def _backward(ctx, dy, dsum=None):
     total, rstd, w = ctx.saved_tensors
+    total = _rows(total)
     rows, n = total.shape
     need_x, need_w, need_r = ctx.needs_input_grad[:3]
     dy = torch.zeros_like(total, dtype=ctx.x_dtype) if dy is None else _rows(dy if dy.dtype == ctx.x_dtype else dy.to(ctx.x_dtype))
@@ -80,16 +85,15 @@ class RMSNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, residual, eps, sum_dtype, prenorm):
-        x2, w = _rows(x), None if weight is None else weight.contiguous()
-        r2 = None if residual is None else _rows(residual)
-        own_sum = r2 is not None or sum_dtype != x.dtype
-        y, _, total, rstd = _forward(x2, w, r2, eps, sum_dtype, own_sum, True)
-        ctx.save_for_backward(total if own_sum else x2, rstd, w)
+        w = None if weight is None else weight.contiguous()
+        own_sum = residual is not None or sum_dtype != x.dtype
+        x = x.contiguous()
+        y, _, total, rstd = _forward(x, w, residual, eps, sum_dtype, own_sum, True)
+        ctx.save_for_backward(total if own_sum else x, rstd, w)
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         ctx.r_dtype = None if residual is None else residual.dtype
         ctx.set_materialize_grads(False)
-        y = _like(y, x.shape)
-        return (y, _like(total, x.shape)) if prenorm else y
+        return (y, total) if prenorm else y
 
     @staticmethod
     def backward(ctx, dy, dsum=None):
@@ -142,10 +146,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[tor
     if _differentiable(x, weight, residual) or _lib.dual(x, weight, residual):
         out = RMSNormFunction.apply(x, weight, residual, float(eps), sum_dtype, prenorm and not same)
         return (out, x) if prenorm and same else out
-    y, _, total, _ = _forward(_rows(x), None if weight is None else weight.contiguous(), None if residual is None else _rows(residual), float(eps),
-                              sum_dtype, prenorm and not same, False)
-    y = _like(y, x.shape)
-    return (y, x if same else _like(total, x.shape)) if prenorm else y
+    y, _, total, _ = _forward(x, weight, residual, float(eps), sum_dtype, prenorm and not same, False)
+    return (y, x if same else total) if prenorm else y
 
 
 def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -157,10 +159,9 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Op
     sum_dtype = _check(x, weight, residual, residual_in_fp32)
     _refuse_derivatives("rms_norm_quant", x, weight, residual)
     same = residual is None and sum_dtype == x.dtype
-    q, scale, total, _ = _forward(_rows(x), None if weight is None else weight.contiguous(), None if residual is None else _rows(residual), float(eps),
-                                  sum_dtype, prenorm and not same, False, quant=True)
-    q, scale = _like(q, x.shape), _like(scale, x.shape[:-1])
-    return (q, scale, x if same else _like(total, x.shape)) if prenorm else (q, scale)
+    q, scale, total, _ = _forward(x, weight, residual, float(eps), sum_dtype, prenorm and not same, False, quant=True)
+    scale = _like(scale, x.shape[:-1])
+    return (q, scale, x if same else total) if prenorm else (q, scale)
 
 
 def quantize_rows(x: torch.Tensor):
@@ -168,8 +169,8 @@ def quantize_rows(x: torch.Tensor):
     `linear_fp8` takes for weights (`[N, K]`, one scale an output) and for tokens that do not come out of `rms_norm_quant`."""
     _check(x, None, None, False)
     _refuse_derivatives("quantize_rows", x)
-    q, scale, _, _ = _forward(_rows(x), None, None, 0.0, x.dtype, False, False, quant=True, norm=False)
-    return _like(q, x.shape), _like(scale, x.shape[:-1])
+    q, scale, _, _ = _forward(x, None, None, 0.0, x.dtype, False, False, quant=True, norm=False)
+    return q, _like(scale, x.shape[:-1])
 
 
 class RMSNorm(nn.Module):

@@ -35,10 +35,11 @@ def _as_is(t: torch.Tensor, n: int) -> bool:
     return n % 8 == 0 and t.data_ptr() % 16 == 0
 
 
-def _forward(x2, w, b, r2, act, want_z):
-    """(y, z or None, the operands' copies or None)"""
+def _forward(x2, w, b, r2, act, want_z, lead):
+    """(y, z or None, the operands' copies or None); y is [*lead, N] from the start, so that the output of an autograd Function is no
+    view and may be changed in place."""
     (M, K), N = x2.shape, w.shape[0]
-    y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
+    y = torch.empty(*lead, N, dtype=x2.dtype, device=x2.device)
     z = torch.empty_like(y) if want_z else None
     copies = None
     if M:
@@ -89,12 +90,12 @@ class LinearFunction(torch.autograd.Function):
         x2, w = _rows(x), weight.contiguous()
         need_x, need_w, need_b, _ = ctx.needs_input_grad[:4]
         y, z, copies = _forward(x2, w, None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act,
-                                act != 0 and (need_x or need_w or need_b))
+                                act != 0 and (need_x or need_w or need_b), x.shape[:-1])
         K = w.shape[1]
         ctx.save_for_backward(x2 if need_w and _as_is(x2, K) else None, w if need_x and _as_is(w, K) else None, z, copies if need_x or need_w else None)
         ctx.places = x2.data_ptr(), w.data_ptr()
         ctx.act, ctx.sizes, ctx.x_shape = act, (x2.shape[0], w.shape[0], K), x.shape
-        return _like(y, x.shape[:-1] + (w.shape[0],))
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -132,8 +133,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     act = ACTIVATIONS[activation]
     if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))) or _lib.dual(x, weight, bias, residual):
         return LinearFunction.apply(x, weight, bias, residual, act)
-    y, _, _ = _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False)
-    return _like(y, x.shape[:-1] + (weight.shape[0],))
+    return _forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual), act, False,
+                    x.shape[:-1])[0]
 
 
 def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -162,7 +163,7 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     b, r2 = None if bias is None else bias.contiguous(), None if residual is None else _rows(residual)
     xs, ws = x_scale.contiguous(), weight_scale.contiguous()
     (M, K), N = x2.shape, w.shape[0]
-    y = torch.empty(M, N, dtype=out_dtype, device=x.device)
+    y = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=x.device)
     if M:
         lib = _lib.load()
         with _lib.device_of(x2):
@@ -171,4 +172,4 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
             rc = lib.flab_linear_e4m3(x2.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), _p(b), _p(r2), y.data_ptr(), M, N, K,
                                       ACTIVATIONS[activation], _DTYPES[out_dtype], _p(scratch), n, _lib.stream_of(x2))
         _lib.finish("flab_linear_e4m3", rc)
-    return _like(y, x.shape[:-1] + (N,))
+    return y

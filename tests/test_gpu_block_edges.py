@@ -261,3 +261,29 @@ def test_names_of_a_replaced_module_stay(there):
              "from fla.ops.hgrn import chunk_hgrn", code[code.index("for bad in"):]])
     run = subprocess.run([sys.executable, "-c", code, os.path.join(ROOT, "flash-linear-attention_b200")], capture_output=True, text=True, timeout=600)
     assert run.returncode == 0 and "as it should be" in run.stdout, run.stdout + run.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(6, 64), (2, 3, 64), (64,), (2, 1, 3, 64)])
+def test_results_may_be_changed_in_place(shape):
+    """As those of nn.Linear may, whatever the number of dimensions."""
+    gen = torch.Generator().manual_seed(3)
+    x, r = (torch.randn(shape, generator=gen).to(DEV).to(BF).requires_grad_(True) for _ in range(2))
+    w = (torch.randn(64, 64, generator=gen) / 8).to(DEV).to(BF).requires_grad_(True)
+    n = torch.ones(64, device=DEV, dtype=BF, requires_grad=True)
+    for make, leaves in ((lambda: linear(x, w, activation="silu"), (x, w)), (lambda: linear(x, w, residual=r), (x, w, r)),
+                         (lambda: rms_norm(x, n), (x, n)), (lambda: rms_norm(x, n, residual=r, prenorm=True)[0], (x, n, r))):
+        y = make()
+        want = torch.autograd.grad(F.silu(y * 2 + 1), leaves, torch.ones_like(y))
+        y = make()
+        y.mul_(2).add_(1)
+        got = torch.autograd.grad(F.silu(y, inplace=True), leaves, torch.ones_like(y))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    y, s = rms_norm(x, n, residual=r, prenorm=True)
+    assert s.shape == x.shape and y.shape == x.shape
+    s += y  # the next block's stream; backward of this norm reads s, so as with any sum that is read again it is not asked for here
+    with torch.no_grad():
+        y = linear(x, w)
+        y += 1
+        assert y.shape == shape
