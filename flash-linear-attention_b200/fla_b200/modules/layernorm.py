@@ -155,7 +155,7 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Op
     """`rms_norm` with an 8-bit output for `linear_fp8`: (q, scale) or, with `prenorm`, (q, scale, s).
 
     q `[..., n]` float8_e4m3fn and scale `[...]` fp32 stand for q * scale; scale is the row's largest |y| / 448, and 0 for a row of
-    zeros. For inference: there is no backward, and a call that would need one is refused."""
+    zeros. (Where that lies below fp32's normal numbers it is 2^-126 for 16-bit x, and rounded up for fp32 x.) For inference: there is no backward, and a call that would need one is refused."""
     sum_dtype = _check(x, weight, residual, residual_in_fp32)
     _refuse_derivatives("rms_norm_quant", x, weight, residual)
     same = residual is None and sum_dtype == x.dtype

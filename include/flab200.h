@@ -129,7 +129,8 @@ int flab_rms_norm_swish_gate_bwd(const void *x, const void *gate, const float *w
 /* ---- RMS norm with the residual's addition, 16 / 32-bit or e4m3 output (the step that opens a block) ----
  * Replaces rms_norm of fla/modules/layernorm.py (weight, no bias) and adds an 8-bit output:
  *   s = round(x + residual) in sum_dtype;  y = s rstd weight,  rstd = 1 / sqrt(mean_n s^2 + eps)
- *   FLAB_NORM_E4M3: y holds e4m3 bytes q = round(y / scale) instead, scale [rows] fp32 = max_n |y| / 448 (0 for a row of zeros)
+ *   FLAB_NORM_E4M3: y holds e4m3 bytes q = round(y / scale) instead, scale [rows] fp32 = max_n |y| / 448 (0 for a row of zeros; not
+ *                   below 2^-126 for 16-bit x, rounded up below it for fp32 x)
  *   FLAB_NORM_NONE (with FLAB_NORM_E4M3): no norm, the rows of x are quantised as they are
  * x, y: [rows, n] contiguous of type dtype; residual (or NULL) of type dtype or fp32; sum (or NULL: not wanted) of type sum_dtype =
  * dtype or fp32 (fp32 where the residual is); weight [n] of type weight_dtype or NULL (ones); rstd [rows] fp32 or NULL.

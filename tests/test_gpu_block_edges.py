@@ -287,3 +287,41 @@ def test_results_may_be_changed_in_place(shape):
         y = linear(x, w)
         y += 1
         assert y.shape == shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FH, F32])
+@pytest.mark.parametrize("n", [512, 33])
+def test_rows_with_tiny_largest_values(dtype, n):
+    """q scale stands for the row down to the smallest numbers: half a step of e4m3, 2^-4 of the value or 2^-10 of the scale, whatever the
+    scale is. (Below 448 2^-126 a scale of fp32 has few bits; it may be larger than max|y| / 448, and never smaller by more than a rounding.)"""
+    tops = [2.0 ** e * f for e in range(-148, -100, 3) for f in (1.0, 1.3)] + [448 * 2.0 ** -126 * f for f in (0.99, 1.0, 1.01)] + [1e-37, 1e-42, 600 * 2.0 ** -149]
+    if dtype == FH:
+        tops = [2.0 ** e * f for e in range(-24, -10, 2) for f in (1.0, 1.5)]
+    gen = torch.Generator().manual_seed(n)
+    y = torch.rand(len(tops), n, generator=gen) * 2 - 1
+    y[:, 0] = 1
+    y = (y.double() * torch.tensor(tops, dtype=torch.float64)[:, None]).float().to(dtype)
+    check_tiny(*quantize_rows(y.to(DEV)), y.double())
+    # the norm of ordinary rows with a tiny weight
+    x = torch.randn(len(tops), n, generator=gen).to(dtype)
+    for top in (tops[2], tops[-1], tops[len(tops) // 2]):
+        w = torch.full((n,), top, dtype=F32)
+        y = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+        # the products are rounded to fp32, subnormal ones to 2^-149
+        check_tiny(*rms_norm_quant(x.to(DEV), w.to(DEV)), y, 96 * U * y.abs() + 2.0 ** -149)
+    # enough rows for the streaming form, which holds rows of 16-byte vectors
+    x = torch.randn(16000, 512, generator=gen).to(dtype)
+    w = torch.full((512,), 2.0 ** -130, dtype=F32)
+    y = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+    check_tiny(*rms_norm_quant(x.to(DEV), w.to(DEV)), y, 96 * U * y.abs() + 2.0 ** -149)
+
+
+def check_tiny(q, scale, y, error=0.0):
+    q, scale = q.cpu().double(), scale.cpu().double()[:, None]
+    top = y.abs().amax(1, keepdim=True)
+    assert torch.isfinite(q).all() and ((scale > 0) | (top <= 2.0 ** -149)).all()
+    assert (scale * (1 + 4 * U) * 448 >= top * (1 - 100 * U) - 2.0 ** -149).all()
+    step = torch.maximum(y.abs() * 2.0 ** -4, scale * 2.0 ** -10)
+    over = ((q * scale - y).abs() - (step * (1 + 200 * U) + 200 * U * y.abs() + error)).max().item()
+    assert over <= 0, over
