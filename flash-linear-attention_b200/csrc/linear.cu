@@ -50,9 +50,11 @@ __device__ __forceinline__ float act_slope(float z, int act) {
       const float s = sigmoid(z);
       return fmaf(z, fmaf(-s, s, s), s);
     }
-    case ACT_SIGMOID: {
-      const float s = sigmoid(z);
-      return fmaf(-s, s, s);
+    case ACT_SIGMOID: {  // e / (1 + e)^2 with e = e^-|z|: s - s^2 would cancel where s is near 1
+      float e, s;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(z) * -1.4426950408889634f));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+      return e * s * s;
     }
     case ACT_LOGSIGMOID: return sigmoid(-z);
     case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);

@@ -325,3 +325,25 @@ def check_tiny(q, scale, y, error=0.0):
     step = torch.maximum(y.abs() * 2.0 ** -4, scale * 2.0 ** -10)
     over = ((q * scale - y).abs() - (step * (1 + 200 * U) + 200 * U * y.abs() + error)).max().item()
     assert over <= 0, over
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["sigmoid", "logsigmoid", "silu"])
+def test_slopes_far_out(act):
+    """dz = act'(z) dy where z is exact (a product with one term): the slope to within 2^-18 of itself, or of z's part in it where it is a
+    sum, on both sides of zero, and its rounding and that of dx."""
+    z = torch.arange(-20, 20.25, 0.25).to(BF)
+    x = torch.zeros(len(z), 8, dtype=BF)
+    x[:, 0] = z
+    w = torch.zeros(8, 8, dtype=BF)
+    w[0, 0] = 1
+    xs = x.to(DEV).requires_grad_(True)
+    y = linear(xs, w.to(DEV), activation=act)
+    (dx,) = torch.autograd.grad(y, xs, torch.ones_like(y))
+    Z = z.double().requires_grad_(True)
+    (want,) = torch.autograd.grad(ACTIVATIONS[act](Z).sum(), Z)
+    s = torch.sigmoid(-Z.detach().abs())
+    own = want.abs() if act != "silu" else want.abs() + (1 + Z.detach().abs()) * torch.sigmoid(Z.detach())
+    bound = 2.0 ** -18 * own + 2.02 * half_step(want, BF)
+    assert (s > 0).all()
+    within("dz", dx[:, 0], want, bound)
