@@ -259,12 +259,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         if (!two) {
           if (b > 0 && lane == 0) {
             tc::tma_store_wait_read();  // of block b - 1
-            if (EPI && p.res) ask(b);
+            if (EPI && p.res && ok) ask(b);
           }
         } else if (EPI && p.res) {
           if (b + 1 < BLOCKS && lane == 0) {
             tc::tma_store_wait_read();  // of block b - 1, a block's work ago
-            ask(b + 1);
+            if (ok) ask(b + 1);  // (behind a wait that ran out nothing is asked for, so that no copy is in flight when the kernel ends)
           }
         } else {
           if (lane == 0) tc::tma_store_wait_read_but_one();  // of block b - 2
@@ -341,7 +341,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         if (EPI && p.res) {
           if (ok) {
             ok = tc::mbar_wait(&res_full[w][q], (seen >> q) & 1);
-            if (!ok) tu_tc_error = 734;
+            if (!ok) {
+              tu_tc_error = 734;
+              if (two && b + 1 < BLOCKS) tc::mbar_wait(&res_full[w][q ^ 1], (seen >> (q ^ 1)) & 1);  // the next block's is on its way
+            }
             seen ^= 1u << q;
           }
 #pragma unroll
@@ -510,10 +513,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmShape<BN>::THREA
         store(p.c, [](float y) { return Num<TO>::t(y); });
         __syncwarp();
         now = next;
-      }
-      if (side >= BN / 32) {  // no block of this tile is this warp's
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive_peer(tc::peer_addr(&acc_empty[half], 0));
       }
     }
   }
