@@ -213,6 +213,11 @@ def once(backward):
     return once_differentiable(backward) if torch.is_grad_enabled() else backward
 
 
+def saved(ctx) -> list:
+    """The saved tensors as the kernels read them: a hook may have brought them back with other strides."""
+    return [t if t is None else t.contiguous() for t in ctx.saved_tensors]
+
+
 def dual(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether one of them carries a forward-mode tangent (with gradients switched off as well). An autograd Function's apply refuses
     it where it has no such derivative; a plain launch would drop it."""

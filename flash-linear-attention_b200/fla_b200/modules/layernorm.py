@@ -53,7 +53,7 @@ def _forward(x, w, r, eps, sum_dtype, want_sum, want_rstd, quant=False, norm=Tru
 
 
 def _backward(ctx, dy, dsum=None):
-    total, rstd, w = ctx.saved_tensors
+    total, rstd, w = _lib.saved(ctx)
     total = _rows(total)
     rows, n = total.shape
     need_x, need_w, need_r = ctx.needs_input_grad[:3]

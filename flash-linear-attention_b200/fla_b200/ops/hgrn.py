@@ -61,7 +61,7 @@ def hgrn_bwd(g, o, h0, do, dht, want_dh0, cu):
 
 
 def _backward(ctx, do, dht):
-    g, o, h0, cu = ctx.saved_tensors
+    g, o, h0, cu = _lib.saved(ctx)
     do = torch.zeros_like(g) if do is None else do.to(g.dtype).contiguous()
     dht = None if dht is None else dht.float().contiguous()
     dx, dg, dh0 = hgrn_bwd(g, o, h0, do, dht, ctx.needs_input_grad[2], cu)

@@ -347,3 +347,44 @@ def test_slopes_far_out(act):
     bound = 2.0 ** -18 * own + 2.02 * half_step(want, BF)
     assert (s > 0).all()
     within("dz", dx[:, 0], want, bound)
+
+
+class Elsewhere(torch.autograd.graph.saved_tensors_hooks):
+    """Saved tensors that come back with other strides, or at an address of two bytes behind a 16-byte boundary."""
+
+    def __init__(self, strided):
+        def pack(t):
+            return t.detach().clone()
+
+        def unpack(t):
+            if strided and t.dim() > 1:
+                return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+            flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+            return flat.view(t.shape).copy_(t)
+
+        super().__init__(pack, unpack)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("strided", [True, False])
+@pytest.mark.parametrize("D", [64, 33])
+def test_saved_tensors_that_come_back_otherwise(D, strided):
+    """A hook may bring saved tensors back in any layout: the gradients are those without it, up to the order of fp32 sums."""
+    gen = torch.Generator().manual_seed(D)
+    x, r, dy = (torch.randn(3, 50, D, generator=gen).to(DEV).to(BF) for _ in range(3))
+    w = (torch.randn(D, D, generator=gen) * D ** -0.5).to(DEV).to(BF)
+    n, h0 = torch.rand(D, generator=gen).to(DEV).to(BF), torch.randn(3, D, generator=gen).to(DEV)
+    for t in (x, r, w, n, h0):
+        t.requires_grad_(True)
+    cases = [(lambda: linear(x, w, activation="silu"), (x, w)), (lambda: linear(x, w, residual=r), (x, w, r)),
+             (lambda: rms_norm(x, n, residual=r), (x, n, r)), (lambda: rms_norm(x, n, residual=r, residual_in_fp32=True), (x, n, r)),
+             (lambda: chunk_hgrn(x, -r.abs(), initial_state=h0)[0], (x, r, h0)), (lambda: fused_recurrent_hgrn(x[:, :9], -r[:, :9].abs())[0], (x, r))]
+    for make, of in cases:
+        y = make()
+        g = dy[:, :y.shape[1]]
+        want = torch.autograd.grad(y, of, g)
+        with Elsewhere(strided):
+            y = make()
+        for a, b in zip(torch.autograd.grad(y, of, g), want):
+            a, b = a.double(), b.double()
+            assert ((a - b).abs() <= 2.02 * half_step(b, BF) + 2.0 ** -14 * b.abs().max()).all()
