@@ -150,7 +150,7 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
         if s.dtype != torch.float32 or s.shape != shape or s.device != x.device:
             raise ValueError(f"{name} must be {tuple(shape)} in float32 on {x.device}, got {s.dtype} {tuple(s.shape)} on {s.device}")
     _check(x, weight, bias, residual, activation, out_dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, weight_scale, bias, residual)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, x_scale, weight, weight_scale, bias, residual)):
         raise NotImplementedError("linear_fp8 has no backward: call it under torch.no_grad()")
     if _lib.dual(x, x_scale, weight, weight_scale, bias, residual):
         raise NotImplementedError("linear_fp8 has no forward-mode derivative")

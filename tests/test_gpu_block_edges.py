@@ -388,3 +388,15 @@ def test_saved_tensors_that_come_back_otherwise(D, strided):
         for a, b in zip(torch.autograd.grad(y, of, g), want):
             a, b = a.double(), b.double()
             assert ((a - b).abs() <= 2.02 * half_step(b, BF) + 2.0 ** -14 * b.abs().max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["x", "weight"])
+def test_eight_bit_operands_that_ask_for_a_gradient(which):
+    q, v = (torch.zeros(n, 32, device=DEV).to(torch.float8_e4m3fn) for n in (4, 8))
+    one = [torch.ones(n, device=DEV) for n in (4, 8)]
+    (q if which == "x" else v).requires_grad_(True)
+    with pytest.raises(NotImplementedError, match="no backward"):
+        linear_fp8(q, one[0], v, one[1])
+    with torch.no_grad():
+        assert linear_fp8(q, one[0], v, one[1]).shape == (4, 8)
