@@ -83,6 +83,11 @@ __device__ __forceinline__ int row_code(const HgrnParams &p, long long t) {
 // infinity.  Gates are exponentials, so no other factor has a sign; one that underflowed to +0 still hands a NaN on.
 #define CUT (-0.f)
 __device__ __forceinline__ bool is_cut(float P) { return __float_as_uint(P) == 0x80000000u; }
+// The factor of a map with factor `a` and one with factor `b` behind it.  A cut stays one: a product with it would make a NaN where gates
+// above 1 have overflowed.  (Only sequences that are packed have cuts.)
+template <bool VAR> __device__ __forceinline__ float behind(float a, float b) {
+  return VAR && (int)(__float_as_uint(a) | __float_as_uint(b)) < 0 ? CUT : a * b;
+}
 // e^g as 2^(g log2 e): the product's rounding moves the result by |g| 2^-24 of itself, less than the exponential's own error
 // wherever the gate is near 1 and errors live long.
 __device__ __forceinline__ float gate(float g) {
@@ -197,6 +202,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
   // the warp's own map
   const float *edge = BWD ? p.dht : p.h0;  // value in front of a sequence, in scan order
   float a[R][V], P[V], Q[V];
+  bool cut = false;
 #pragma unroll
   for (int j = 0; j < V; ++j) P[j] = 1.f, Q[j] = 0.f;
 #pragma unroll
@@ -207,8 +213,9 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
       const int code = sCode[t];
       live = live && !(code & ROW_OUT);
       if (code & (ROW_OUT | (BWD ? ROW_END : ROW_START))) {
+        cut = true;
 #pragma unroll
-        for (int j = 0; j < V; ++j) P[j] = CUT, Q[j] = (code & ROW_OUT) || !edge || !on ? 0.f : edge[(size_t)(code >> ROW_SHIFT) * p.D + ch + j];
+        for (int j = 0; j < V; ++j) Q[j] = (code & ROW_OUT) || !edge || !on ? 0.f : edge[(size_t)(code >> ROW_SHIFT) * p.D + ch + j];
       }
     }
 #pragma unroll
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
     }
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) sP[w][lane * V + j] = P[j], sQ[w][lane * V + j] = Q[j];
+  for (int j = 0; j < V; ++j) sP[w][lane * V + j] = VAR && cut ? CUT : P[j], sQ[w][lane * V + j] = Q[j];
   __syncthreads();
 
   auto joined = [&](int j) -> float2 {  // the tile's map of channel j of this lane
@@ -229,7 +236,7 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
     for (int i = 0; i < W; ++i) {
       const float Pi = sP[i][lane * V + j];
       jQ = through(Pi, sQ[i][lane * V + j], jQ);
-      jP = is_cut(Pi) ? CUT : jP * Pi;
+      jP = behind<VAR>(jP, Pi);
     }
     return make_float2(jP, jQ);
   };
@@ -387,10 +394,10 @@ struct Map2 {
   float2 P, Q;
 };
 __device__ __forceinline__ float2 through(const Map2 &m, float2 c) { return make_float2(through(m.P.x, m.Q.x, c.x), through(m.P.y, m.Q.y, c.y)); }
-__device__ __forceinline__ Map2 join(const Map2 &a, const Map2 &b) {
+template <bool VAR> __device__ __forceinline__ Map2 join(const Map2 &a, const Map2 &b) {
   Map2 m;
   m.Q = through(b, a.Q);
-  m.P = make_float2(is_cut(b.P.x) ? CUT : a.P.x * b.P.x, is_cut(b.P.y) ? CUT : a.P.y * b.P.y);
+  m.P = make_float2(behind<VAR>(a.P.x, b.P.x), behind<VAR>(a.P.y, b.P.y));
   return m;
 }
 
@@ -476,6 +483,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       } else {
         // kept short: unrolled, this rarely run code cost more in instruction fetches than it saved
         const int ch = sh.at[s].cg * C + lane * 2;
+        bool cut = false;
 #pragma unroll 1
         for (int r = 0; r < R; ++r) {
           const float2 g = unpack2(gs + row(w, r) * C), x = unpack2(xs + row(w, r) * C);
@@ -484,12 +492,13 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
             const int code = __shfl_sync(0xffffffffu, mine, r);
             out = code & ROW_OUT;
             if (code & (ROW_OUT | AHEAD)) {
-              P = make_float2(CUT, CUT);
+              cut = true;
               Q = out || !edge || ch >= p.D ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2 *>(edge + (size_t)(code >> ROW_SHIFT) * p.D + ch);
             }
           }
           if (!out) take(g, x);
         }
+        if (cut) P = make_float2(CUT, CUT);
       }
       st.P[w][lane] = P;
       st.Q[w][lane] = Q;
@@ -599,8 +608,8 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         return m;
       };
       // the tile's map, by halves: what other tiles wait for goes out first
-      const Map2 tile = join(join(join(rows_map(0), rows_map(1)), join(rows_map(2), rows_map(3))),
-                             join(join(rows_map(4), rows_map(5)), join(rows_map(6), rows_map(7))));
+      const Map2 tile = join<VAR>(join<VAR>(join<VAR>(rows_map(0), rows_map(1)), join<VAR>(rows_map(2), rows_map(3))),
+                                  join<VAR>(join<VAR>(rows_map(4), rows_map(5)), join<VAR>(rows_map(6), rows_map(7))));
       if (before < G - 1 && z.step + 1 < p.nT) {
         put(words(p.maps, z.step), map_word(tile.P.x, tile.Q.x));
         put(words(p.maps, z.step) + 1, map_word(tile.P.y, tile.Q.y));
@@ -620,7 +629,7 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         for (int i = 1; i < W; ++i) {
           const Map2 own = rows_map(i);
           st.P[i][lane] = to.P, st.Q[i][lane] = to.Q;
-          if (i + 1 < W) to = join(to, own);
+          if (i + 1 < W) to = join<VAR>(to, own);
         }
       }
       const long long asked = clock64();
@@ -657,7 +666,8 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
         m.Q = i < before ? make_float2(x.y, y.y) : make_float2(0.f, 0.f);
         return m;
       };
-      const Map2 group_map = join(join(join(tile_map(0), tile_map(1)), join(tile_map(2), tile_map(3))), join(join(tile_map(4), tile_map(5)), tile_map(6)));
+      const Map2 group_map = join<VAR>(join<VAR>(join<VAR>(tile_map(0), tile_map(1)), join<VAR>(tile_map(2), tile_map(3))),
+                                       join<VAR>(join<VAR>(tile_map(4), tile_map(5)), tile_map(6)));
       float2 c = make_float2(0.f, 0.f);
       if (group > 0) {
         c = make_float2(end_of(await<false>(ends, e[0], p.abort)), end_of(await<false>(ends + 1, e[1], p.abort)));

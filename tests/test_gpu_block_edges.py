@@ -400,3 +400,27 @@ def test_eight_bit_operands_that_ask_for_a_gradient(which):
         linear_fp8(q, one[0], v, one[1])
     with torch.no_grad():
         assert linear_fp8(q, one[0], v, one[1]).shape == (4, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 63])
+def test_products_of_gates_that_overflow_behind_an_edge(D):
+    """A sequence that holds nothing stays at nothing, although the products of its gates overflow and the sequence before it ended in
+    something; in backward the same in front of a sequence's end."""
+    lengths = [1500, 1700, 90]
+    T = sum(lengths)
+    off = torch.tensor([0, 1500, 3200, T], device=DEV)
+    gen = torch.Generator().manual_seed(0)
+    x, g = torch.randn(T, D, generator=gen), -torch.rand(T, D, generator=gen)
+    x[1500:3200] = 0
+    g[1500:3200] = 60
+    do = torch.randn(T, D, generator=gen)
+    do[1500:3200] = 0
+    xs, gs = (v.to(DEV).view(1, T, D).requires_grad_(True) for v in (x, g))
+    o, ht = chunk_hgrn(xs, gs, output_final_state=True, offsets=off)
+    dht = torch.ones(3, D, device=DEV)
+    dht[1] = 0
+    dx, dg = torch.autograd.grad([o, ht], [xs, gs], [do.to(DEV).view_as(o), dht])
+    for v in (o, dx, dg):
+        assert torch.isfinite(v).all() and (v[0, 1500:3200] == 0).all() and (v[0, :1500] != 0).any() and (v[0, 3200:] != 0).any()
+    assert torch.isfinite(ht).all() and (ht[1] == 0).all()
