@@ -267,6 +267,7 @@ struct NormBwdParams {
   float *part;
   long long rows;
   int n, tpr, w_type;
+  int in_place;  // rows too long for shared memory: dw is summed in the partial row itself
 };
 
 // one partial row of dw a block; the block's groups of TPR threads take rows in turn
@@ -277,10 +278,16 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
   constexpr int KEEP = NV ? NV : 1;
   const int loops = NV ? NV : (p.n + V * p.tpr - 1) / (V * p.tpr);
   float acc[KEEP][V] = {};
-  if (!NV && p.part) {  // rows too long for registers: the thread's columns are its own in shared memory
+  // rows too long for registers: the thread's columns are its own in shared memory, or in its block's partial row (one group a block)
+  float *const own = p.part + (size_t)blockIdx.x * p.n;
+  if (!NV && p.part) {
     for (int k = 0; k < loops; ++k)
-      for (int j = 0; j < V; ++j)
-        if ((k * p.tpr + li) * V < p.n) sdw[(k * p.tpr + li) * V + j] = 0.f;
+      for (int j = 0; j < V; ++j) {
+        const int c = (k * p.tpr + li) * V + j;
+        if (c >= p.n) continue;
+        if (p.in_place) own[c] = 0.f;
+        else sdw[c] = 0.f;
+      }
   }
   int par = 0;
   for (long long r0 = (long long)blockIdx.x * groups; r0 < p.rows; r0 += (long long)gridDim.x * groups, par ^= 1) {
@@ -314,6 +321,7 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
           const float xh = Num<S>::f(s[i].v[j]) * rstd, d = Num<T>::f(dy[i].v[j]);
           dot = fmaf(xh, w[j] * d, dot);
           if (NV) acc[i][j] = fmaf(d, xh, acc[i][j]);
+          else if (p.in_place) own[c + j] = fmaf(d, xh, own[c + j]);
           else if (p.part) sdw[c + j] = fmaf(d, xh, sdw[c + j]);
         }
       }
@@ -334,7 +342,7 @@ template <typename T, typename S, int V, int NV> __global__ void __launch_bounds
         if (p.dr) store_f<S, V>(p.dr, base + c, d);
       }
   }
-  if (!p.part) return;
+  if (!p.part || (!NV && p.in_place)) return;
   if (NV) {
     for (int k = 0; k < (NV ? NV : 0); ++k) {
       const int c = (k * p.tpr + li) * V;
@@ -723,8 +731,9 @@ template <typename T, typename S> int launch_norm_bwd(NormBwdParams p, cudaStrea
   const NormBwdPlan q = norm_bwd_plan(p.rows, p.n, sizeof(T), by);
   p.tpr = q.tpr;
   parts = q.grid;
-  const size_t bytes = p.part ? (size_t)(q.block / q.tpr) * p.n * sizeof(float) : 0;
-  FLAB_REQUIRE(bytes <= 227 * 1024 - 1024, FLAB_E_UNSUPPORTED, "rms_norm_bwd: rows of %d elements are not supported", p.n);
+  size_t bytes = p.part ? (size_t)(q.block / q.tpr) * p.n * sizeof(float) : 0;
+  // (from 57857 elements on, at four bytes a column; what fits registers is far below: 16384 columns)
+  if (bytes > 227 * 1024 - 1024) p.in_place = 1, bytes = 0;
 #define FLAB_NORM(VV, NN)                                                                                                                   \
   do {                                                                                                                                      \
     auto kernel = rms_norm_bwd_kernel<T, S, VV, NN>;                                                                                        \
@@ -812,7 +821,7 @@ int flab_rms_norm_bwd(const void *sum, const void *dy, const void *dsum, const v
   int parts = 0;
   if (rows > 0) {
     FLAB_REQUIRE(sum && dy && rstd && (dx || dresidual || dweight), FLAB_E_BADARG, "rms_norm_bwd needs sum, dy, rstd and an output");
-    NormBwdParams p = {sum, dy, dsum, weight, rstd, dx, dresidual, dweight ? dw_partial : nullptr, rows, n, 0, weight_dtype};
+    NormBwdParams p = {sum, dy, dsum, weight, rstd, dx, dresidual, dweight ? dw_partial : nullptr, rows, n, 0, weight_dtype, 0};
     const bool wide = sum_dtype == FLAB_FP32;
     int rc;
     switch (dtype) {

@@ -424,3 +424,25 @@ def test_products_of_gates_that_overflow_behind_an_edge(D):
     for v in (o, dx, dg):
         assert torch.isfinite(v).all() and (v[0, 1500:3200] == 0).all() and (v[0, :1500] != 0).any() and (v[0, 3200:] != 0).any()
     assert torch.isfinite(ht).all() and (ht[1] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(1, 57856), (3, 57856), (300, 57856), (1, 57857), (3, 57857), (300, 57857), (300, 70000), (1, 300001), (3, 300001)])
+def test_the_weight_gradient_of_long_rows(rows, n):
+    """Sums over the rows that shared memory holds (57856 columns), and longer ones, with rows for more than one turn of every block."""
+    gen = torch.Generator().manual_seed(n)
+    x, dy = torch.randn(rows, n, generator=gen), torch.randn(rows, n, generator=gen)
+    for dtype, wdtype in ((BF, F32), (F32, F32), (FH, FH)):
+        w = (1 + 0.1 * torch.randn(n, generator=gen)).to(wdtype)
+        xs, ws = x.to(dtype).to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+        dx, dw = torch.autograd.grad(rms_norm(xs, ws), (xs, ws), dy.to(dtype).to(DEV))
+        X, D, W = x.to(dtype).double(), dy.to(dtype).double(), w.double()
+        rstd = 1 / (X.square().mean(1, keepdim=True) + 1e-6).sqrt()
+        xhat = X * rstd
+        # a thread adds n / 1024 values in turn, then the tree: 293 + 10 + a handful
+        adds = (n / 1024 + 30) * U
+        want = (D * xhat).sum(0)
+        within("dw", dw, want, (adds + rows * U) * (D * xhat).abs().sum(0) + half_step(want, wdtype))
+        want = rstd * (W * D - xhat * (xhat * W * D).mean(1, keepdim=True))
+        size = rstd * ((W * D).abs() + xhat.abs() * (xhat * W * D).abs().mean(1, keepdim=True))
+        within("dx", dx, want, adds * size + half_step(want, dtype))
