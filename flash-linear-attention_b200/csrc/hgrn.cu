@@ -48,6 +48,7 @@ struct HgrnParams {
   int cu64;
   int B, D, N;
   int nT, nCG;       // tiles along time, channel groups
+  int share;         // of the sequences, looked through for empty ones by each tile along time
   long long T;
   int *ticket;
   int *abort;                // set by a wait of this launch that ran out
@@ -340,8 +341,8 @@ __global__ void __launch_bounds__(W * 32, 2) hgrn_tile_kernel(const HgrnParams p
     }
   }
   // empty sequences hand their edge value through
-  if (VAR && p.ht && step == 0 && on) {
-    for (int n = w; n < p.N; n += W)
+  if (VAR && p.ht && on) {
+    for (int n = step * p.share + w, to = min(step * p.share + p.share, p.N); n < to; n += W)
       if (cu_at(p, n) >= cu_at(p, n + 1)) {
 #pragma unroll
         for (int j = 0; j < V; ++j) p.ht[(size_t)n * p.D + ch + j] = edge ? edge[(size_t)n * p.D + ch + j] : 0.f;
@@ -387,6 +388,13 @@ template <int L> __device__ __forceinline__ void tile_codes(const HgrnParams &p,
     }
     if (!__all_sync(0xffffffffu, inside)) break;
   }
+}
+
+// Empty sequences, where there are more of them than tokens: a warp each.
+__global__ void __launch_bounds__(256) hgrn_empty_kernel(const HgrnParams p, const float *edge) {
+  for (int n = blockIdx.x * 8 + (threadIdx.x >> 5); n < p.N; n += gridDim.x * 8)
+    if (cu_at(p, n) >= cu_at(p, n + 1))
+      for (int ch = threadIdx.x & 31; ch < p.D; ch += 32) p.ht[(size_t)n * p.D + ch] = edge ? edge[(size_t)n * p.D + ch] : 0.f;
 }
 
 // maps of two channels, one after the other (`a` first)
@@ -575,8 +583,8 @@ __global__ void __launch_bounds__(Stream<T, R, S, BWD>::THREADS, 1)
       }
       // rows past T are the identity, so the last warp's last value is the sequence's
       if (!VAR && z.step == p.nT - 1 && w == W - 1 && p.ht && on) *reinterpret_cast<float2 *>(p.ht + (size_t)z.b * p.D + ch) = c;
-      if (VAR && p.ht && z.step == 0 && on) {  // empty sequences hand their edge value through
-        for (int n = w; n < p.N; n += W)
+      if (VAR && p.ht && on) {  // empty sequences hand their edge value through
+        for (int n = z.step * p.share + w, to = min(z.step * p.share + p.share, p.N); n < to; n += W)
           if (cu_at(p, n) >= cu_at(p, n + 1))
             *reinterpret_cast<float2 *>(p.ht + (size_t)n * p.D + ch) = edge ? *reinterpret_cast<const float2 *>(edge + (size_t)n * p.D + ch) : none;
       }
@@ -875,6 +883,20 @@ int hgrn_scratch(HgrnParams &p, const HgrnPlan &q, void *ws, size_t ws_bytes, cu
   return FLAB_OK;
 }
 
+// Which sequences the tiles look through.  One by one they take a tile's warps 0.1 us each (4 million by a single tile 350 ms, and a wait
+// that runs out is not far), so every tile along time takes a share; and where that is more than two a token, so that most are
+// empty, a kernel of their own looks through all.
+int share_of(const HgrnParams &p, int L) {
+  const long long share = ((long long)p.N + p.nT - 1) / p.nT;
+  return !p.ht || share > 2 * L ? 0 : (int)share;
+}
+template <bool BWD> int pass_empty(const HgrnParams &p, cudaStream_t st) {
+  if (!p.cu || !p.ht || p.share) return FLAB_OK;
+  const long long blocks = ((long long)p.N + 7) / 8, most = sm_count() * 8ll;
+  hgrn_empty_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(p, BWD ? p.dht : p.h0);
+  return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+}
+
 template <typename T, bool BWD, bool VAR, int V> int launch_hgrn(HgrnParams p, void *ws, size_t ws_bytes, cudaStream_t st) {
   typedef HgrnTile<T> Z;
   const HgrnPlan q = hgrn_plan(p.B, p.T, p.D, V, Z::L);
@@ -883,8 +905,10 @@ template <typename T, bool BWD, bool VAR, int V> int launch_hgrn(HgrnParams p, v
     const int rc = hgrn_scratch(p, q, ws, ws_bytes, st);
     if (rc) return rc;
   }
+  p.share = share_of(p, Z::L);
   hgrn_tile_kernel<T, V, Z::W, Z::R, BWD, VAR><<<(unsigned)q.tiles, Z::W * 32, 0, st>>>(p);
-  return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+  const int rc = check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+  return rc ? rc : pass_empty<BWD>(p, st);
 }
 
 template <typename T, bool BWD> struct StreamOf {  // 32 KB (48 KB) of inputs a stage, as many stages as an SM holds
@@ -913,8 +937,10 @@ int launch_stream(HgrnParams p, void *ws, size_t ws_bytes, cudaStream_t st) {
   if ((rc = set_smem(kernel, bytes))) return rc;
   const int sms = sm_count();
   const long long grid = q.tiles < sms ? q.tiles : sms;
+  p.share = share_of(p, Z::L);
   kernel<<<(unsigned)grid, Z::THREADS, bytes, st>>>(p, m[0], m[1], m[2], m[3], m[4]);
-  return check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+  rc = check_launch(BWD ? "hgrn_bwd" : "hgrn_fwd");
+  return rc ? rc : pass_empty<BWD>(p, st);
 }
 
 // Fixed-length sequences of up to WALK tokens are walked by one thread a channel group instead of being put into tiles, which they
@@ -939,6 +965,10 @@ template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws,
     tma = tma && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   }
   for (const float *q : {p.h0, p.dht, (const float *)p.ht}) tma = tma && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  // The streaming form walks all sequences that lie in a tile, 32 in 0.5 us, and a million empty ones may lie in one; more of them go by the
+  // tile form, which searches for each row's.  (A run of 4 million took 350 ms; past them in steps that double, the code that does it
+  // cost every packed call 2 %.)
+  if (p.cu && p.N > 1 << 20) tma = false;
   constexpr int WIDE = 16 / sizeof(T);
   bool wide = tma && p.D % WIDE == 0;
   for (const float *q : {p.h0, p.dht, (const float *)p.ht}) {

@@ -446,3 +446,37 @@ def test_the_weight_gradient_of_long_rows(rows, n):
         want = rstd * (W * D - xhat * (xhat * W * D).mean(1, keepdim=True))
         size = rstd * ((W * D).abs() + xhat.abs() * (xhat * W * D).abs().mean(1, keepdim=True))
         within("dx", dx, want, adds * size + half_step(want, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [8, 9])
+@pytest.mark.parametrize("tokens,empty", [(300, 1 << 22), (1, 1 << 22), (40000, 70000), (300, 0)])
+def test_more_empty_sequences_than_tokens(tokens, empty, D):
+    """A table of one-token sequences with a run of empty ones in its middle: states pass through, outputs are those without the run, and
+    the call's time does not go by the run's length one sequence after the other (a third of a second, of which a wait bears one)."""
+    gen = torch.Generator().manual_seed(5)
+    x, g = (torch.randn(1, tokens, D, generator=gen).to(DEV) for _ in range(2))
+    g = -g.abs()
+    head = tokens // 2
+    off = torch.cat([torch.arange(head + 1), torch.full((empty,), head), torch.arange(head + 1, tokens + 1)]).to(torch.int32).to(DEV)
+    N = tokens + empty
+    h0, dht = (torch.randn(N, D, device=DEV, generator=torch.Generator(DEV).manual_seed(i)) for i in range(2))
+    full = torch.ones(N, dtype=torch.bool, device=DEV)
+    full[head:head + empty] = False
+    xs, gs, hs = (v.requires_grad_(True) for v in (x, g, h0))
+    o, ht = chunk_hgrn(xs, gs, initial_state=hs, output_final_state=True, offsets=off)
+    grads = torch.autograd.grad([o, ht], [xs, gs, hs], [torch.ones_like(o), dht])
+    few = h0.detach()[full].requires_grad_(True)
+    dense = torch.arange(tokens + 1, dtype=torch.int32, device=DEV)
+    o2, ht2 = chunk_hgrn(xs, gs, initial_state=few, output_final_state=True, offsets=dense)
+    want = torch.autograd.grad([o2, ht2], [xs, gs, few], [torch.ones_like(o2), dht[full]])
+    assert torch.equal(o, o2) and torch.equal(ht[full], ht2) and torch.equal(ht[~full], h0[~full])
+    assert torch.equal(grads[0], want[0]) and torch.equal(grads[1], want[1])
+    assert torch.equal(grads[2][full], want[2]) and torch.equal(grads[2][~full], dht[~full])
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    chunk_hgrn(x.detach(), g.detach(), initial_state=h0.detach(), output_final_state=True, offsets=off)
+    end.record()
+    torch.cuda.synchronize()
+    assert begin.elapsed_time(end) < 100
+    assert _lib.load().flab_tc_error_state() == 0
