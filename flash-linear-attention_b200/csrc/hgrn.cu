@@ -17,10 +17,12 @@
 // tiles whose blocks already run; one launch then reads everything once, where a two-pass scan would read the inputs twice.
 // Three forms: rows that TMA can address stream through a persistent block (hgrn_stream_kernel), others go tile by tile through
 // registers (hgrn_tile_kernel), and a few tokens a sequence are walked by one thread a channel group (hgrn_step_kernel).
-// Measured against the bytes above at the copy rate of 6.55 TB/s, bf16: [8, 4096, 2048] forward 68 us (91 %), backward 107 us (96 %);
-// [1, 262144, 2048] forward 548 us (90 %), backward 872 us (94 %): 32 channel groups side by side, where a tile's wait for the maps
-// of the tiles before it is what the stages no longer cover whole ([1, 262144, 1024] 310 and 480 us, 79 and 85 %); 64 packed
-// sequences of 290000 tokens 660 and 987 us (82 and 92 %); one token of 256 x 2048 2.5 us.
+// Measured against the bytes above at the copy rate of 6.55 TB/s, bf16: [8, 4096, 2048] forward 68 us (91 %), backward 107 us (96 %), in fp32
+// 131 and 215 us with their launches (94 and 95 %); [1, 262144, 2048] forward 548 us (90 %), backward 872 us (94 %): 32 channel groups side
+// by side, where a tile's wait for the maps of the tiles before it is what the stages no longer cover whole ([1, 262144, 1024] 310 and
+// 480 us, 79 and 85 %; [1, 65536, 512] 55 and 83, 56 and 62 %); 64 packed sequences of 295926 tokens with their states 679 and 1044 us with
+// the launches (82 and 89 %); one token of 256 x 2048 2.5 us.  Rows that TMA cannot address: [8, 4096, 2047] 267 and 288 us (23 and 36 %),
+// loads of one element; the backward of that form spills 12 to 52 bytes a thread.
 // All arithmetic and every state is fp32; o, dx, dg are rounded once, when stored.  Backward takes h_{t-1} from the stored o:
 // dg is a plain product with it, so the 16-bit rounding of o enters dg once, with the size of dg's own rounding, and backward
 // needs neither x nor a second forward scan.

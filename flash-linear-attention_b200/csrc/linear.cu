@@ -4,8 +4,10 @@
 //   backward:  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum over rows of dz;  dr = dy
 // One tcgen05 kernel computes all three products, C[m, n] = sum_k A(m, k) B(n, k), with either operand stored row by row
 // (K-major) or column by column (MN-major: W in dx, dz and x in dW), so nothing is transposed in memory.  Accumulation fp32 in TMEM;
-// the epilogue is fp32 and rounds once.  z is kept for backward in the type of x (one rounding of the argument of act', whose effect
-// is below the rounding of dz), and dz is rounded to that type because it is an operand of both products.
+// the epilogue is fp32 and rounds once.  z is kept for backward in the type of x, and dz is rounded to that type because it is an operand
+// of both products.  The rounding of z moves a slope by up to |act''| |z| eps / 2: below dz's own rounding where the slope is near 1,
+// above it where the slope is small (in the tails of the two sigmoids |z| times it, 8 times at z = 8; near a zero of silu's or gelu's slope
+// without bound, relative to it).  It halves the bytes of what is kept; gradients are 2.4e-3 off the 64-bit ones where fp32 would give 1.7e-3.
 //
 // Layout: a pair of CTAs works on a 256 x BN tile (cta_group::2), each CTA loading its 128 rows of A and its half of B, S stages of
 // 128-byte rows by TMA; the accumulator is double buffered in TMEM so that a tile's epilogue runs under the next tile's products.
@@ -13,10 +15,12 @@
 // residual comes in the same way, a block ahead.  Outputs whose rows do not begin on 16-byte boundaries go through a transposition in
 // shared memory instead, so that a warp reads and writes runs of 64 bytes.  Tiles go in groups of 8 rows of tiles, so that what the
 // pairs work on at one time shares operands in L2.
-// Measured, bf16, 32768 x 2048 x 2048: product alone 184 us (1490 TFLOP/s; the library's 180), with silu, bias and residual 194 us, dx
-// 183, dW 186 us; 8192 x 8192 x 8192 706 us (1558 TFLOP/s; the library's 663).  e4m3, 32768 x 2048 x 2048 with scales 105 us (2620
-// TFLOP/s), with silu 121 us.  Bound by the tensor pipe under the power cap (88 to 93 % active without an epilogue, 83 % with
-// one); 256 x 2048 x 2048 takes 12.2 us, the loop over 32 blocks.
+// Measured, bf16, 32768 x 2048 x 2048: product alone 183 us (1499 TFLOP/s; the library's 179), with silu, bias and residual 194 us, dx
+// 181, dW 185 us (the library's 179); 8192 x 8192 x 8192 706 to 736 us by box (the library's 649 to 663), dx 858 to 870, dW 860 (757 to
+// 815).  e4m3, 32768 x 2048 x 2048 with scales 105 to 108 us, with silu 121 to 135.  Bound by the tensor pipe under the power cap (88 to
+// 93 % active without an epilogue, 83 % with one).  256 x 2048 x 2048 takes 12.0 us (the library's 5.1): one row of tiles, so 64 of 148
+// SMs, each bound by what it can take in from L2; 16 x 2048 x 8192 16.4 us (5.6), where most of a tile is rows that are not there.
+// The forward epilogue without tile stores spills 52 to 136 bytes a thread.
 #include <type_traits>
 
 #include "tc.cuh"
