@@ -967,10 +967,11 @@ template <typename T, bool BWD> int dispatch_hgrn(const HgrnParams &p, void *ws,
     tma = tma && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   }
   for (const float *q : {p.h0, p.dht, (const float *)p.ht}) tma = tma && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  // The streaming form walks all sequences that lie in a tile, 32 in 0.5 us, and a million empty ones may lie in one; more of them go by the
-  // tile form, which searches for each row's.  (A run of 4 million took 350 ms; past them in steps that double, the code that does it
-  // cost every packed call 2 %.)
-  if (p.cu && p.N > 1 << 20) tma = false;
+  // The streaming form walks all sequences that lie in a tile, 32 in half a microsecond, and all of the table may lie in one (empty ones):
+  // some 50 ms for 4 million, of the second that a wait bears.  Larger tables go by the tile form, which searches for each row's sequence:
+  // 2 million sequences of two tokens, 64 channels, take it 5.3 ms where the streaming form takes 2.7.  (Past runs of empty ones in steps
+  // that double, the code that does it cost every packed call 2 %.)
+  if (p.cu && p.N > 1 << 22) tma = false;
   constexpr int WIDE = 16 / sizeof(T);
   bool wide = tma && p.D % WIDE == 0;
   for (const float *q : {p.h0, p.dht, (const float *)p.ht}) {
