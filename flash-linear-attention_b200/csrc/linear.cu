@@ -16,7 +16,7 @@
 // shared memory instead, so that a warp reads and writes runs of 64 bytes.  Tiles go in groups of 8 rows of tiles, so that what the
 // pairs work on at one time shares operands in L2.
 // Measured, bf16, 32768 x 2048 x 2048: product alone 183 us (1499 TFLOP/s; the library's 179), with silu, bias and residual 194 us, dx
-// 181, dW 185 us (the library's 179); 8192 x 8192 x 8192 706 to 736 us by box (the library's 649 to 663), dx 858 to 870, dW 860 (757 to
+// 181, dW 185 us (the library's 179); 8192 x 8192 x 8192 706 to 736 us by card (the library's 649 to 663), dx 858 to 870, dW 860 (757 to
 // 815).  e4m3, 32768 x 2048 x 2048 with scales 105 to 108 us, with silu 121 to 135.  Bound by the tensor pipe under the power cap (88 to
 // 93 % active without an epilogue, 83 % with one).  256 x 2048 x 2048 takes 12.0 us (the library's 5.1): one row of tiles, so 64 of 148
 // SMs, each bound by what it can take in from L2; 16 x 2048 x 8192 16.4 us (5.6), where most of a tile is rows that are not there.
